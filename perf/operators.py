@@ -307,7 +307,7 @@ def _plain_gemv(s):
 
 
 def _plain_rows(s):
-    """Queries and keys behind norm and rotation in 64 bits: the keys' codes are decided from them."""
+    """Queries and keys behind norm and rotation, in 64 bits: the keys are rounded once, to 32, before their codes are decided."""
     case = s["case"]
     hq, hkv, hd = case["hq"], case["hkv"], case["hd"]
     rows = s["qkv"][:, :(hq + 2 * hkv) * hd].double().unflatten(1, (-1, hd))
@@ -328,7 +328,7 @@ def _plain_append(s):
     hd, group = case["hd"], case["group"]
     q, k, v = _plain_rows(s)
     page, slot = s["table"][s["seq"].long(), s["pos"].long() // PAGE].long(), s["pos"].long() % PAGE
-    kcode, kpair = _quantise(k, group)
+    kcode, kpair = _quantise(k.float().double(), group)
     vcode, vpair = _quantise(v, group)
     kb, vb = _pack(kcode, vcode, hd, slot[:, None])
     kc, ks, vc, vs = _views(s["pages"], hd, group)
@@ -510,4 +510,4 @@ def exact(case, seed):
     if case["kind"] == "rope":
         return [q.flatten(1), k.flatten(1)]
     v = s["qkv"][:, (hq + hkv) * hd:(hq + 2 * hkv) * hd].double().reshape(-1, hkv, hd)
-    return [q.flatten(1), _exact_held(k, case["group"]), _exact_held(v, case["group"])]
+    return [q.flatten(1), _exact_held(k.float().double(), case["group"]), _exact_held(v, case["group"])]
