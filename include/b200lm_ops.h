@@ -5,7 +5,9 @@
  * (runtime/executor/llm_litert_compiled_model_executor.cc:271,407,522), so these
  * entry points have no one-to-one reference symbol; each names the step of
  * that opaque graph it stands for.  They exist for the operator parity tests
- * and for the attention / GEMM micro-benchmarks.  All pointers are HOST
+ * and for the attention / GEMM micro-benchmarks; those on device memory (the
+ * decode attention without allocations and what follows it) are also for use in
+ * a serving loop of one's own.  All pointers are HOST
  * memory unless a name says "dev"; the calls copy in, run the kernel, copy out.
  * Same status-code and error-string conventions as b200lm.h.
  */
@@ -138,6 +140,138 @@ int B200LmOps_AttentionDecodeStaticClusters(int32_t device, int32_t batch, int32
  * DeadlineExceeded when a bounded device-side wait gave up; *device_error
  * (optional) receives the raw word.  No counterpart in the reference. */
 int B200LmOps_AttentionDecodeStaticStatus(int32_t device, void* stream, int32_t* device_error, char** err);
+
+/* ---------------------------------------------------------------------------
+ * Operators over caller-owned DEVICE memory: int4 products with group scales,
+ * QK norm with rotation, and a cache held in 4 bits with the attention over it.
+ * The reference has no counterpart.  Common to all of them:
+ *   - arguments ending in _dev are device memory of `device`; arguments are
+ *     checked on the host first, on failure nothing has been queued.  Work goes
+ *     to `stream` (NULL: the default stream), the call returns without waiting,
+ *     allocates nothing, keeps no state and may be captured into a CUDA graph
+ *     (the first call of a kind on a device raises kernel attributes: make it
+ *     before the capture).  The caller's current device is left as it was.
+ *   - element types are B200LM_F32, B200LM_BF16, B200LM_F16; strides count
+ *     elements.  Rows need no more alignment than their type's.  Inputs and
+ *     outputs do not overlap unless said so.
+ *   - status_dev (may be NULL) is a word of the caller's, zero at first, to which
+ *     the kernels add what only they can see: a position or a length outside the
+ *     cache, the page table or the rotation table, a page number outside the
+ *     pool.  What such a token or sequence would have written stays as it was;
+ *     the others are served.  B200LmOps_DeviceStatus reads the word. */
+#define B200LM_F32 0
+#define B200LM_BF16 1
+#define B200LM_F16 2
+
+/* Waits for `stream`, then reads and clears *status_dev.  OK when the word was
+ * zero, InvalidArgument for a bad position, length or page, DeadlineExceeded when
+ * a bounded device-side wait gave up; *device_error (optional) receives the word. */
+int B200LmOps_DeviceStatus(int32_t device, void* stream, int32_t* status_dev, int32_t* device_error, char** err);
+
+/* Weights of a grouped int4 product, laid out once on the host.  packed as above
+ * ([n][k/2], two's complement, k even), scale and offset (NULL: none)
+ * [n][ceil(k/group)] as 16-bit words, fp16 or bf16.  The image is made of strips
+ * of 16 rows and, in a strip, blocks of 128 k; rows and k past the end are zero.
+ * A block is two tiles of 64 k of the W4T layout (512 bytes each), then the scales
+ * [8][128/group][2] of the rows g and g + 8, then the offsets likewise.
+ * GemvW4GroupedBytes gives the image's size. */
+int B200LmOps_GemvW4GroupedBytes(int64_t n, int64_t k, int32_t group, int32_t has_offset, int64_t* bytes, char** err);
+int B200LmOps_RepackW4Grouped(const uint8_t* packed, const uint16_t* scale, const uint16_t* offset, int64_t n, int64_t k,
+                              int32_t group, uint8_t* out, char** err);
+
+/* y[c][r] = sum over the groups g of k of
+ *   scale[r][g] * sum_{j in g} q[r][j] x[c][j]  +  offset[r][g] * sum_{j in g} x[c][j]
+ * for ncols = 1 .. 8 columns x [ncols] rows of ldx, y [ncols] rows of ldy.  group is
+ * 32, 64 or 128 (the last group may be shorter), scale_type B200LM_BF16 or _F16.
+ * w_dev is the image above, on a 16-byte boundary.  The sums are exact to fp32
+ * whatever x's type; an infinity or NaN in a column makes all of its outputs NaN. */
+int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_type, int32_t has_offset, int64_t n, int64_t k,
+                            int32_t group, const void* x_dev, int32_t x_type, int64_t ldx, int32_t ncols, void* y_dev,
+                            int32_t y_type, int64_t ldy, void* stream, char** err);
+
+/* RMSNorm of every query and key head (gains q_gain_dev, k_gain_dev [hd] fp32;
+ * NULL: no norm) and the rotation of its first `rot` elements, element i paired
+ * with i + rot/2, by row pos_dev[t] of cos_dev, sin_dev [rope_rows][rot/2] fp32.
+ * qkv_dev holds `tokens` rows of qkv_stride elements, the layout of a fused QKV
+ * projection: hq query heads, hkv key heads, hkv value heads.  Queries go to
+ * q_out_dev [tokens] rows of q_stride, keys to k_out_dev rows of k_stride, in
+ * qkv's type; they may be the rows' own places.  hd is 64, 128 or 256, rot a
+ * multiple of hd/16 up to hd (0: no rotation; cos_dev and sin_dev are not read).
+ * A token with a negative position is padding: its rows are left alone. */
+int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens, int32_t hq,
+                         int32_t hkv, int32_t hd, int32_t rot, const float* q_gain_dev, const float* k_gain_dev, float eps,
+                         const float* cos_dev, const float* sin_dev, int32_t rope_rows, const int32_t* pos_dev,
+                         void* q_out_dev, int64_t q_stride, void* k_out_dev, int64_t k_stride, int32_t* status_dev,
+                         void* stream, char** err);
+
+/* A paged cache in 4 bits.  For each page and kv head lie, in this order, the K
+ * codes, K scales, V codes and V scales of 256 positions.  A row of hd elements is
+ * cut into groups of 64 or 128; of each group are kept m = its lowest value,
+ * s = (highest - lowest) / 15, both rounded to fp16 (rounded to fp32 before, and
+ * held within the fp16 range), and a code of 4 bits for each element,
+ * c = rint((x - m) / s) held to 0 .. 15, which stands for s c + m.  A group with an
+ * infinity or NaN stands for NaN.
+ * Scales are [256][hd/group] pairs (s, m).  Codes lie in planes of 128 elements
+ * (64 at hd 64), [plane][256] rows of 64 (32) bytes.  In a K row byte
+ * w t + 4 j + i (t, i < 4; w = 16 or 8) holds the elements 32 j + 4 t + i (low
+ * nibble) and 16 more (high).  In a V row byte b of unit g (8 units of 8 or 4
+ * bytes) holds the elements 16 b + g and 8 more; where planes are 128 wide the
+ * units of positions with bit 1 set lie four further, modulo eight.
+ * page_table_dev [batch] rows of table_stride: physical page of each logical page
+ * of 256 positions.  pages_dev on a 16-byte boundary. */
+typedef struct B200LmKv4Cache {
+  int32_t struct_size;           /* sizeof(B200LmKv4Cache) */
+  int32_t batch;                 /* sequences (rows of the page table) */
+  int32_t hkv, hd, group;
+  int32_t reserved;              /* 0 */
+  void* pages_dev;
+  int64_t num_pages;
+  const int32_t* page_table_dev;
+  int64_t table_stride;          /* logical pages of a sequence */
+} B200LmKv4Cache;
+
+/* Bytes of one page: 512 * hkv * (hd/2 + 4 * hd/group). */
+int B200LmOps_Kv4PageBytes(int32_t hkv, int32_t hd, int32_t group, int64_t* bytes, char** err);
+
+/* QkNormRope whose keys, with the value heads of the rows, go into the cache: token
+ * t is position pos_dev[t] of sequence seq_dev[t] (NULL: sequence t).  Norm and
+ * rotation of the keys are computed in fp64 and rounded to fp32, so that codes do
+ * not depend on the order of sums.  No two tokens of a call may share a position. */
+int B200LmOps_QkNormRopeAppendKv4(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens,
+                                  int32_t hq, int32_t hkv, int32_t hd, int32_t rot, const float* q_gain_dev,
+                                  const float* k_gain_dev, float eps, const float* cos_dev, const float* sin_dev,
+                                  int32_t rope_rows, const int32_t* pos_dev, void* q_out_dev, int64_t q_stride,
+                                  const B200LmKv4Cache* cache, const int32_t* seq_dev, int32_t* status_dev, void* stream,
+                                  char** err);
+
+/* The values that cached positions stand for: rows pos_dev[t] of sequences
+ * seq_dev[t] (NULL: sequence t), k_out_dev and v_out_dev [tokens][hkv][hd] of
+ * out_type (either may be NULL).  Negative positions are padding. */
+int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, const int32_t* seq_dev, const int32_t* pos_dev,
+                      int32_t tokens, int32_t out_type, void* k_out_dev, void* v_out_dev, int32_t* status_dev, void* stream,
+                      char** err);
+
+/* softmax(scale q K^T) V over the cache.  q_dev holds the query tokens of all
+ * sequences one behind the other, `tokens` rows of q_stride elements with hq heads
+ * of hd first; sequence b has the rows q_start_dev[b] .. q_start_dev[b + 1] - 1
+ * (NULL: one row each), at most max_q of them.  kv_len_dev[b] positions of it are
+ * cached, the query tokens being the last of them: token i of n sits at position
+ * kv_len - n + i, sees the positions up to its own and, with window > 0, the last
+ * `window` of those.  A row that sees none gives zeros.  kv_len_dev[b] is at most
+ * max_kv, max_kv at most 256 * table_stride.  scale <= 0 means 1/sqrt(hd).  out_dev
+ * is of q's type; rows behind the last sequence's are left as they were.
+ *
+ * workspace_dev (16-byte boundary; NULL where AttentionKv4Workspace says 0) holds the
+ * partial results of sequences whose keys are shared out.  Zero it once before its
+ * first use; every call leaves the part that has to be zero at zero.  It serves one
+ * call at a time: calls, or replays of captured ones, that may overlap need
+ * workspaces of their own. */
+int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, int32_t hkv, int32_t hd, int32_t hq, int32_t max_q,
+                                    int32_t max_kv, int64_t* bytes, char** err);
+int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cache, const void* q_dev, int32_t q_type, int64_t q_stride,
+                           const int32_t* kv_len_dev, const int32_t* q_start_dev, int32_t tokens, int32_t max_q,
+                           int32_t max_kv, int32_t hq, int32_t window, float scale, void* out_dev, int64_t out_stride,
+                           void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev, void* stream, char** err);
 
 #ifdef __cplusplus
 }

@@ -51,6 +51,31 @@ class B200LmConfig(C.Structure):
                 ("tp_rank", C.c_int32), ("tp_world", C.c_int32), ("tp_unique_id", C.c_void_p)]
 
 
+class B200LmKv4Cache(C.Structure):
+    _fields_ = [("struct_size", C.c_int32), ("batch", C.c_int32), ("hkv", C.c_int32), ("hd", C.c_int32), ("group", C.c_int32),
+                ("reserved", C.c_int32), ("pages_dev", C.c_void_p), ("num_pages", C.c_int64), ("page_table_dev", C.c_void_p),
+                ("table_stride", C.c_int64)]
+
+
+class Kv4Cache:
+    """A paged cache in 4 bits in the caller's device memory (raw addresses): pages of ``page_bytes()`` each and a page
+    table [batch][table_stride].  The memory has to outlive the calls that it is passed to."""
+
+    __slots__ = ("desc", "ref")
+
+    def __init__(self, pages_dev: int, num_pages: int, page_table_dev: int, table_stride: int, batch: int, hkv: int, hd: int,
+                 group: int = 64) -> None:
+        self.desc = B200LmKv4Cache(C.sizeof(B200LmKv4Cache), batch, hkv, hd, group, 0, pages_dev, num_pages, page_table_dev,
+                                   table_stride)
+        self.ref = C.byref(self.desc)
+
+    @staticmethod
+    def page_bytes(hkv: int, hd: int, group: int = 64) -> int:
+        n = C.c_int64()
+        _call("B200LmOps_Kv4PageBytes", hkv, hd, group, C.byref(n))
+        return n.value
+
+
 _lib: Optional[C.CDLL] = None
 
 _EXEC_SYMBOLS = ["B200Lm_Create", "B200Lm_CreateShared", "B200Lm_Destroy", "B200Lm_Prefill", "B200Lm_DecodeLogits",
@@ -61,7 +86,13 @@ _EXEC_SYMBOLS = ["B200Lm_Create", "B200Lm_CreateShared", "B200Lm_Destroy", "B200
 _OPS_SYMBOLS = ["B200LmOps_RepackW4T", "B200LmOps_RepackW4G", "B200LmOps_UnpackW4", "B200LmOps_GemvW4",
                 "B200LmOps_GemmW4", "B200LmOps_GemmGegluW4", "B200LmOps_Attention", "B200LmOps_AttentionPrefillTc",
                 "B200LmOps_AttentionDecodeStatic", "B200LmOps_AttentionDecodeStaticStatus",
-                "B200LmOps_AttentionDecodeStaticClusters"]
+                "B200LmOps_AttentionDecodeStaticClusters", "B200LmOps_DeviceStatus", "B200LmOps_GemvW4GroupedBytes",
+                "B200LmOps_RepackW4Grouped", "B200LmOps_GemvW4Grouped", "B200LmOps_QkNormRope",
+                "B200LmOps_QkNormRopeAppendKv4", "B200LmOps_Kv4PageBytes", "B200LmOps_Kv4Read",
+                "B200LmOps_AttentionKv4Workspace", "B200LmOps_AttentionKv4"]
+
+# element types of the operators over device memory
+F32, BF16, F16 = 0, 1, 2
 
 
 def load_library() -> C.CDLL:
@@ -73,8 +104,9 @@ def load_library() -> C.CDLL:
         raise RuntimeError(f"{LIB_PATH} is missing: build it with `python litert-lm_b200/build.py` "
                            "(there is no CPU fallback)")
     lib = C.CDLL(LIB_PATH)
-    vp, i32, i64, u64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64
+    vp, i32, i64, u64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
     errp = C.POINTER(C.c_char_p)
+    rows = [i32, vp, i32, i64, i32, i32, i32, i32, i32, vp, vp, f32, vp, vp, i32, vp, vp, i64]
     sig = {
         "B200Lm_Create": [C.POINTER(B200LmConfig), vp, u64, C.c_char_p, C.POINTER(vp), errp],
         "B200Lm_CreateShared": [vp, C.POINTER(B200LmConfig), C.POINTER(vp), errp],
@@ -109,6 +141,16 @@ def load_library() -> C.CDLL:
         "B200LmOps_AttentionDecodeStatic": [i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, errp],
         "B200LmOps_AttentionDecodeStaticStatus": [i32, vp, vp, errp],
         "B200LmOps_AttentionDecodeStaticClusters": [i32] * 8 + [vp, errp],
+        "B200LmOps_DeviceStatus": [i32, vp, vp, vp, errp],
+        "B200LmOps_GemvW4GroupedBytes": [i64, i64, i32, i32, vp, errp],
+        "B200LmOps_RepackW4Grouped": [vp, vp, vp, i64, i64, i32, vp, errp],
+        "B200LmOps_GemvW4Grouped": [i32, vp, i32, i32, i64, i64, i32, vp, i32, i64, i32, vp, i32, i64, vp, errp],
+        "B200LmOps_QkNormRope": rows + [vp, i64, vp, vp, errp],
+        "B200LmOps_QkNormRopeAppendKv4": rows + [vp, vp, vp, vp, errp],
+        "B200LmOps_Kv4PageBytes": [i32, i32, i32, vp, errp],
+        "B200LmOps_Kv4Read": [i32, vp, vp, vp, i32, i32, vp, vp, vp, vp, errp],
+        "B200LmOps_AttentionKv4Workspace": [i32] * 7 + [vp, errp],
+        "B200LmOps_AttentionKv4": [i32, vp, vp, i32, i64, vp, vp, i32, i32, i32, i32, i32, f32, vp, i64, vp, i64, vp, vp, errp],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -437,3 +479,99 @@ class ops:
         word = C.c_int32(-1)
         _call("B200LmOps_AttentionDecodeStaticStatus", device, C.c_void_p(stream) if stream else None, C.byref(word))
         return word.value
+
+    # -- operators over device memory: int4 products with group scales, QK norm + rotation, the cache in 4 bits.  Addresses
+    # -- are raw (0: null) and go straight through, as these are called once per layer and step.
+    @staticmethod
+    def device_status(status_dev: int, stream: int = 0, device: int = 0) -> int:
+        """Waits for `stream`, reads and clears the status word; 0 = clean, raises StatusError when it is set."""
+        word = C.c_int32(-1)
+        _call("B200LmOps_DeviceStatus", device, stream or None, status_dev, C.byref(word))
+        return word.value
+
+    @staticmethod
+    def repack_w4_grouped(packed: np.ndarray, scale: np.ndarray, offset: Optional[np.ndarray] = None, group: int = 64) -> np.ndarray:
+        """Host-only: [n][k/2] nibbles and [n][ceil(k/group)] scales (and offsets), fp16 or bf16 as any 2-byte dtype, as
+        the image that `gemv_w4_grouped` reads."""
+        packed = np.ascontiguousarray(packed, dtype=np.uint8)
+        n, k = packed.shape[0], packed.shape[1] * 2
+        words = []
+        for a in (scale, offset):
+            if a is not None:
+                a = np.ascontiguousarray(a)
+                if a.dtype.itemsize != 2 or a.shape != (n, -(-k // max(group, 1))):
+                    raise StatusError(INVALID_ARGUMENT, "scales and offsets: [n][ceil(k/group)] of a 2-byte type")
+            words.append(a)
+        size = C.c_int64()
+        _call("B200LmOps_GemvW4GroupedBytes", n, k, group, int(offset is not None), C.byref(size))
+        out = np.empty(size.value, dtype=np.uint8)
+        _call("B200LmOps_RepackW4Grouped", _ptr(packed), _ptr(words[0]), _ptr(words[1]) if offset is not None else None, n, k, group,
+              _ptr(out))
+        return out
+
+    @staticmethod
+    def gemv_w4_grouped(w_dev: int, x_dev: int, y_dev: int, n: int, k: int, group: int, ncols: int = 1, x_type: int = F32,
+                        y_type: int = F32, scale_type: int = F16, has_offset: bool = False, ldx: int = 0, ldy: int = 0,
+                        stream: int = 0, device: int = 0) -> None:
+        """y[c] = W x[c] for 1 .. 8 columns, W int4 with a scale (and offset) for each group of k; rows of x and y are ldx
+        and ldy elements apart (0: k and n)."""
+        err = C.c_char_p()
+        code = (_lib or load_library()).B200LmOps_GemvW4Grouped(
+            device, w_dev, scale_type, has_offset, n, k, group, x_dev, x_type, ldx or k, ncols, y_dev, y_type, ldy or n, stream or None,
+            C.byref(err))
+        if code != OK:
+            _check(code, err)
+
+    @staticmethod
+    def qk_norm_rope(qkv_dev: int, type: int, qkv_stride: int, tokens: int, hq: int, hkv: int, hd: int, rot: int, q_gain_dev: int,
+                     k_gain_dev: int, eps: float, cos_dev: int, sin_dev: int, rope_rows: int, pos_dev: int, q_out_dev: int, q_stride: int,
+                     k_out_dev: int, k_stride: int, status_dev: int = 0, stream: int = 0, device: int = 0) -> None:
+        """RMSNorm of each query and key head and the rotation, in one pass over rows of a fused QKV projection."""
+        err = C.c_char_p()
+        code = (_lib or load_library()).B200LmOps_QkNormRope(
+            device, qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev,
+            q_out_dev, q_stride, k_out_dev, k_stride, status_dev, stream or None, C.byref(err))
+        if code != OK:
+            _check(code, err)
+
+    @staticmethod
+    def qk_norm_rope_append_kv4(qkv_dev: int, type: int, qkv_stride: int, tokens: int, hq: int, hkv: int, hd: int, rot: int,
+                                q_gain_dev: int, k_gain_dev: int, eps: float, cos_dev: int, sin_dev: int, rope_rows: int, pos_dev: int,
+                                q_out_dev: int, q_stride: int, cache: Kv4Cache, seq_dev: int = 0, status_dev: int = 0, stream: int = 0,
+                                device: int = 0) -> None:
+        """`qk_norm_rope` whose keys, with the rows' values, go into the cache in 4 bits."""
+        err = C.c_char_p()
+        code = (_lib or load_library()).B200LmOps_QkNormRopeAppendKv4(
+            device, qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev,
+            q_out_dev, q_stride, cache.ref, seq_dev, status_dev, stream or None, C.byref(err))
+        if code != OK:
+            _check(code, err)
+
+    @staticmethod
+    def kv4_read(cache: Kv4Cache, seq_dev: int, pos_dev: int, tokens: int, out_type: int, k_out_dev: int, v_out_dev: int,
+                 status_dev: int = 0, stream: int = 0, device: int = 0) -> None:
+        """The values that cached positions stand for, [tokens][hkv][hd]."""
+        err = C.c_char_p()
+        code = (_lib or load_library()).B200LmOps_Kv4Read(device, cache.ref, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev,
+                                                          status_dev, stream or None, C.byref(err))
+        if code != OK:
+            _check(code, err)
+
+    @staticmethod
+    def attention_kv4_workspace(batch: int, hkv: int, hd: int, hq: int, max_q: int, max_kv: int, device: int = 0) -> int:
+        """Bytes of workspace that `attention_kv4` needs for calls up to these sizes."""
+        n = C.c_int64()
+        _call("B200LmOps_AttentionKv4Workspace", device, batch, hkv, hd, hq, max_q, max_kv, C.byref(n))
+        return n.value
+
+    @staticmethod
+    def attention_kv4(cache: Kv4Cache, q_dev: int, q_type: int, q_stride: int, kv_len_dev: int, q_start_dev: int, tokens: int, max_q: int,
+                      max_kv: int, hq: int, out_dev: int, out_stride: int, workspace_dev: int = 0, workspace_bytes: int = 0,
+                      window: int = 0, scale: float = 0.0, status_dev: int = 0, stream: int = 0, device: int = 0) -> None:
+        """Attention of ragged sequences over the cache: causal, windowed, one query token a sequence or many."""
+        err = C.c_char_p()
+        code = (_lib or load_library()).B200LmOps_AttentionKv4(
+            device, cache.ref, q_dev, q_type, q_stride, kv_len_dev, q_start_dev, tokens, max_q, max_kv, hq, window, scale, out_dev, out_stride,
+            workspace_dev, workspace_bytes, status_dev, stream or None, C.byref(err))
+        if code != OK:
+            _check(code, err)

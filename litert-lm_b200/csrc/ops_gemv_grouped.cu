@@ -1,0 +1,132 @@
+// Entry points of the grouped int4 matrix-vector product (include/b200lm_ops.h).
+#include "../../include/b200lm_ops.h"
+#include "gemv_grouped.cuh"
+#include "op_host.h"
+
+#include <algorithm>
+#include <exception>
+
+namespace b200lm {
+
+static void check_grouped(int64_t n, int64_t k, int32_t group) {
+  B2_CHECK(n > 0 && n <= (1ll << 30) && k > 0 && k <= (1ll << 30) && k % 2 == 0, kInvalidArgument, "n, k: positive, at most 2^30, k even");
+  B2_CHECK(group == 32 || group == 64 || group == 128, kUnimplemented, "group must be 32, 64 or 128");
+}
+static int64_t grouped_block(int group, bool off) { return 1024 + 32 * (128 / group) * (off ? 2 : 1); }
+static int64_t grouped_bytes(int64_t n, int64_t k, int group, bool off) { return (n + 15) / 16 * ((k + 127) / 128) * grouped_block(group, off); }
+
+template <int GROUP, bool OFF, int NB>
+static void launch_gg(cudaStream_t st, GgArgs a, int sms) {
+  using S = GgShape<GROUP, OFF, NB>;
+  // Strips of a CTA and CTAs of a cluster: the fewest CTAs' rounds of blocks, then the fewest times that x is cut into digits.
+  a.rs = 8;
+  a.cs = 1;
+  while (a.rs > 1 && (a.strips + a.rs - 1) / a.rs < 2 * sms) a.rs /= 2;
+  while (a.cs < 8 && (a.strips + a.rs - 1) / a.rs * a.cs < 2 * sms && a.blocks / (a.cs * 2) >= 8 / a.rs) a.cs *= 2;
+  const int round = 8 / a.rs * S::kAhead, own = (a.blocks + a.cs - 1) / a.cs;
+  a.chunk = std::min(own, std::max(1, 64 / NB / round) * round);
+  const size_t smem = S::smem(a.chunk);
+  raise_dyn_smem(gemv_grouped_kernel<GROUP, OFF, NB>, S::smem(64 / NB > 8 * S::kAhead ? 64 / NB : 8 * S::kAhead));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.strips + a.rs - 1) / a.rs * a.cs));
+  cfg.blockDim = dim3(kGgThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)a.cs;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  B2_CUDA(cudaLaunchKernelEx(&cfg, gemv_grouped_kernel<GROUP, OFF, NB>, (const GgArgs)a));
+}
+
+template <int GROUP, bool OFF>
+static void launch_gg_cols(cudaStream_t st, const GgArgs& a, int sms) {
+  if (a.ncols <= 2) launch_gg<GROUP, OFF, 1>(st, a, sms);
+  else if (a.ncols <= 4) launch_gg<GROUP, OFF, 2>(st, a, sms);
+  else launch_gg<GROUP, OFF, 4>(st, a, sms);
+}
+
+}  // namespace b200lm
+
+using namespace b200lm;
+
+#define GG_TRY if (err) *err = nullptr; try {
+#define GG_END                                                                          \
+  return kOk; }                                                                         \
+  catch (const Error& e_) { return static_fail(err, e_.code, e_.msg); }                 \
+  catch (const std::exception& e_) { return static_fail(err, kInternal, e_.what()); }   \
+  catch (...) { return static_fail(err, kInternal, "unknown failure"); }
+
+extern "C" int B200LmOps_GemvW4GroupedBytes(int64_t n, int64_t k, int32_t group, int32_t has_offset, int64_t* bytes, char** err) {
+  GG_TRY
+  B2_CHECK(bytes, kInvalidArgument, "null pointer");
+  check_grouped(n, k, group);
+  *bytes = grouped_bytes(n, k, group, has_offset != 0);
+  GG_END
+}
+
+extern "C" int B200LmOps_RepackW4Grouped(const uint8_t* packed, const uint16_t* scale, const uint16_t* offset, int64_t n, int64_t k,
+                                         int32_t group, uint8_t* out, char** err) {
+  GG_TRY
+  B2_CHECK(packed && scale && out, kInvalidArgument, "null pointer");
+  check_grouped(n, k, group);
+  const int64_t blocks = (k + 127) / 128, bytes = grouped_block(group, offset != nullptr), groups = (k + group - 1) / group;
+  const int per = 128 / group;
+  memset(out, 0, (size_t)grouped_bytes(n, k, group, offset != nullptr));
+  for (int64_t r = 0; r < n; ++r) {
+    const int g = (int)(r % 8), high = (int)(r % 16 / 8);
+    uint8_t* strip = out + r / 16 * blocks * bytes;
+    for (int64_t j = 0; j < k; ++j) {
+      const int q = (packed[r * (k / 2) + j / 2] >> (4 * (j % 2))) & 15, c = (int)(j % 64);
+      uint8_t* tile = strip + j / 128 * bytes + j % 128 / 64 * 512;
+      tile[(4 * g + c % 16 / 4) * 16 + (2 * (c / 32) + c % 32 / 16) * 4 + c % 4] |= (uint8_t)(q << (4 * high));
+    }
+    for (int64_t j = 0; j < groups; ++j) {
+      uint8_t* at = strip + j / per * bytes + 1024 + ((g * per + j % per) * 2 + high) * 2;
+      memcpy(at, scale + r * groups + j, 2);
+      if (offset) memcpy(at + 32 * per, offset + r * groups + j, 2);
+    }
+  }
+  GG_END
+}
+
+extern "C" int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_type, int32_t has_offset, int64_t n, int64_t k,
+                                       int32_t group, const void* x_dev, int32_t x_type, int64_t ldx, int32_t ncols, void* y_dev,
+                                       int32_t y_type, int64_t ldy, void* stream, char** err) {
+  GG_TRY
+  B2_CHECK(w_dev && x_dev && y_dev, kInvalidArgument, "null pointer");
+  check_grouped(n, k, group);
+  B2_CHECK(scale_type == kBf16 || scale_type == kF16, kInvalidArgument, "scale_type must be B200LM_BF16 or B200LM_F16");
+  B2_CHECK(x_type >= kF32 && x_type <= kF16 && y_type >= kF32 && y_type <= kF16, kInvalidArgument, "unknown element type");
+  B2_CHECK(ncols >= 1 && ncols <= 8, kInvalidArgument, "ncols must be 1 .. 8");
+  B2_CHECK(ncols == 1 || (ldx >= k && ldy >= n), kInvalidArgument, "a row stride is shorter than its row");
+  B2_CHECK((uintptr_t)w_dev % 16 == 0, kInvalidArgument, "w_dev must lie on a 16-byte boundary");
+  B2_CHECK((uintptr_t)x_dev % elem_size(x_type) == 0 && (uintptr_t)y_dev % elem_size(y_type) == 0, kInvalidArgument, "x_dev or y_dev is misaligned");
+  B2_CHECK((n + 15) / 16 * 8 <= 0x7FFFFFFF, kInvalidArgument, "too many rows");
+  require_device(device);
+  DeviceScope scope(device);
+  GgArgs a{};
+  a.w = reinterpret_cast<const uint8_t*>(w_dev);
+  a.n = (int)n;
+  a.ncols = ncols;
+  a.strips = (int)((n + 15) / 16);
+  a.blocks = (int)((k + 127) / 128);
+  a.k = k;
+  a.x = x_dev;
+  a.ldx = ldx;
+  a.y = y_dev;
+  a.ldy = ldy;
+  a.x_type = x_type;
+  a.y_type = y_type;
+  a.scale_bf16 = scale_type == kBf16;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int sms = device_sms(device);
+  if (group == 32) has_offset ? launch_gg_cols<32, true>(st, a, sms) : launch_gg_cols<32, false>(st, a, sms);
+  else if (group == 64) has_offset ? launch_gg_cols<64, true>(st, a, sms) : launch_gg_cols<64, false>(st, a, sms);
+  else has_offset ? launch_gg_cols<128, true>(st, a, sms) : launch_gg_cols<128, false>(st, a, sms);
+  GG_END
+}

@@ -1,0 +1,245 @@
+// Entry points of the QK norm with rotation, of the cache in 4 bits and of the attention over it (include/b200lm_ops.h).
+#include "../../include/b200lm_ops.h"
+#include "kv4_attn.cuh"
+#include "kv4_rows.cuh"
+#include "op_host.h"
+
+#include <algorithm>
+#include <exception>
+
+namespace b200lm {
+
+static void check_heads(int hkv, int hd) {
+  B2_CHECK(hkv > 0 && hkv <= 1024, kInvalidArgument, "hkv must be 1 .. 1024");
+  B2_CHECK(hd == 64 || hd == 128 || hd == 256, kUnimplemented, "hd must be 64, 128 or 256");
+}
+static void check_group(int hd, int group) {
+  B2_CHECK((group == 64 || group == 128) && group <= hd, kUnimplemented, "group must be 64 or 128 and at most hd");
+}
+static void check_query_heads(int hq) { B2_CHECK(hq > 0 && hq <= 4096, kInvalidArgument, "hq must be 1 .. 4096"); }
+static void check_type(int type) { B2_CHECK(type >= kF32 && type <= kF16, kInvalidArgument, "unknown element type"); }
+static void check_pointer(const void* p, size_t align, const char* name) {
+  B2_CHECK(p, kInvalidArgument, std::string(name) + " is null");
+  B2_CHECK((uintptr_t)p % align == 0, kInvalidArgument, std::string(name) + " is misaligned");
+}
+static void check_optional(const void* p, size_t align, const char* name) {
+  if (p) check_pointer(p, align, name);
+}
+
+static Kv4Args cache_args(const B200LmKv4Cache* c) {
+  B2_CHECK(c, kInvalidArgument, "cache is null");
+  B2_CHECK(c->struct_size == (int32_t)sizeof(B200LmKv4Cache), kInvalidArgument, "cache: struct_size does not match this library");
+  B2_CHECK(c->reserved == 0, kInvalidArgument, "cache: reserved must be 0");
+  check_heads(c->hkv, c->hd);
+  check_group(c->hd, c->group);
+  B2_CHECK(c->batch > 0 && c->batch <= 65535, kInvalidArgument, "cache: batch must be 1 .. 65535");
+  B2_CHECK(c->num_pages > 0 && c->num_pages <= 0x7FFFFFFF, kInvalidArgument, "cache: num_pages out of range");
+  B2_CHECK(c->table_stride > 0 && c->table_stride <= 0x7FFFFFFF / kKv4Page, kInvalidArgument, "cache: table_stride out of range");
+  check_pointer(c->pages_dev, 16, "cache: pages_dev");
+  check_pointer(c->page_table_dev, 4, "cache: page_table_dev");
+  Kv4Args k{};
+  k.pages = reinterpret_cast<uint8_t*>(c->pages_dev);
+  k.num_pages = c->num_pages;
+  k.table = c->page_table_dev;
+  k.table_stride = c->table_stride;
+  k.batch = c->batch;
+  k.hkv = c->hkv;
+  k.d = Kv4Dims{c->hd, c->group};
+  return k;
+}
+
+// Rows of a call, checked; the caller adds where keys go.
+static RowArgs row_args(const void* qkv, int type, int64_t stride, int tokens, int hq, int hkv, int hd, int rot, const float* q_gain, const float* k_gain, float eps,
+                        const float* cos, const float* sin, int rope_rows, const int* pos, void* q_out, int64_t q_stride, int* status) {
+  check_type(type);
+  check_heads(hkv, hd);
+  check_query_heads(hq);
+  B2_CHECK(tokens >= 0, kInvalidArgument, "tokens is negative");
+  B2_CHECK(stride >= (int64_t)(hq + 2 * hkv) * hd && q_stride >= (int64_t)hq * hd, kInvalidArgument, "a row stride is shorter than its row");
+  B2_CHECK(rot >= 0 && rot <= hd && rot % (hd / 16) == 0, kInvalidArgument, "rot must be a multiple of hd / 16 up to hd");
+  B2_CHECK(eps >= 0.f, kInvalidArgument, "eps must not be negative");
+  check_pointer(qkv, elem_size(type), "qkv_dev");
+  check_pointer(q_out, elem_size(type), "q_out_dev");
+  check_pointer(pos, 4, "pos_dev");
+  check_optional(q_gain, 4, "q_gain_dev");
+  check_optional(k_gain, 4, "k_gain_dev");
+  check_optional(status, 4, "status_dev");
+  if (rot > 0) {
+    check_pointer(cos, 4, "cos_dev");
+    check_pointer(sin, 4, "sin_dev");
+    B2_CHECK(rope_rows > 0, kInvalidArgument, "rope_rows must be positive");
+  }
+  RowArgs a{};
+  a.qkv = qkv; a.stride = stride; a.type = type; a.tokens = tokens; a.hq = hq; a.hkv = hkv; a.rot = rot;
+  a.q_gain = q_gain; a.k_gain = k_gain; a.eps = eps; a.cos = cos; a.sin = sin; a.rope_rows = rope_rows; a.pos = pos;
+  a.q_out = q_out; a.q_stride = q_stride; a.status = status;
+  return a;
+}
+
+template <bool APPEND>
+static void launch_rows(cudaStream_t st, RowArgs a, int hd, int sms) {
+  const int heads = a.hq + (APPEND ? 2 : 1) * a.hkv;
+  // one head a warp while that does not fill the GPU, more where the token's rotation row would be read too often
+  a.heads_per_warp = 1;
+  while (a.heads_per_warp < 8 && (long long)a.tokens * heads / a.heads_per_warp > 64ll * sms) a.heads_per_warp *= 2;
+  const long long jobs = (long long)a.tokens * ((heads + a.heads_per_warp - 1) / a.heads_per_warp);
+  B2_CHECK((jobs + 3) / 4 <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
+  const dim3 grid((unsigned)((jobs + 3) / 4));
+  if (hd == 64) launch_pdl(qk_norm_rope_kernel<64, APPEND>, grid, dim3(128), 0, st, a);
+  else if (hd == 128) launch_pdl(qk_norm_rope_kernel<128, APPEND>, grid, dim3(128), 0, st, a);
+  else launch_pdl(qk_norm_rope_kernel<256, APPEND>, grid, dim3(128), 0, st, a);
+}
+
+}  // namespace b200lm
+
+using namespace b200lm;
+
+#define KV4_TRY if (err) *err = nullptr; try {
+#define KV4_END                                                                         \
+  return kOk; }                                                                         \
+  catch (const Error& e_) { return static_fail(err, e_.code, e_.msg); }                 \
+  catch (const std::exception& e_) { return static_fail(err, kInternal, e_.what()); }   \
+  catch (...) { return static_fail(err, kInternal, "unknown failure"); }
+
+extern "C" int B200LmOps_DeviceStatus(int32_t device, void* stream, int32_t* status_dev, int32_t* device_error, char** err) {
+  KV4_TRY
+  check_pointer(status_dev, 4, "status_dev");
+  require_device(device);
+  DeviceScope scope(device);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int word = 0;
+  B2_CUDA(cudaMemcpyAsync(&word, status_dev, sizeof(int), cudaMemcpyDeviceToHost, st));
+  B2_CUDA(cudaStreamSynchronize(st));
+  if (device_error) *device_error = word;
+  if (word != kDevOk) B2_CUDA(cudaMemsetAsync(status_dev, 0, sizeof(int), st));
+  if (word == kDevBadPosition) throw Error{kInvalidArgument, "a position, length or page lay outside its table"};
+  if (word == kDevBarrierTimeout) throw Error{kDeadlineExceeded, "a bounded device-side wait gave up"};
+  if (word != kDevOk) throw Error{kInternal, "device error word " + std::to_string(word)};
+  KV4_END
+}
+
+extern "C" int B200LmOps_Kv4PageBytes(int32_t hkv, int32_t hd, int32_t group, int64_t* bytes, char** err) {
+  KV4_TRY
+  B2_CHECK(bytes, kInvalidArgument, "null pointer");
+  check_heads(hkv, hd);
+  check_group(hd, group);
+  *bytes = (int64_t)hkv * Kv4Dims{hd, group}.head_bytes();
+  KV4_END
+}
+
+extern "C" int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens, int32_t hq,
+                                    int32_t hkv, int32_t hd, int32_t rot, const float* q_gain_dev, const float* k_gain_dev, float eps,
+                                    const float* cos_dev, const float* sin_dev, int32_t rope_rows, const int32_t* pos_dev,
+                                    void* q_out_dev, int64_t q_stride, void* k_out_dev, int64_t k_stride, int32_t* status_dev,
+                                    void* stream, char** err) {
+  KV4_TRY
+  RowArgs a = row_args(qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev, q_out_dev, q_stride, status_dev);
+  check_pointer(k_out_dev, elem_size(type), "k_out_dev");
+  B2_CHECK(k_stride >= (int64_t)hkv * hd, kInvalidArgument, "a row stride is shorter than its row");
+  a.k_out = k_out_dev;
+  a.k_stride = k_stride;
+  require_device(device);
+  if (tokens == 0) return kOk;
+  DeviceScope scope(device);
+  launch_rows<false>(reinterpret_cast<cudaStream_t>(stream), a, hd, device_sms(device));
+  KV4_END
+}
+
+extern "C" int B200LmOps_QkNormRopeAppendKv4(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens,
+                                             int32_t hq, int32_t hkv, int32_t hd, int32_t rot, const float* q_gain_dev,
+                                             const float* k_gain_dev, float eps, const float* cos_dev, const float* sin_dev,
+                                             int32_t rope_rows, const int32_t* pos_dev, void* q_out_dev, int64_t q_stride,
+                                             const B200LmKv4Cache* cache, const int32_t* seq_dev, int32_t* status_dev, void* stream,
+                                             char** err) {
+  KV4_TRY
+  RowArgs a = row_args(qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev, q_out_dev, q_stride, status_dev);
+  a.kv = cache_args(cache);
+  B2_CHECK(cache->hkv == hkv && cache->hd == hd, kInvalidArgument, "the cache's heads are not the rows'");
+  check_optional(seq_dev, 4, "seq_dev");
+  B2_CHECK(seq_dev || tokens <= cache->batch, kInvalidArgument, "more tokens than sequences: seq_dev says whose they are");
+  a.seq = seq_dev;
+  require_device(device);
+  if (tokens == 0) return kOk;
+  DeviceScope scope(device);
+  launch_rows<true>(reinterpret_cast<cudaStream_t>(stream), a, hd, device_sms(device));
+  KV4_END
+}
+
+extern "C" int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, const int32_t* seq_dev, const int32_t* pos_dev,
+                                 int32_t tokens, int32_t out_type, void* k_out_dev, void* v_out_dev, int32_t* status_dev, void* stream,
+                                 char** err) {
+  KV4_TRY
+  const Kv4Args kv = cache_args(cache);
+  check_type(out_type);
+  B2_CHECK(tokens >= 0, kInvalidArgument, "tokens is negative");
+  B2_CHECK(k_out_dev || v_out_dev, kInvalidArgument, "null pointer");
+  check_optional(k_out_dev, elem_size(out_type), "k_out_dev");
+  check_optional(v_out_dev, elem_size(out_type), "v_out_dev");
+  check_optional(seq_dev, 4, "seq_dev");
+  check_optional(status_dev, 4, "status_dev");
+  check_pointer(pos_dev, 4, "pos_dev");
+  B2_CHECK(seq_dev || tokens <= cache->batch, kInvalidArgument, "more tokens than sequences: seq_dev says whose they are");
+  const long long jobs = (long long)tokens * kv.hkv * ((k_out_dev != nullptr) + (v_out_dev != nullptr));
+  B2_CHECK((jobs + 3) / 4 <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
+  require_device(device);
+  if (tokens == 0) return kOk;
+  DeviceScope scope(device);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)((jobs + 3) / 4));
+  if (kv.d.hd == 64) launch_pdl(kv4_read_kernel<64>, grid, dim3(128), 0, st, kv, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev);
+  else if (kv.d.hd == 128) launch_pdl(kv4_read_kernel<128>, grid, dim3(128), 0, st, kv, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev);
+  else launch_pdl(kv4_read_kernel<256>, grid, dim3(128), 0, st, kv, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev);
+  KV4_END
+}
+
+static void check_attention(int batch, int hkv, int hd, int hq, int max_q, int max_kv) {
+  check_heads(hkv, hd);
+  check_query_heads(hq);
+  B2_CHECK(batch > 0 && batch <= 65535, kInvalidArgument, "batch must be 1 .. 65535");
+  B2_CHECK(hq % hkv == 0, kInvalidArgument, "hq must be a multiple of hkv");
+  B2_CHECK(max_q >= 1 && max_kv >= 0, kInvalidArgument, "max_q must be positive, max_kv not negative");
+}
+
+extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, int32_t hkv, int32_t hd, int32_t hq, int32_t max_q,
+                                               int32_t max_kv, int64_t* bytes, char** err) {
+  KV4_TRY
+  B2_CHECK(bytes, kInvalidArgument, "null pointer");
+  check_attention(batch, hkv, hd, hq, max_q, max_kv);
+  require_device(device);
+  *bytes = 0;
+  KV4_END
+}
+
+extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cache, const void* q_dev, int32_t q_type, int64_t q_stride,
+                                      const int32_t* kv_len_dev, const int32_t* q_start_dev, int32_t tokens, int32_t max_q,
+                                      int32_t max_kv, int32_t hq, int32_t window, float scale, void* out_dev, int64_t out_stride,
+                                      void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev, void* stream, char** err) {
+  KV4_TRY
+  Kv4AttnArgs a{};
+  a.kv = cache_args(cache);
+  check_attention(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv);
+  check_type(q_type);
+  B2_CHECK(tokens >= 0, kInvalidArgument, "tokens is negative");
+  B2_CHECK(q_start_dev || (tokens == cache->batch && max_q == 1), kInvalidArgument, "without q_start_dev every sequence has one token: tokens = batch, max_q = 1");
+  B2_CHECK(max_kv <= cache->table_stride * kKv4Page, kInvalidArgument, "max_kv is beyond the page table");
+  B2_CHECK(q_stride >= (int64_t)hq * cache->hd && out_stride >= (int64_t)hq * cache->hd, kInvalidArgument, "a row stride is shorter than its row");
+  check_pointer(q_dev, elem_size(q_type), "q_dev");
+  check_pointer(out_dev, elem_size(q_type), "out_dev");
+  check_pointer(kv_len_dev, 4, "kv_len_dev");
+  check_optional(q_start_dev, 4, "q_start_dev");
+  check_optional(status_dev, 4, "status_dev");
+  check_optional(workspace_dev, 16, "workspace_dev");
+  require_device(device);
+  if (tokens == 0) return kOk;
+  DeviceScope scope(device);
+  a.q = q_dev; a.q_type = q_type; a.q_stride = q_stride; a.kv_len = kv_len_dev; a.q_start = q_start_dev;
+  a.tokens = tokens; a.max_q = max_q; a.max_kv = max_kv; a.hq = hq; a.window = window;
+  a.qscale = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)cache->hd));
+  a.out = out_dev; a.out_stride = out_stride; a.status = status_dev;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)(max_q * hq), (unsigned)cache->batch);
+  if (cache->hd == 64) launch_pdl(kv4_attn_simple_kernel<64>, grid, dim3(256), 0, st, a);
+  else if (cache->hd == 128) launch_pdl(kv4_attn_simple_kernel<128>, grid, dim3(256), 0, st, a);
+  else launch_pdl(kv4_attn_simple_kernel<256>, grid, dim3(256), 0, st, a);
+  KV4_END
+}

@@ -15,10 +15,10 @@
 #include "attn_tc.cuh"
 #include "common.cuh"
 #include "decode_ops.cuh"
+#include "op_host.h"
 #include "page_map.h"
 #include "prefill_ops.cuh"
 
-#include <atomic>
 #include <mutex>
 
 namespace b200lm {
@@ -76,40 +76,6 @@ static StaticScratch static_scratch_for(int device) {
     s.base = reinterpret_cast<unsigned char*>(p);
   }
   return s;
-}
-
-// Makes `device` current for the duration of a call and puts the caller's device back afterwards.
-struct DeviceScope {
-  int prev = -1;
-  explicit DeviceScope(int device) {
-    if (cudaGetDevice(&prev) != cudaSuccess) { cudaGetLastError(); prev = -1; }
-    if (prev == device) prev = -1;            // already current: nothing to set, nothing to put back
-    else B2_CUDA(cudaSetDevice(device));
-  }
-  ~DeviceScope() {
-    if (prev >= 0) cudaSetDevice(prev);
-  }
-};
-
-static int static_fail(char** err, int code, const std::string& msg) {
-  if (err) {
-    *err = reinterpret_cast<char*>(malloc(msg.size() + 1));
-    if (*err) memcpy(*err, msg.c_str(), msg.size() + 1);
-  }
-  return code;
-}
-
-static void require_device(int device) {
-  static std::atomic<int> known{0};           // the count does not change while a process runs
-  int ndev = known.load(std::memory_order_relaxed);
-  if (ndev <= 0) {
-    if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev <= 0) {
-      cudaGetLastError();
-      throw Error{kFailedPrecondition, "no CUDA device: this backend has no CPU fallback"};
-    }
-    known.store(ndev, std::memory_order_relaxed);
-  }
-  B2_CHECK(device >= 0 && device < ndev, kInvalidArgument, "device ordinal out of range");
 }
 
 // Splits of a batch's queries whose partials the scratch holds.
