@@ -1,8 +1,26 @@
-// Attention of ragged sequences over the cache in 4 bits.
+// Attention of ragged sequences over the cache in 4 bits, for a few query rows of a kv head (head of its group x token).
 //
-// One CTA a query row (token and head): its warps take every eighth key, hold hd / 32 elements a lane, and meet at the end.
+//   S = scale q K^T,  K = s c + m per group of dims:   S = sum_g s_g (q . c)_g + sum_g m_g (sum of q over g)
+//   O = P V,          V = s c + m:                      O = sum_keys (P s_g) (c - 8) + sum_keys P (m_g + 8 s_g)
+//
+// The codes go from the cache into the A operands of mma.sync as they are, and the precision lies in the other operand:
+//   S  int8 products (m16n8k32, unsigned codes): a row of q is cut into four digits of seven bits below its largest power of
+//      two, the eight columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
+//   O  bf16 products (m16n8k16) with the codes as bf16 numbers c - 8 (exact) and P s in two bf16 terms (16-bit rows: 2^-17 of
+//      each weight) or three (fp32 rows, 2^-25).  Codes centred at zero keep the sums small; uncentred ones (16 + c, one
+//      instruction less for two codes) would cancel against their offset and lose five bits.  The tensor core cuts its sums off:
+//      fp32 rows take them out after every product, 16-bit rows at the end (at most 2^-24 an add).
+//
+// A warp walks its own tiles of keys (16 at head size 256, else 32) with a ring of its own that it fills by 16-byte asynchronous
+// copies: K and V rows lie in the cache in the order in which the fragments want them, so a lane's loads are 8 or 16 bytes
+// wide and free of bank conflicts.  Warps meet only at the end.  The softmax keeps a reference per row and warp that moves when a
+// score passes it by 8 powers of two, so that an ordinary tile takes one vote and no exchange of maxima.
+//
+// A CTA serves RB rows over a share of the keys; shares of a sequence are joined by the last CTA to arrive.  How many
+// keys a share has is decided on the host from the largest length, how many shares a sequence has on the device from its own.
 #pragma once
 #include "kv4_rows.cuh"
+#include "split_ticket.h"
 
 namespace b200lm {
 
@@ -17,64 +35,532 @@ struct Kv4AttnArgs {
   void* out;
   long long out_stride;
   int* status;
+  int row_tiles, share, splits;           // row tiles of a kv head, keys of a share, most shares of a sequence
+  unsigned* tickets;                      // one per (sequence, kv head, row tile), zero between calls
+  float* parts;                           // [unit][split][RB][HD + 2]: O, maximum, sum (negative: a page outside the pool)
 };
 
-template <int HD>
-__global__ void __launch_bounds__(256) kv4_attn_simple_kernel(const Kv4AttnArgs a) {
-  constexpr int V = HD / 32;
-  __shared__ float so[8][HD], sm[8], sl[8];
+constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps;
+constexpr int kKaTickets = 4096;          // words at the start of a workspace
+constexpr int kKaStages = 3;
+
+template <int HD, int GROUP, int RB, int TV>
+struct KaShape {
+  static constexpr int PL = HD < 128 ? HD : 128, P = HD / PL;        // plane, planes
+  static constexpr int ROW = PL / 2, NG = HD / GROUP;
+  static constexpr int NB = RB / 2;                                  // column blocks of S: two rows of four digits
+  static constexpr int CV = RB * TV, NBV = (CV + 7) / 8;             // columns of O, blocks of them
+  static constexpr int kCtas = HD / 16 * NBV * 4 > 64 ? 1 : 2;       // of an SM: O takes up to half of a thread's registers, or more
+  static constexpr int KT = HD == 256 ? 16 : 32, SUB = KT / 16, MT = HD / 16;
+  static constexpr int kCodes = KT * HD / 2, kScales = KT * NG * 4, kStage = 2 * (kCodes + kScales);
+  static constexpr int kRing = kKaWarps * kKaStages * kStage;
+  static constexpr int kDigits = HD / 64 * NB * 512;
+  static constexpr int kUnit = kRing + kDigits;                      // [RB], then the group sums [RB][NG]
+  static constexpr int OR = TV == 2 ? RB : CV;                       // rows of a warp's O as it is handed over
+  static constexpr int kMergeO = kKaWarps * OR * HD * 4, kMergeOff = kKaWarps * RB * NG * 4;
+  static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 <= kRing, "the exchange fits over the ring");
+  static_assert(RB * KT * 4 <= kCodes, "P of a tile fits over its K codes");
+  static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
+};
+
+__device__ __forceinline__ void ka_mma_s(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ka_mma_o(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ka_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ka_copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+// Nibble p of both halves of x, as bf16 numbers c - 8: 16 + c has its code in the mantissa's upper bits.
+template <int p>
+__device__ __forceinline__ uint32_t ka_codes(uint32_t x) {
+  const uint32_t y = ((p == 0 ? x << 3 : x >> (4 * p - 3)) & 0x00780078u) | 0x41804180u;
+  const uint32_t off = 0x41C041C0u;                                  // 24
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&off));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ka_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float ka_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+
+template <int N>
+__device__ __forceinline__ void ka_words(const unsigned char* p, uint32_t (&d)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    d[0] = v.x; d[1] = v.y;
+  } else {
+    d[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+template <int HD, int GROUP, int RB, int TV>
+__global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a) {
+  using S = KaShape<HD, GROUP, RB, TV>;
+  constexpr int NG = S::NG, NB = S::NB, NBV = S::NBV, KT = S::KT, SUB = S::SUB, W4 = S::PL / 32;
+  extern __shared__ __align__(128) unsigned char ka_sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
-  const int tok0 = a.q_start ? a.q_start[b] : b, n = a.q_start ? a.q_start[b + 1] - tok0 : 1, len = a.kv_len[b];
-  const int i = blockIdx.x / a.hq, h = blockIdx.x % a.hq;
-  if (tok0 < 0 || n < 0 || n > a.max_q || tok0 + n > a.tokens || len < 0 || len > a.max_kv) {
+  pdl_launch_dependents();
+  // ---- which rows and keys
+  const int tile = blockIdx.x % a.row_tiles, split = blockIdx.x / a.row_tiles % a.splits, kvh = blockIdx.x / a.row_tiles / a.splits, b = blockIdx.y;
+  const int G = a.hq / a.kv.hkv;
+  const int tok0 = a.q_start ? a.q_start[b] : b, nq = a.q_start ? a.q_start[b + 1] - tok0 : 1, len = a.kv_len[b];
+  if (tok0 < 0 || nq < 0 || nq > a.max_q || tok0 > a.tokens - nq || len < 0 || len > a.max_kv) {
     if (threadIdx.x == 0) set_status(a.status, kDevBadPosition);
     return;
   }
-  if (i >= n) return;
-  const int at = len - n + i, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
-  const Kv4Dims d{HD, a.kv.d.group};
-  const int kvh = h / (a.hq / a.kv.hkv), e0 = lane * V;
-  float q[V], o[V], m = -INFINITY, l = 0.f;
-  row_load<V>(a.q, (tok0 + i) * a.q_stride + (long long)h * HD + e0, a.q_type, q);
+  const int r0 = tile * RB, rows = min(RB, nq * G - r0);
+  if (rows <= 0) return;
+  const int first = len - nq + r0 / G, lastp = len - nq + (r0 + rows - 1) / G;              // positions of the first and last row
+  const int key0 = (a.window > 0 ? max(0, first - a.window + 1) : 0) & ~(KT - 1), key1 = lastp + 1;     // keys that any of them sees
+  const int nsplit = max(1, (key1 - key0 + a.share - 1) / a.share);
+  if (split >= nsplit) return;
+  const int t0 = (key0 + split * a.share) / KT, t1 = (min(key1, key0 + (split + 1) * a.share) + KT - 1) / KT;
+
+  // ---- this warp's ring
+  unsigned char* ring = ka_sm + warp * (kKaStages * S::kStage);
+  const Kv4Dims d{HD, GROUP};
+  const long long head = (long long)kvh * d.head_bytes(), page_bytes = (long long)a.kv.hkv * d.head_bytes();
+  const int* table = a.kv.table + b * a.kv.table_stride;
+  bool bad = false;
+  int next = t0 + warp, slot_in = 0;
+  int page = next < t1 ? __ldg(table + next * KT / kKv4Page) : 0;
+  auto issue = [&]() {
+    if (next < t1) {
+      if (page < 0 || page >= a.kv.num_pages) bad = true;
+      else {
+        const unsigned char* src = a.kv.pages + page * page_bytes + head;
+        unsigned char* dst = ring + slot_in * S::kStage;
+        const int at = next * KT % kKv4Page;
 #pragma unroll
-  for (int j = 0; j < V; ++j) o[j] = 0.f;
-  for (int p = lo + warp; p <= at; p += 8) {
-    const uint8_t* page = kv4_page(a.kv, b, p, a.status);
-    if (!page) continue;
-    const uint8_t* head = page + (long long)kvh * d.head_bytes();
-    const int slot = p % kKv4Page;
-    const __half2 ks = reinterpret_cast<const __half2*>(head + d.k_scales())[slot * d.groups() + e0 / d.group];
-    const __half2 vs = reinterpret_cast<const __half2*>(head + d.v_scales())[slot * d.groups() + e0 / d.group];
-    float s = 0.f;
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+          for (int p = 0; p < S::P; ++p)
+#pragma unroll
+            for (int i = 0; i < KT * S::ROW / 512; ++i)
+              ka_copy16(dst + side * S::kCodes + p * KT * S::ROW + i * 512 + lane * 16,
+                        src + (side ? d.v_codes() : d.k_codes()) + p * kKv4Page * S::ROW + at * S::ROW + i * 512 + lane * 16);
+        constexpr int N = S::kScales / 16;                           // 16-byte pieces of a side's scales: 8 or 16
+        if (lane < 2 * N) {
+          const int side = lane / N, i = lane % N;
+          ka_copy16(dst + 2 * S::kCodes + side * S::kScales + i * 16, src + (side ? d.v_scales() : d.k_scales()) + at * NG * 4 + i * 16);
+        }
+      }
+      next += kKaWarps;
+      if (next < t1) page = __ldg(table + next * KT / kKv4Page);
+    }
+    if (++slot_in == kKaStages) slot_in = 0;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kKaStages - 1; ++i) issue();
+
+  // ---- query rows as digits; what multiplies their sums, and their sums over the groups
+  uint32_t* digits = reinterpret_cast<uint32_t*>(ka_sm + S::kRing);                         // [64 dims][nb][lane][4]
+  float* unit_s = reinterpret_cast<float*>(ka_sm + S::kUnit);
+  float* qsum_s = unit_s + RB;
+  for (int r = warp; r < RB; r += kKaWarps) {
+    constexpr int V = HD / 32;
+    float x[V];
+    const int row = r0 + r;
+    if (r < rows) row_load<V>(a.q, (tok0 + row / G) * a.q_stride + (long long)(kvh * G + row % G) * HD + lane * V, a.q_type, x);
+    float top = 0.f, sum = 0.f;
+    bool odd = false;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const uint32_t byte = head[d.k_codes() + d.k_byte(slot, e0 + j)], c = d.k_high(e0 + j) ? byte >> 4 : byte & 15;
-      s = fmaf(q[j], fmaf(__low2float(ks), (float)c, __high2float(ks)), s);
+      if (r >= rows) x[j] = 0.f;
+      top = fmaxf(top, fabsf(x[j]));
+      odd = odd || !isfinite(x[j]);
+      sum += x[j];
     }
-    s = warp_sum(s) * a.qscale;
-    const float top = fmaxf(m, s), keep = exp2f(m - top), w = exp2f(s - top);
-    m = top;
-    l = l * keep + w;
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, odd ? 0x7F800000u : __float_as_uint(top));
+    const int e = max((int)(bits >> 23), 30);
+    const float f = __uint_as_float((uint32_t)(254 + 5 - e) << 23);
+    const bool spoilt = bits >= 0x7F800000u;
+    uint32_t word[4][(V + 3) / 4] = {};
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const uint32_t byte = head[d.v_codes() + d.v_byte(slot, e0 + j)], c = d.v_high(e0 + j) ? byte >> 4 : byte & 15;
-      o[j] = fmaf(w, fmaf(__low2float(vs), (float)c, __high2float(vs)), o[j] * keep);
+      float y = spoilt ? 0.f : x[j] * f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float q = rintf(y);
+        word[i][j / 4] |= ((uint32_t)(int)q & 0xFFu) << (8 * (j % 4));
+        y = (y - q) * 128.f;
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // element e0 = 64 T + 32 step + 16 half + 4 t + byte lies in word (T, step, half) of lane (column 4 (r & 1) + i, t)
+      const int e0 = lane * V, at = ((e0 / 64 * NB + (r >> 1)) * 32 + (4 * (r & 1) + i) * 4) * 4 + e0 % 64 / 16;
+      if constexpr (V == 2) {
+        const uint32_t both = word[i][0] | __shfl_down_sync(0xffffffffu, word[i][0], 1) << 16;
+        if (!(lane & 1)) digits[at + e0 % 16 / 4 * 4] = both;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) digits[at + (e0 + 4 * j) % 16 / 4 * 4] = word[i][j];
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < GROUP / V; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane % (GROUP / V) == 0) qsum_s[r * NG + lane / (GROUP / V)] = sum * a.qscale;
+    if (lane == 0) unit_s[r] = spoilt ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 5) << 23) * a.qscale;
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) so[warp][e0 + j] = o[j];
-  if (lane == 0) { sm[warp] = m; sl[warp] = l; }
   __syncthreads();
-  if (threadIdx.x >= HD) return;
-  float top = -INFINITY, sum = 0.f, v = 0.f;
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, sm[w]);
-  for (int w = 0; w < 8 && top != -INFINITY; ++w) {
-    const float f = exp2f(sm[w] - top);
-    sum += f * sl[w];
-    v += f * so[w][threadIdx.x];
+  float unit[NB], qsum[NB][NG], m[NB], l[NB];
+  int hi[NB], lo[NB];                                                // the keys that this lane's rows see
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = 2 * nb + (t >> 1);
+    unit[nb] = unit_s[r];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) qsum[nb][i] = qsum_s[r * NG + i];
+    const int at = len - nq + (r0 + r) / G;
+    hi[nb] = r < rows ? at : -1;
+    lo[nb] = a.window > 0 ? at - a.window + 1 : 0;
+    m[nb] = -INFINITY;
+    l[nb] = 0.f;
   }
-  gg_store1(a.out, (tok0 + i) * a.out_stride + (long long)h * HD + threadIdx.x, a.q_type, sum == 0.f ? 0.f : v / sum);
+  float o[S::MT][NBV][4], off[NBV][NG];
+#pragma unroll
+  for (int c = 0; c < NBV; ++c) {
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) off[c][i] = 0.f;
+  }
+  // keys that every row sees, so that tiles within them need no mask
+  const int open1 = rows == RB ? first + 1 : 0, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
+
+  auto add = [](float (&acc)[4], const uint32_t (&x)[4], const uint32_t (&y)[2]) {
+    if constexpr (TV == 2) {
+      ka_mma_o(acc, x, y[0], y[1]);
+    } else {
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      ka_mma_o(part, x, y[0], y[1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += part[i];
+    }
+  };
+  int slot = 0;
+#pragma unroll 1
+  for (int tl = t0 + warp; tl < t1; tl += kKaWarps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kKaStages - 2) : "memory");
+    __syncwarp();                                                    // the tile is there, and the tile before is done with
+    issue();
+    unsigned char* st = ring + slot * S::kStage;
+    if (++slot == kKaStages) slot = 0;
+    const bool edge = tl * KT < open0 || tl * KT + KT > open1;
+
+    // ---- S: lane (g, t) gathers the digit pair t & 1 of row 2 nb + (t >> 1) for the keys g and g + 8
+    float s[SUB][NB][2], smin[SUB][NB];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[u][nb][0] = s[u][nb][1] = smin[u][nb] = 0.f;
+    {
+      uint32_t ks[SUB][2][NG];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) ka_words<NG>(st + 2 * S::kCodes + (u * 16 + g + 8 * h) * NG * 4, ks[u][h]);
+      int c[SUB][NB][4];
+#pragma unroll
+      for (int p = 0; p < S::P; ++p) {
+        uint32_t k[SUB][2][W4];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) ka_words<W4>(st + p * KT * S::ROW + (u * 16 + g + 8 * h) * S::ROW + t * (S::ROW / 4), k[u][h]);
+#pragma unroll
+        for (int j = 0; j < W4; ++j) {                               // 32 dims
+          const int dim = p * S::PL + j * 32, grp = dim / GROUP;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const uint2 q = *reinterpret_cast<const uint2*>(digits + ((dim / 64 * NB + nb) * 32 + lane) * 4 + (j & 1) * 2);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+              if (dim % GROUP == 0) c[u][nb][0] = c[u][nb][1] = c[u][nb][2] = c[u][nb][3] = kGgMagic;
+              const uint32_t x = k[u][0][j], y = k[u][1][j];
+              constexpr uint32_t n = 0x0F0F0F0Fu;
+              ka_mma_s(c[u][nb], x & n, y & n, (x >> 4) & n, (y >> 4) & n, q.x, q.y);
+            }
+          }
+          if ((dim + 32) % GROUP == 0) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+              const float2 s0 = __half22float2(*reinterpret_cast<const __half2*>(&ks[u][0][grp]));
+              const float2 s1 = __half22float2(*reinterpret_cast<const __half2*>(&ks[u][1][grp]));
+              const float low = t & 1 ? s1.y : s0.y;
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                constexpr float big = 12582912.f;
+                const float d0 = __int_as_float(c[u][nb][0]) - big, d1 = __int_as_float(c[u][nb][1]) - big;
+                const float d2 = __int_as_float(c[u][nb][2]) - big, d3 = __int_as_float(c[u][nb][3]) - big;
+                s[u][nb][0] = fmaf(s0.x, fmaf(d1, 1.f / 128, d0), s[u][nb][0]);
+                s[u][nb][1] = fmaf(s1.x, fmaf(d3, 1.f / 128, d2), s[u][nb][1]);
+                smin[u][nb] = fmaf(low, qsum[nb][grp], smin[u][nb]);
+              }
+            }
+          }
+        }
+      }
+    }
+    // ---- whole scores: lane keeps key g + 8 (t & 1); softmax against the row's reference
+    float p[SUB][NB];
+    bool over = false;
+    const float digit = t & 1 ? 1.f / 16384 : 1.f;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float mine = (t & 1 ? s[u][nb][1] : s[u][nb][0]) * digit, other = (t & 1 ? s[u][nb][0] : s[u][nb][1]) * digit;
+        float x = fmaf(mine + __shfl_xor_sync(0xffffffffu, other, 1), unit[nb], smin[u][nb]);
+        if (edge) {
+          const int key = tl * KT + u * 16 + g + 8 * (t & 1);
+          if (key > hi[nb] || key < lo[nb]) x = -INFINITY;
+        }
+        p[u][nb] = x;
+        over = over || x > m[nb] + 8.f;
+      }
+    if (__any_sync(0xffffffffu, over)) {
+      float f[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float top = m[nb];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) top = fmaxf(top, p[u][nb]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        f[nb] = m[nb] == top ? 1.f : ka_ex2(m[nb] - top);            // equal: both may be -inf
+        m[nb] = top;
+        l[nb] *= f[nb];
+      }
+      auto of_row = [&](int r) {                                     // factor of row r, from a lane that holds it
+        float v = 1.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const float x = __shfl_sync(0xffffffffu, f[nb], (r & 1) * 2);
+          if (r >> 1 == nb) v = x;
+        }
+        return v;
+      };
+#pragma unroll
+      for (int c = 0; c < NBV; ++c) {
+        const float f0 = of_row((c * 8 + 2 * t) / TV), f1 = of_row((c * 8 + 2 * t + 1) / TV), fo = of_row((c * 8 + g) / TV);
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) { o[i][c][0] *= f0; o[i][c][1] *= f1; o[i][c][2] *= f0; o[i][c][3] *= f1; }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) off[c][i] *= fo;
+      }
+    }
+    // ---- P in the order of the keys in O's products: key t + 4 i of a block of 16 at 4 t + i.  It lies over the K codes.
+    float* ps = reinterpret_cast<float*>(st);
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float x = ka_ex2(p[u][nb] - (m[nb] == -INFINITY ? 0.f : m[nb]));
+        l[nb] += x;
+        const int key = g + 8 * (t & 1);
+        ps[(2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4] = x;
+      }
+    __syncwarp();
+
+    // ---- O: lane (g, t) holds column g of P s for the keys t + 4 i, and the codes of unit g of those keys
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      float w[NBV][4];
+#pragma unroll
+      for (int c = 0; c < NBV; ++c) {
+        const int r = (c * 8 + g) / TV;
+        const float4 v = *reinterpret_cast<const float4*>(ps + (r < RB ? r : 0) * KT + u * 16 + 4 * t);
+        w[c][0] = v.x; w[c][1] = v.y; w[c][2] = v.z; w[c][3] = v.w;
+      }
+      uint32_t vs[4][NG];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ka_words<NG>(st + 2 * S::kCodes + S::kScales + (u * 16 + t + 4 * i) * NG * 4, vs[i]);
+      uint32_t bt[NBV][2];
+#pragma unroll
+      for (int pl = 0; pl < S::P; ++pl) {
+        constexpr int WU = S::ROW / 32;                              // words of a unit: 2, at head size 64 one
+        uint32_t v[4][WU];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int unit_at = S::PL == 128 ? g ^ (4 * (t >> 1)) : g;
+          ka_words<WU>(st + S::kCodes + pl * KT * S::ROW + (u * 16 + t + 4 * i) * S::ROW + unit_at * (S::ROW / 8), v[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < WU; ++j) {                               // 64 dims
+          const int dim = pl * S::PL + j * 64, grp = dim / GROUP;
+          if (dim % GROUP == 0) {
+            float sc[4], mn[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vs[i][grp]));
+              sc[i] = f.x;
+              mn[i] = fmaf(8.f, f.x, f.y);
+            }
+#pragma unroll
+            for (int c = 0; c < NBV; ++c) {
+              float x[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                x[i] = w[c][i] * sc[i];
+                float y = w[c][i] * mn[i];
+                if (edge && w[c][i] == 0.f) x[i] = y = 0.f;          // a row that is not seen may hold anything
+                off[c][grp] += y;
+              }
+              uint32_t b0 = ka_pack(x[0], x[1]), b1 = ka_pack(x[2], x[3]);
+              const int term = (c * 8 + g) % TV;
+#pragma unroll
+              for (int k = 1; k < TV; ++k) {                         // the next term, in the lanes whose column is one
+                x[0] -= ka_lo(b0); x[1] -= ka_hi(b0); x[2] -= ka_lo(b1); x[3] -= ka_hi(b1);
+                const uint32_t n0 = ka_pack(x[0], x[1]), n1 = ka_pack(x[2], x[3]);
+                if (term >= k) { b0 = n0; b1 = n1; }
+              }
+              bt[c][0] = b0;
+              bt[c][1] = b1;
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {                              // 32 dims: a half of the units' words
+            const uint32_t x = __byte_perm(v[0][j], v[1][j], h ? 0x7632 : 0x5410), y = __byte_perm(v[2][j], v[3][j], h ? 0x7632 : 0x5410);
+            const uint32_t a0[4] = {ka_codes<0>(x), ka_codes<1>(x), ka_codes<0>(y), ka_codes<1>(y)};
+            const uint32_t a1[4] = {ka_codes<2>(x), ka_codes<3>(x), ka_codes<2>(y), ka_codes<3>(y)};
+            const int mt = dim / 16 + 2 * h;
+#pragma unroll
+            for (int c = 0; c < NBV; ++c) {
+              add(o[mt][c], a0, bt[c]);
+              add(o[mt + 1][c], a1, bt[c]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---- the warps' sums
+  float* mo = reinterpret_cast<float*>(ka_sm);                       // [warp][OR][HD]
+  float* moff = mo + S::kMergeO / 4;                                 // [warp][RB][NG]
+  float* ml = moff + S::kMergeOff / 4;                               // [warp][RB][2]
+  const bool spoilt = __syncthreads_or(bad) != 0;                    // every warp is done with its ring, too
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float x = l[nb];
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+    if (g == 0 && !(t & 1)) {
+      ml[(warp * RB + 2 * nb + (t >> 1)) * 2] = m[nb];
+      ml[(warp * RB + 2 * nb + (t >> 1)) * 2 + 1] = x;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NBV; ++c) {
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      float x = off[c][i];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      if (t == 0 && (c * 8 + g) % TV == 0 && c * 8 + g < S::CV) moff[(warp * RB + (c * 8 + g) / TV) * NG + i] = x;
+    }
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int dim = i * 16 + h * 8 + g;
+        if constexpr (TV == 2) {                                     // the two terms of row 4 c + t
+          if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + dim] = o[i][c][2 * h] + o[i][c][2 * h + 1];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (c * 8 + 2 * t + k < S::CV) mo[(warp * S::OR + c * 8 + 2 * t + k) * HD + dim] = o[i][c][2 * h + k];
+        }
+      }
+  }
+  __syncthreads();
+  auto out_at = [&](int r) {
+    const int row = r0 + r;
+    return (long long)(tok0 + row / G) * a.out_stride + (long long)(kvh * G + row % G) * HD;
+  };
+  const long long u = ((long long)b * a.kv.hkv + kvh) * a.row_tiles + tile;
+  float* rec = a.parts + (u * a.splits + split) * (RB * (HD + 2));
+  for (int i = threadIdx.x; i < RB * HD; i += kKaThreads) {
+    const int r = i / HD, dim = i % HD;
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, ml[(w * RB + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < kKaWarps; ++w) {
+      const float mw = ml[(w * RB + r) * 2], f = mw == top ? 1.f : ka_ex2(mw - top);
+      float x = moff[(w * RB + r) * NG + dim / GROUP];
+      if constexpr (TV == 2) x += mo[(w * RB + r) * HD + dim];
+      else x += mo[(w * S::OR + r * 3) * HD + dim] + (mo[(w * S::OR + r * 3 + 1) * HD + dim] + mo[(w * S::OR + r * 3 + 2) * HD + dim]);
+      sum += f * ml[(w * RB + r) * 2 + 1];
+      v += f * x;
+    }
+    if (nsplit == 1) {
+      if (r < rows && !spoilt) gg_store1(a.out, out_at(r) + dim, a.q_type, sum == 0.f ? 0.f : v / sum);
+    } else {
+      rec[r * (HD + 2) + dim] = v;
+      if (dim == 0) {
+        rec[r * (HD + 2) + HD] = top;
+        rec[r * (HD + 2) + HD + 1] = spoilt ? -1.f : sum;
+      }
+    }
+  }
+  if (nsplit == 1) {
+    if (spoilt && threadIdx.x == 0) set_status(a.status, kDevBadPosition);
+    return;
+  }
+  // ---- the shares' sums: the last CTA of the unit to arrive
+  __shared__ int last_s;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last_s = ticket_last(a.tickets + u, nsplit, [](unsigned* p, unsigned n) { return atomicInc(p, n); });
+  __syncthreads();
+  if (!last_s) return;
+  __threadfence();
+  const float* all = a.parts + u * a.splits * (RB * (HD + 2));
+  for (int i = threadIdx.x; i < rows * HD; i += kKaThreads) {
+    const int r = i / HD, dim = i % HD;
+    const float* at = all + r * (HD + 2);
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+    bool lost = false;
+    for (int k = 0; k < nsplit; ++k) {
+      const float* x = at + k * (RB * (HD + 2));
+      top = fmaxf(top, __ldcg(x + HD));
+      lost = lost || __ldcg(x + HD + 1) < 0.f;
+    }
+    for (int k = 0; k < nsplit; ++k) {
+      const float* x = at + k * (RB * (HD + 2));
+      const float mk = __ldcg(x + HD), f = mk == top ? 1.f : ka_ex2(mk - top);
+      sum += f * __ldcg(x + HD + 1);
+      v += f * __ldcg(x + dim);
+    }
+    if (lost) { if (i == 0) set_status(a.status, kDevBadPosition); }
+    else gg_store1(a.out, out_at(r) + dim, a.q_type, sum == 0.f ? 0.f : v / sum);
+  }
 }
+
+// Rows of a CTA for `rows` query rows of a kv head: the fewest that hold them, and four at head size 256, where O of eight would
+// not fit the registers.
+constexpr int ka_rows(int hd, long long rows) { return rows <= 2 ? 2 : rows <= 4 || hd == 256 ? 4 : 8; }
 
 }  // namespace b200lm

@@ -90,6 +90,36 @@ static void launch_rows(cudaStream_t st, RowArgs a, int hd, int sms) {
   else launch_pdl(qk_norm_rope_kernel<256, APPEND>, grid, dim3(128), 0, st, a);
 }
 
+void launch_kv4_attn_64(cudaStream_t st, const Kv4AttnArgs& a, int rb);
+void launch_kv4_attn_128(cudaStream_t st, const Kv4AttnArgs& a, int rb);
+void launch_kv4_attn_256(cudaStream_t st, const Kv4AttnArgs& a, int rb);
+
+// How a call's keys are shared out.  A unit is a (sequence, kv head, row tile).
+struct Kv4Plan {
+  int rb, row_tiles, share, splits;
+  int64_t units, bytes;
+};
+static Kv4Plan plan_attention(int batch, int hkv, int hd, int hq, int max_q, int max_kv, int window, int sms) {
+  Kv4Plan p;
+  const long long rows = (long long)max_q * (hq / hkv);
+  p.rb = ka_rows(hd, rows);
+  const long long tiles = (rows + p.rb - 1) / p.rb;
+  p.units = tiles * hkv * batch;
+  B2_CHECK(tiles * hkv <= 0x7FFFFFFF, kInvalidArgument, "too many query rows for one call");
+  p.row_tiles = (int)tiles;
+  // Shares of 2 CTAs an SM four times over, so that sequences of different lengths even out; none shorter than a round of
+  // the CTA's warps.
+  const int round = (hd == 256 ? 16 : 32) * kKaWarps;
+  const long long most = std::max<long long>(1, 8ll * sms / p.units);
+  const long long keys = (window > 0 ? std::min<long long>(max_kv, (long long)window + max_q) : max_kv) + 32;
+  p.share = (int)std::min<long long>((keys / most + round) / round * round, 1 << 30);
+  p.splits = (int)std::min<long long>(std::max<long long>(1, (keys + p.share - 1) / p.share), most);
+  B2_CHECK(tiles * hkv * p.splits <= 0x7FFFFFFF, kInvalidArgument, "too many query rows for one call");
+  // what a call of any length up to these sizes may need
+  p.bytes = most == 1 ? 0 : kKaTickets * 4 + p.units * most * p.rb * (hd + 2) * 4;
+  return p;
+}
+
 }  // namespace b200lm
 
 using namespace b200lm;
@@ -197,7 +227,7 @@ static void check_attention(int batch, int hkv, int hd, int hq, int max_q, int m
   check_query_heads(hq);
   B2_CHECK(batch > 0 && batch <= 65535, kInvalidArgument, "batch must be 1 .. 65535");
   B2_CHECK(hq % hkv == 0, kInvalidArgument, "hq must be a multiple of hkv");
-  B2_CHECK(max_q >= 1 && max_kv >= 0, kInvalidArgument, "max_q must be positive, max_kv not negative");
+  B2_CHECK(max_q >= 1 && max_q <= (1 << 30) && max_kv >= 0 && max_kv <= (1 << 30), kInvalidArgument, "max_q must be 1 .. 2^30, max_kv 0 .. 2^30");
 }
 
 extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, int32_t hkv, int32_t hd, int32_t hq, int32_t max_q,
@@ -206,7 +236,8 @@ extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, in
   B2_CHECK(bytes, kInvalidArgument, "null pointer");
   check_attention(batch, hkv, hd, hq, max_q, max_kv);
   require_device(device);
-  *bytes = 0;
+  DeviceScope scope(device);
+  *bytes = plan_attention(batch, hkv, hd, hq, max_q, max_kv, 0, device_sms(device)).bytes;
   KV4_END
 }
 
@@ -237,9 +268,14 @@ extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cach
   a.qscale = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)cache->hd));
   a.out = out_dev; a.out_stride = out_stride; a.status = status_dev;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)(max_q * hq), (unsigned)cache->batch);
-  if (cache->hd == 64) launch_pdl(kv4_attn_simple_kernel<64>, grid, dim3(256), 0, st, a);
-  else if (cache->hd == 128) launch_pdl(kv4_attn_simple_kernel<128>, grid, dim3(256), 0, st, a);
-  else launch_pdl(kv4_attn_simple_kernel<256>, grid, dim3(256), 0, st, a);
+  const Kv4Plan p = plan_attention(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv, window, device_sms(device));
+  B2_CHECK(p.splits == 1 || (workspace_dev && workspace_bytes >= p.bytes), kInvalidArgument,
+           "the workspace is smaller than AttentionKv4Workspace says: " + std::to_string(p.bytes) + " bytes");
+  a.row_tiles = p.row_tiles; a.share = p.share; a.splits = p.splits;
+  a.tickets = reinterpret_cast<unsigned*>(workspace_dev);
+  a.parts = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(workspace_dev) + kKaTickets * 4);
+  if (cache->hd == 64) launch_kv4_attn_64(st, a, p.rb);
+  else if (cache->hd == 128) launch_kv4_attn_128(st, a, p.rb);
+  else launch_kv4_attn_256(st, a, p.rb);
   KV4_END
 }
