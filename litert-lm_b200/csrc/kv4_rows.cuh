@@ -123,12 +123,12 @@ __device__ __forceinline__ void row_store(void* p, long long i, int type, const 
 // Norm and rotation of the V elements that this lane holds of a head, in T.  `sn` is negative in the lanes of the first half of
 // the pairs, so that the same line serves both; `off` is 0 in lanes that do not rotate.
 template <typename T, int V>
-__device__ __forceinline__ void norm_rotate(const float (&x)[V], const float* gain, float eps, const float (&c)[V], const float (&sn)[V],
+__device__ __forceinline__ void norm_rotate(const float (&x)[V], bool norm, const float (&gain)[V], float eps, const float (&c)[V], const float (&sn)[V],
                                             int off, int lane, bool rotates, bool any, T (&y)[V]) {
   constexpr int HD = 32 * V;
 #pragma unroll
   for (int j = 0; j < V; ++j) y[j] = (T)x[j];
-  if (gain) {
+  if (norm) {
     T sum = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) sum += y[j] * y[j];
@@ -138,7 +138,7 @@ __device__ __forceinline__ void norm_rotate(const float (&x)[V], const float* ga
     if constexpr (sizeof(T) == 8) inv = 1.0 / sqrt(sum / HD + (double)eps);
     else inv = 1.f / sqrtf(sum / HD + eps);
 #pragma unroll
-    for (int j = 0; j < V; ++j) y[j] = y[j] * inv * (T)__ldg(gain + lane * V + j);
+    for (int j = 0; j < V; ++j) y[j] = y[j] * inv * (T)gain[j];
   }
   if (any) {
 #pragma unroll
@@ -169,25 +169,49 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[V], int gl, uint32
   constexpr float top = 65504.f;                           // fp16's largest
   const __half m = __float2half_rn(fminf(fmaxf(low, -top), top));
   const __half s = __float2half_rn(fminf((float)(((double)high - (double)low) / 15.0), top));
-  const double md = (double)__half2float(m), sd = (double)__half2float(s);
+  const float mf = __half2float(m), sf = __half2float(s), inv = sf > 0.f ? 1.f / sf : 0.f;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const double c = sd > 0 ? rint(((double)x[j] - md) / sd) : 0.0;
-    code[j] = bad ? 0u : (uint32_t)fmin(fmax(c, 0.0), 15.0);
+    // three roundings leave a code below 16 off by at most 3 * 2^-24 * 16 = 3e-6: nearer to a border than that fp64 decides
+    const float c = (x[j] - mf) * inv, whole = rintf(c);
+    float decided = whole;
+    if (fabsf(fabsf(c - whole) - 0.5f) < 1e-5f && sf > 0.f) decided = (float)rint(((double)x[j] - (double)mf) / (double)sf);
+    code[j] = bad ? 0u : (uint32_t)fminf(fmaxf(decided, 0.f), 15.f);
   }
   if (bad) return 0x7E007E00u;                             // NaN, NaN
   return (uint32_t)__half_as_ushort(s) | (uint32_t)__half_as_ushort(m) << 16;
 }
 
-// Writes a head's codes: the two elements of a byte lie 16 (K) or 8 (V) apart.
+// Writes a row's codes; `stage` is the warp's own.  Of K a lane has the bytes of whole words (elements 16 apart share a byte, four
+// neighbours a word).  Of V, neighbours lie in different units: the row is put together in shared memory first.
 template <int V>
-__device__ __forceinline__ void put_codes(uint8_t* codes, const Kv4Dims& d, int slot, bool is_v, int lane, const uint32_t (&code)[V]) {
+__device__ __forceinline__ void put_codes(uint8_t* codes, const Kv4Dims& d, int slot, bool is_v, int lane, const uint32_t (&code)[V], uint8_t* stage) {
   const int e0 = lane * V, apart = (is_v ? 8 : 16) / V;
-  const bool low = is_v ? !d.v_high(e0) : !d.k_high(e0);
+  uint32_t byte[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const uint32_t other = __shfl_down_sync(0xffffffffu, code[j], apart);
-    if (low) codes[is_v ? d.v_byte(slot, e0 + j) : d.k_byte(slot, e0 + j)] = (uint8_t)(code[j] | other << 4);
+  for (int j = 0; j < V; ++j) byte[j] = code[j] | __shfl_down_sync(0xffffffffu, code[j], apart) << 4;
+  if (!is_v) {
+    if (d.k_high(e0)) return;
+    if constexpr (V == 2) {
+      *reinterpret_cast<uint16_t*>(codes + d.k_byte(slot, e0)) = (uint16_t)(byte[0] | byte[1] << 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; j += 4)
+        *reinterpret_cast<uint32_t*>(codes + d.k_byte(slot, e0 + j)) = byte[j] | byte[j + 1] << 8 | byte[j + 2] << 16 | byte[j + 3] << 24;
+    }
+    return;
+  }
+  constexpr int ROW = V >= 4 ? 64 : 32, PLANES = V == 8 ? 2 : 1;     // bytes of a plane's row
+  const int plane = e0 / (2 * ROW);
+  __syncwarp();                                                      // the row before has been taken away
+  if (!d.v_high(e0)) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) stage[plane * ROW + d.v_byte(slot, e0 + j) - (plane * kKv4Page + slot) * ROW] = (uint8_t)byte[j];
+  }
+  __syncwarp();
+  if (lane * 4 < PLANES * ROW) {
+    const int p = lane * 4 / ROW, at = lane * 4 % ROW;
+    *reinterpret_cast<uint32_t*>(codes + (p * kKv4Page + slot) * ROW + at) = *reinterpret_cast<const uint32_t*>(stage + lane * 4);
   }
 }
 
@@ -202,6 +226,7 @@ __device__ __forceinline__ uint8_t* kv4_page(const Kv4Args& kv, int seq, int pos
 template <int HD, bool APPEND>
 __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
   constexpr int V = HD / 32;
+  __shared__ __align__(16) uint8_t stage[4][APPEND ? HD / 2 : 16];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -220,20 +245,27 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
   }
   const bool rotates = e0 < a.rot, first = e0 < half;
   const int off = rotates ? (first ? half / V : -(half / V)) : 0;
-  float c[V], sn[V];
+  float c[V], sn[V], qg[V], kg[V], ahead[V];
+  row_load<V>(a.qkv, tok * a.stride + (long long)h0 * HD + e0, a.type, ahead);
+  if (rotates) {
+    const long long i = (long long)pos * half + e0 - (first ? 0 : half);
+    row_load<V>(a.cos, i, kF32, c);
+    row_load<V>(a.sin, i, kF32, sn);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const long long i = (long long)pos * half + e0 + j - (first ? 0 : half);
-    c[j] = rotates ? __ldg(a.cos + i) : 1.f;
-    sn[j] = rotates ? (first ? -__ldg(a.sin + i) : __ldg(a.sin + i)) : 0.f;
+    for (int j = 0; j < V; ++j) sn[j] = first ? -sn[j] : sn[j];
   }
+  if (a.q_gain) row_load<V>(a.q_gain, e0, kF32, qg);
+  if (a.k_gain) row_load<V>(a.k_gain, e0, kF32, kg);
 #pragma unroll 1
   for (int h = h0; h < h1; ++h) {
     float x[V];
-    row_load<V>(a.qkv, tok * a.stride + (long long)h * HD + e0, a.type, x);
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = ahead[j];
+    if (h + 1 < h1) row_load<V>(a.qkv, tok * a.stride + (long long)(h + 1) * HD + e0, a.type, ahead);
     if (h < a.hq || !APPEND) {
       float y[V];
-      norm_rotate<float, V>(x, h < a.hq ? a.q_gain : a.k_gain, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
+      if (h < a.hq) norm_rotate<float, V>(x, a.q_gain != nullptr, qg, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
+      else norm_rotate<float, V>(x, a.k_gain != nullptr, kg, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
       if (h < a.hq) row_store<V>(a.q_out, tok * a.q_stride + (long long)h * HD + e0, a.type, y);
       else row_store<V>(a.k_out, tok * a.k_stride + (long long)(h - a.hq) * HD + e0, a.type, y);
       continue;
@@ -241,7 +273,7 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
     const bool is_v = h >= a.hq + a.hkv;
     if (!is_v) {
       double y[V];
-      norm_rotate<double, V>(x, a.k_gain, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
+      norm_rotate<double, V>(x, a.k_gain != nullptr, kg, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
 #pragma unroll
       for (int j = 0; j < V; ++j) x[j] = (float)y[j];
     }
@@ -250,7 +282,7 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
     const int slot = pos % kKv4Page, gl = d.group / V;
     uint32_t code[V];
     const uint32_t pair = quantise<V>(x, gl, code);
-    put_codes<V>(head + (is_v ? d.v_codes() : d.k_codes()), d, slot, is_v, lane, code);
+    put_codes<V>(head + (is_v ? d.v_codes() : d.k_codes()), d, slot, is_v, lane, code, stage[threadIdx.x >> 5]);
     if (lane % gl == 0)
       reinterpret_cast<uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + lane / gl] = pair;
   }
@@ -277,11 +309,17 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const i
   const int slot = p % kKv4Page, e0 = lane * V;
   const uint32_t pair = reinterpret_cast<const uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + e0 / d.group];
   const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+  // the row's bytes come in words; V's neighbours lie in different units and are picked from shared memory
+  constexpr int ROW = V >= 4 ? 64 : 32;
+  __shared__ __align__(16) uint8_t stage[4][HD / 2];
+  uint8_t* row = stage[threadIdx.x >> 5];
+  if (lane * 8 < HD) reinterpret_cast<uint32_t*>(row)[lane] = *reinterpret_cast<const uint32_t*>(codes + (lane * 4 / ROW * kKv4Page + slot) * ROW + lane * 4 % ROW);
+  __syncwarp();
   float x[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int e = e0 + j;
-    const uint32_t byte = codes[is_v ? d.v_byte(slot, e) : d.k_byte(slot, e)];
+    const int e = e0 + j, plane = e / (2 * ROW);
+    const uint32_t byte = row[(is_v ? d.v_byte(slot, e) : d.k_byte(slot, e)) - (plane * kKv4Page + slot) * ROW + plane * ROW];
     const uint32_t c = (is_v ? d.v_high(e) : d.k_high(e)) ? byte >> 4 : byte & 15;
     x[j] = fmaf(sm.x, (float)c, sm.y);
   }
