@@ -5,8 +5,9 @@
 //   m = fp16(low), s = fp16((high - low) / 15), code = rint((x - m) / s) held to 0 .. 15
 //
 // Every byte is read and written once: what bounds it is HBM for many tokens, one chain of latencies (row, two warp sums,
-// table row) for a few.  A warp takes some heads of one token and keeps the token's rotation in registers; a lane holds hd / 32
-// neighbouring elements, so that the other half of a pair lies at the same place of a lane rot / hd * 16 further.
+// table row) for a few.  A warp takes up to four heads of one kind and token, asks for their rows at once and keeps gain and
+// rotation multiplied in registers; a lane holds hd / 32 neighbouring elements, so that the other half of a pair lies at the
+// same place of a lane rot / hd * 16 further and comes from there as it lay in memory.
 // Queries are computed in fp32.  Keys that go into the cache are computed in fp64 and rounded to fp32 before their
 // codes are decided: a code next to a border would otherwise depend on the order of the sum, and one step of a code is a
 // fifteenth of the group's range.
@@ -43,7 +44,7 @@ struct RowArgs {
   long long k_stride;
   const int* seq;
   Kv4Args kv;
-  int heads_per_warp;
+  bool vec, vec_q, vec_k;      // rows of qkv, q_out, k_out start on 16-byte boundaries
   int* status;
 };
 
@@ -51,59 +52,72 @@ __device__ __forceinline__ void set_status(int* status, int code) {
   if (status) atomicMax(status, code);
 }
 
-// V neighbouring elements of a row; one load where the address allows it.
-template <int V>
-__device__ __forceinline__ void row_load(const void* p, long long i, int type, float (&x)[V]) {
-  const char* a = reinterpret_cast<const char*>(p) + i * elem_size(type);
-  if (type == kF32) {
-    if constexpr (V >= 4) {
-      if ((reinterpret_cast<uintptr_t>(a) & 15) == 0) {
+// V neighbouring elements of a row as they lie in memory: whole words where the row starts allow it (`vec`), else one by one.
+template <int TYPE, int V>
+struct RawRow {
+  static constexpr int N = TYPE == kF32 ? V : V / 2;
+  uint32_t u[N];
+  __device__ __forceinline__ void load(const void* p, long long i, bool vec) {
+    const char* a = reinterpret_cast<const char*>(p) + i * elem_size(TYPE);
+    if (vec) {
+      if constexpr (N >= 4) {
 #pragma unroll
-        for (int j = 0; j < V; j += 4) {
-          const float4 v = reinterpret_cast<const float4*>(a)[j / 4];
-          x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
+        for (int j = 0; j < N; j += 4) {
+          const uint4 v = reinterpret_cast<const uint4*>(a)[j / 4];
+          u[j] = v.x; u[j + 1] = v.y; u[j + 2] = v.z; u[j + 3] = v.w;
         }
-        return;
+      } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(a);
+        u[0] = v.x; u[1] = v.y;
+      } else {
+        u[0] = *reinterpret_cast<const uint32_t*>(a);
       }
-    }
-  } else if ((reinterpret_cast<uintptr_t>(a) & (2 * V - 1)) == 0) {
-    uint32_t u[V / 2];
-    if constexpr (V == 8) {
-      const uint4 v = *reinterpret_cast<const uint4*>(a);
-      u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w;
-    } else if constexpr (V == 4) {
-      const uint2 v = *reinterpret_cast<const uint2*>(a);
-      u[0] = v.x; u[1] = v.y;
     } else {
-      u[0] = *reinterpret_cast<const uint32_t*>(a);
-    }
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) {
-      const float2 f = gg_pair(u[j], type == kBf16);
-      x[2 * j] = f.x;
-      x[2 * j + 1] = f.y;
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) x[j] = gg_load1(p, i + j, type);
-}
-template <int V>
-__device__ __forceinline__ void row_store(void* p, long long i, int type, const float (&x)[V]) {
-  char* a = reinterpret_cast<char*>(p) + i * elem_size(type);
-  if (type == kF32) {
-    if constexpr (V >= 4) {
-      if ((reinterpret_cast<uintptr_t>(a) & 15) == 0) {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) reinterpret_cast<float4*>(a)[j / 4] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-        return;
+      for (int j = 0; j < N; ++j) {
+        if constexpr (TYPE == kF32) u[j] = reinterpret_cast<const uint32_t*>(a)[j];
+        else u[j] = reinterpret_cast<const uint16_t*>(a)[2 * j] | (uint32_t)reinterpret_cast<const uint16_t*>(a)[2 * j + 1] << 16;
       }
     }
-  } else if ((reinterpret_cast<uintptr_t>(a) & (2 * V - 1)) == 0) {
-    uint32_t u[V / 2];
+  }
+  __device__ __forceinline__ void store(void* p, long long i, bool vec) const {
+    char* a = reinterpret_cast<char*>(p) + i * elem_size(TYPE);
+    if (vec) {
+      if constexpr (N >= 4) {
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) {
-      if (type == kBf16) {
+        for (int j = 0; j < N; j += 4) reinterpret_cast<uint4*>(a)[j / 4] = make_uint4(u[j], u[j + 1], u[j + 2], u[j + 3]);
+      } else if constexpr (N == 2) {
+        *reinterpret_cast<uint2*>(a) = make_uint2(u[0], u[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(a) = u[0];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if constexpr (TYPE == kF32) reinterpret_cast<uint32_t*>(a)[j] = u[j];
+        else {
+          reinterpret_cast<uint16_t*>(a)[2 * j] = (uint16_t)u[j];
+          reinterpret_cast<uint16_t*>(a)[2 * j + 1] = (uint16_t)(u[j] >> 16);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[V]) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (TYPE == kF32) x[j] = __uint_as_float(u[j]);
+      else {
+        const float2 f = gg_pair(u[j], TYPE == kBf16);
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(const float (&x)[V]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (TYPE == kF32) u[j] = __float_as_uint(x[j]);
+      else if constexpr (TYPE == kBf16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
         u[j] = *reinterpret_cast<const uint32_t*>(&h);
       } else {
@@ -111,61 +125,68 @@ __device__ __forceinline__ void row_store(void* p, long long i, int type, const 
         u[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    if constexpr (V == 8) *reinterpret_cast<uint4*>(a) = make_uint4(u[0], u[1], u[2], u[3]);
-    else if constexpr (V == 4) *reinterpret_cast<uint2*>(a) = make_uint2(u[0], u[1]);
-    else *reinterpret_cast<uint32_t*>(a) = u[0];
-    return;
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) gg_store1(p, i + j, type, x[j]);
+};
+template <int V>
+__device__ __forceinline__ void row_load(const void* p, long long i, int type, float (&x)[V]) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p) + i * elem_size(type);
+  auto as = [&](auto raw) {
+    constexpr int bytes = 4 * decltype(raw)::N;
+    raw.load(p, i, at % (bytes < 16 ? bytes : 16) == 0);
+    raw.get(x);
+  };
+  if (type == kF32) as(RawRow<kF32, V>());
+  else if (type == kBf16) as(RawRow<kBf16, V>());
+  else as(RawRow<kF16, V>());
 }
 
-// Norm and rotation of the V elements that this lane holds of a head, in T.  `sn` is negative in the lanes of the first half of
-// the pairs, so that the same line serves both; `off` is 0 in lanes that do not rotate.
+// Norm and rotation of the V elements x that this lane holds of a head, `other` being those of the lane with the other halves of the
+// pairs: y = inv (x ca + other sb), ca = gain * cos, sb = +- the other's gain * sin.
 template <typename T, int V>
-__device__ __forceinline__ void norm_rotate(const float (&x)[V], bool norm, const float (&gain)[V], float eps, const float (&c)[V], const float (&sn)[V],
-                                            int off, int lane, bool rotates, bool any, T (&y)[V]) {
+__device__ __forceinline__ void norm_rotate(const float (&x)[V], const float (&other)[V], bool norm, float eps, const T (&ca)[V], const T (&sb)[V], bool rotates, T (&y)[V]) {
   constexpr int HD = 32 * V;
-#pragma unroll
-  for (int j = 0; j < V; ++j) y[j] = (T)x[j];
+  T inv = 1;
   if (norm) {
     T sum = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum += y[j] * y[j];
+    for (int j = 0; j < V; ++j) sum += (T)x[j] * (T)x[j];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    T inv;
-    if constexpr (sizeof(T) == 8) inv = 1.0 / sqrt(sum / HD + (double)eps);
-    else inv = 1.f / sqrtf(sum / HD + eps);
-#pragma unroll
-    for (int j = 0; j < V; ++j) y[j] = y[j] * inv * (T)gain[j];
+    const T mean = sum * (T)(1.0 / HD) + (T)eps;
+    inv = rsqrtf((float)mean);
+    if constexpr (sizeof(T) == 8) inv = inv * (1.5 - 0.5 * mean * inv * inv);      // 2^-22 -> 2^-43
   }
-  if (any) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const T other = __shfl_sync(0xffffffffu, y[j], lane + off);
-      if (rotates) y[j] = y[j] * (T)c[j] + other * (T)sn[j];
-    }
+  for (int j = 0; j < V; ++j) {
+    y[j] = (T)x[j] * ca[j];
+    if (rotates) y[j] += (T)other[j] * sb[j];
+    y[j] *= inv;
   }
 }
 
 // Codes of the group that this lane's V elements lie in (GL lanes of it); returns the pair (s, m) as fp16 bits.
-template <int V>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[V], int gl, uint32_t (&code)[V]) {
+template <int V, int GL>
+__device__ __forceinline__ uint32_t quantise(const float (&x)[V], uint32_t (&code)[V]) {
   float low = x[0], high = x[0];
-  bool odd = !isfinite(x[0]);
+  bool nan = x[0] != x[0];
 #pragma unroll
   for (int j = 1; j < V; ++j) {
     low = fminf(low, x[j]);
     high = fmaxf(high, x[j]);
-    odd = odd || !isfinite(x[j]);
+    nan = nan || x[j] != x[j];
   }
-  uint32_t bad = odd;
-  for (int o = 1; o < gl; o <<= 1) {
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+  if (nan) high = INFINITY;                                // the comparisons pass a NaN over
+  if constexpr (GL == 32) {                                // one instruction for the whole warp
+    asm volatile("redux.sync.min.f32 %0, %0, 0xffffffff;" : "+f"(low));
+    asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(high));
+  } else {
+#pragma unroll
+    for (int o = 1; o < GL; o <<= 1) {
+      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
   }
+  const bool bad = !isfinite(low) || !isfinite(high);
   constexpr float top = 65504.f;                           // fp16's largest
   const __half m = __float2half_rn(fminf(fmaxf(low, -top), top));
   const __half s = __float2half_rn(fminf((float)(((double)high - (double)low) / 15.0), top));
@@ -180,6 +201,14 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[V], int gl, uint32
   }
   if (bad) return 0x7E007E00u;                             // NaN, NaN
   return (uint32_t)__half_as_ushort(s) | (uint32_t)__half_as_ushort(m) << 16;
+}
+
+// Byte of element e0 + j (e0 = lane V) of a V row whose planes lie one behind the other.
+template <int V>
+__device__ __forceinline__ int v_place(int slot, int e0, int j) {
+  constexpr int PL = V >= 4 ? 128 : 64, ROW = PL / 2;
+  const int turn = PL == 128 ? 4 * (slot >> 1 & 1) : 0;
+  return e0 / PL * ROW + ((e0 + j) % 8 ^ turn) * (ROW / 8) + e0 % PL / 16;
 }
 
 // Writes a row's codes; `stage` is the warp's own.  Of K a lane has the bytes of whole words (elements 16 apart share a byte, four
@@ -201,18 +230,14 @@ __device__ __forceinline__ void put_codes(uint8_t* codes, const Kv4Dims& d, int 
     }
     return;
   }
-  constexpr int ROW = V >= 4 ? 64 : 32, PLANES = V == 8 ? 2 : 1;     // bytes of a plane's row
-  const int plane = e0 / (2 * ROW);
+  constexpr int ROW = V >= 4 ? 64 : 32, HALF = 16 * V;               // bytes of a plane's row, of all planes'
   __syncwarp();                                                      // the row before has been taken away
   if (!d.v_high(e0)) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) stage[plane * ROW + d.v_byte(slot, e0 + j) - (plane * kKv4Page + slot) * ROW] = (uint8_t)byte[j];
+    for (int j = 0; j < V; ++j) stage[v_place<V>(slot, e0, j)] = (uint8_t)byte[j];
   }
   __syncwarp();
-  if (lane * 4 < PLANES * ROW) {
-    const int p = lane * 4 / ROW, at = lane * 4 % ROW;
-    *reinterpret_cast<uint32_t*>(codes + (p * kKv4Page + slot) * ROW + at) = *reinterpret_cast<const uint32_t*>(stage + lane * 4);
-  }
+  if (lane * 4 < HALF) *reinterpret_cast<uint32_t*>(codes + (lane * 4 / ROW * kKv4Page + slot) * ROW + lane * 4 % ROW) = *reinterpret_cast<const uint32_t*>(stage + lane * 4);
 }
 
 // Physical page of (sequence, position), or null (and the status set) where there is none.
@@ -223,87 +248,123 @@ __device__ __forceinline__ uint8_t* kv4_page(const Kv4Args& kv, int seq, int pos
   return kv.pages + (long long)page * kv.hkv * kv.d.head_bytes();
 }
 
-template <int HD, bool APPEND>
+// NH heads of one kind and token a warp; GROUP 0: keys are written out, else keys and values go into the cache.
+template <int HD, int TYPE, int GROUP, int NH>
 __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
   constexpr int V = HD / 32;
+  constexpr bool APPEND = GROUP > 0;
   __shared__ __align__(16) uint8_t stage[4][APPEND ? HD / 2 : 16];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int heads = a.hq + (APPEND ? 2 : 1) * a.hkv, per = (heads + a.heads_per_warp - 1) / a.heads_per_warp;
-  const long long job = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int tok = (int)(job / per), h0 = (int)(job % per) * a.heads_per_warp, h1 = min(h0 + a.heads_per_warp, heads);
+  // a token's jobs: query heads, key heads, value heads
+  const int jq = (a.hq + NH - 1) / NH, jk = (a.hkv + NH - 1) / NH;
+  const uint32_t per = jq + (APPEND ? 2 : 1) * jk, job = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int tok = (int)(job / per), part = (int)(job - tok * per);
   if (tok >= a.tokens) return;
+  const bool is_q = part < jq, is_v = APPEND && part >= jq + jk;
+  const int h0 = (is_q ? part : is_v ? part - jq - jk : part - jq) * NH, hn = min(NH, (is_q ? a.hq : a.hkv) - h0), e0 = lane * V;
+  const long long row = tok * a.stride + ((is_q ? 0 : is_v ? a.hq + a.hkv : a.hq) + h0) * HD + e0;
+  RawRow<TYPE, V> raw[NH];
+#pragma unroll
+  for (int i = 0; i < NH; ++i)
+    if (i < hn) raw[i].load(a.qkv, row + i * HD, a.vec);
   const int pos = a.pos[tok];
   if (pos < 0) return;
-  const int half = a.rot / 2, e0 = lane * V;
   if (a.rot > 0 && pos >= a.rope_rows) { set_status(a.status, kDevBadPosition); return; }
   uint8_t* page = nullptr;
   if constexpr (APPEND) {
     page = kv4_page(a.kv, a.seq ? a.seq[tok] : tok, pos, a.status);
     if (!page) return;
   }
-  const bool rotates = e0 < a.rot, first = e0 < half;
-  const int off = rotates ? (first ? half / V : -(half / V)) : 0;
-  float c[V], sn[V], qg[V], kg[V], ahead[V];
-  row_load<V>(a.qkv, tok * a.stride + (long long)h0 * HD + e0, a.type, ahead);
+  const int half = a.rot / 2, slot = pos % kKv4Page;
+  const bool rotates = e0 < a.rot && !is_v, first = e0 < half;
+  const int other_lane = lane + (rotates ? (first ? half / V : -(half / V)) : 0);
+  const bool norm = (is_q ? a.q_gain : a.k_gain) != nullptr && !is_v;
+  float ca[V], sb[V], gain[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) ca[j] = gain[j] = 1.f, sb[j] = 0.f;
+  if (norm) row_load<V>(is_q ? a.q_gain : a.k_gain, e0, kF32, gain);
   if (rotates) {
     const long long i = (long long)pos * half + e0 - (first ? 0 : half);
-    row_load<V>(a.cos, i, kF32, c);
-    row_load<V>(a.sin, i, kF32, sn);
-#pragma unroll
-    for (int j = 0; j < V; ++j) sn[j] = first ? -sn[j] : sn[j];
+    row_load<V>(a.cos, i, kF32, ca);
+    row_load<V>(a.sin, i, kF32, sb);
   }
-  if (a.q_gain) row_load<V>(a.q_gain, e0, kF32, qg);
-  if (a.k_gain) row_load<V>(a.k_gain, e0, kF32, kg);
-#pragma unroll 1
-  for (int h = h0; h < h1; ++h) {
-    float x[V];
+  auto heads = [&](auto one, auto&& done) {                          // one: a number of the type that norm and rotation are computed in
+    using T = decltype(one);
+    T c[V], s[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = ahead[j];
-    if (h + 1 < h1) row_load<V>(a.qkv, tok * a.stride + (long long)(h + 1) * HD + e0, a.type, ahead);
-    if (h < a.hq || !APPEND) {
-      float y[V];
-      if (h < a.hq) norm_rotate<float, V>(x, a.q_gain != nullptr, qg, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
-      else norm_rotate<float, V>(x, a.k_gain != nullptr, kg, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
-      if (h < a.hq) row_store<V>(a.q_out, tok * a.q_stride + (long long)h * HD + e0, a.type, y);
-      else row_store<V>(a.k_out, tok * a.k_stride + (long long)(h - a.hq) * HD + e0, a.type, y);
-      continue;
+    for (int j = 0; j < V; ++j) {
+      const float other_gain = __shfl_sync(0xffffffffu, gain[j], other_lane);
+      c[j] = (T)ca[j] * (T)gain[j];
+      s[j] = (T)(first ? -sb[j] : sb[j]) * (T)other_gain;
     }
-    const bool is_v = h >= a.hq + a.hkv;
-    if (!is_v) {
-      double y[V];
-      norm_rotate<double, V>(x, a.k_gain != nullptr, kg, a.eps, c, sn, off, lane, rotates, a.rot > 0, y);
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      if (i >= hn) break;
+      RawRow<TYPE, V> fellow;
+#pragma unroll
+      for (int j = 0; j < RawRow<TYPE, V>::N; ++j) fellow.u[j] = __shfl_sync(0xffffffffu, raw[i].u[j], other_lane);
+      float x[V], f[V];
+      raw[i].get(x);
+      fellow.get(f);
+      T y[V];
+      norm_rotate<T, V>(x, f, norm, a.eps, c, s, rotates, y);
 #pragma unroll
       for (int j = 0; j < V; ++j) x[j] = (float)y[j];
+      done(i, x);
     }
-    const Kv4Dims d{HD, a.kv.d.group};
-    uint8_t* head = page + (long long)(h - a.hq - (is_v ? a.hkv : 0)) * d.head_bytes();
-    const int slot = pos % kKv4Page, gl = d.group / V;
-    uint32_t code[V];
-    const uint32_t pair = quantise<V>(x, gl, code);
-    put_codes<V>(head + (is_v ? d.v_codes() : d.k_codes()), d, slot, is_v, lane, code, stage[threadIdx.x >> 5]);
-    if (lane % gl == 0)
-      reinterpret_cast<uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + lane / gl] = pair;
+  };
+  if (is_q || !APPEND) {
+    void* out = is_q ? a.q_out : a.k_out;
+    const long long at = tok * (is_q ? a.q_stride : a.k_stride) + h0 * HD + e0;
+    const bool vec = is_q ? a.vec_q : a.vec_k;
+    heads(1.f, [&](int i, const float (&x)[V]) {
+      RawRow<TYPE, V> y;
+      y.put(x);
+      y.store(out, at + i * HD, vec);
+    });
+  }
+  if constexpr (APPEND) {
+    constexpr Kv4Dims d{HD, GROUP};
+    constexpr int gl = GROUP / V;
+    auto put = [&](int i, const float (&x)[V]) {
+      uint8_t* head = page + (long long)(h0 + i) * d.head_bytes();
+      uint32_t code[V];
+      const uint32_t pair = quantise<V, gl>(x, code);
+      put_codes<V>(head + (is_v ? d.v_codes() : d.k_codes()), d, slot, is_v, lane, code, stage[threadIdx.x >> 5]);
+      if (lane % gl == 0) reinterpret_cast<uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + lane / gl] = pair;
+    };
+    if (is_v) {
+#pragma unroll
+      for (int i = 0; i < NH; ++i) {
+        if (i >= hn) break;
+        float x[V];
+        raw[i].get(x);
+        put(i, x);
+      }
+    } else if (!is_q) {
+      heads(1.0, put);
+    }
   }
 }
 
 // A warp per (token, kv head, K or V); a lane reads the bytes of V elements and their fellows.
-template <int HD>
-__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const int* __restrict__ seq, const int* __restrict__ pos, int tokens, int out_type, void* k_out, void* v_out, int* status) {
+template <int HD, int TYPE, int GROUP>
+__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const int* __restrict__ seq, const int* __restrict__ pos, int tokens, void* k_out, void* v_out, bool vec, int* status) {
   constexpr int V = HD / 32;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, sides = (k_out != nullptr) + (v_out != nullptr);
-  const long long job = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int tok = (int)(job / (sides * kv.hkv)), h = (int)(job % (sides * kv.hkv)) / sides;
+  const uint32_t per = sides * kv.hkv, job = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int tok = (int)(job / per), part = (int)(job - tok * per), h = sides == 2 ? part >> 1 : part;
   if (tok >= tokens) return;
-  const bool is_v = k_out == nullptr || job % sides == 1;
+  const bool is_v = k_out == nullptr || (sides == 2 && (part & 1));
   const int p = pos[tok];
   if (p < 0) return;
   const uint8_t* page = kv4_page(kv, seq ? seq[tok] : tok, p, status);
   if (!page) return;
-  const Kv4Dims d{HD, kv.d.group};
+  constexpr Kv4Dims d{HD, GROUP};
   const uint8_t* head = page + (long long)h * d.head_bytes();
   const uint8_t* codes = head + (is_v ? d.v_codes() : d.k_codes());
   const int slot = p % kKv4Page, e0 = lane * V;
@@ -316,14 +377,16 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const i
   if (lane * 8 < HD) reinterpret_cast<uint32_t*>(row)[lane] = *reinterpret_cast<const uint32_t*>(codes + (lane * 4 / ROW * kKv4Page + slot) * ROW + lane * 4 % ROW);
   __syncwarp();
   float x[V];
+  const int k_at = e0 / (2 * ROW) * ROW + e0 % 16 / 4 * (ROW / 4) + e0 % (2 * ROW) / 32 * 4 + e0 % 4;     // and 4 neighbours, the next 4 a quarter row on
+  const bool high = is_v ? d.v_high(e0) : d.k_high(e0);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int e = e0 + j, plane = e / (2 * ROW);
-    const uint32_t byte = row[(is_v ? d.v_byte(slot, e) : d.k_byte(slot, e)) - (plane * kKv4Page + slot) * ROW + plane * ROW];
-    const uint32_t c = (is_v ? d.v_high(e) : d.k_high(e)) ? byte >> 4 : byte & 15;
-    x[j] = fmaf(sm.x, (float)c, sm.y);
+    const uint32_t byte = row[is_v ? v_place<V>(slot, e0, j) : k_at + j / 4 * (ROW / 4) + j % 4];
+    x[j] = fmaf(sm.x, (float)(high ? byte >> 4 : byte & 15), sm.y);
   }
-  row_store<V>(is_v ? v_out : k_out, ((long long)tok * kv.hkv + h) * HD + e0, out_type, x);
+  RawRow<TYPE, V> y;
+  y.put(x);
+  y.store(is_v ? v_out : k_out, ((long long)tok * kv.hkv + h) * HD + e0, vec);
 }
 
 }  // namespace b200lm

@@ -76,18 +76,44 @@ static RowArgs row_args(const void* qkv, int type, int64_t stride, int tokens, i
   return a;
 }
 
-template <bool APPEND>
-static void launch_rows(cudaStream_t st, RowArgs a, int hd, int sms) {
-  const int heads = a.hq + (APPEND ? 2 : 1) * a.hkv;
-  // one head a warp while that does not fill the GPU, more where the token's rotation row would be read too often
-  a.heads_per_warp = 1;
-  while (a.heads_per_warp < 8 && (long long)a.tokens * heads / a.heads_per_warp > 64ll * sms) a.heads_per_warp *= 2;
-  const long long jobs = (long long)a.tokens * ((heads + a.heads_per_warp - 1) / a.heads_per_warp);
-  B2_CHECK((jobs + 3) / 4 <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
-  const dim3 grid((unsigned)((jobs + 3) / 4));
-  if (hd == 64) launch_pdl(qk_norm_rope_kernel<64, APPEND>, grid, dim3(128), 0, st, a);
-  else if (hd == 128) launch_pdl(qk_norm_rope_kernel<128, APPEND>, grid, dim3(128), 0, st, a);
-  else launch_pdl(qk_norm_rope_kernel<256, APPEND>, grid, dim3(128), 0, st, a);
+template <int HD, int TYPE, int GROUP>
+static void launch_rows_as(cudaStream_t st, const RowArgs& a, int sms) {
+  auto jobs = [&](int n) { return (long long)a.tokens * ((a.hq + n - 1) / n + (GROUP ? 2 : 1) * ((a.hkv + n - 1) / n)); };
+  B2_CHECK(jobs(1) <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
+  // one head a warp while that leaves room on the GPU (a token's chain of latencies), else four: rotation and gains are read less often
+  const bool few = jobs(1) <= 16ll * sms;
+  const dim3 grid((unsigned)((jobs(few ? 1 : 4) + 3) / 4));
+  if (few) launch_pdl(qk_norm_rope_kernel<HD, TYPE, GROUP, 1>, grid, dim3(128), 0, st, a);
+  else launch_pdl(qk_norm_rope_kernel<HD, TYPE, GROUP, 4>, grid, dim3(128), 0, st, a);
+}
+template <int HD, int GROUP>
+static void launch_rows_type(cudaStream_t st, const RowArgs& a, int sms) {
+  if (a.type == kF32) launch_rows_as<HD, kF32, GROUP>(st, a, sms);
+  else if (a.type == kBf16) launch_rows_as<HD, kBf16, GROUP>(st, a, sms);
+  else launch_rows_as<HD, kF16, GROUP>(st, a, sms);
+}
+// group 0: keys are written out.
+static void launch_rows(cudaStream_t st, RowArgs a, int hd, int group, int sms) {
+  const int esz = elem_size(a.type);
+  auto aligned = [&](const void* p, long long stride) { return ((uintptr_t)p | (uintptr_t)(stride * esz)) % 16 == 0; };
+  a.vec = aligned(a.qkv, a.stride);
+  a.vec_q = aligned(a.q_out, a.q_stride);
+  a.vec_k = aligned(a.k_out, a.k_stride);
+  if (hd == 64) group ? launch_rows_type<64, 64>(st, a, sms) : launch_rows_type<64, 0>(st, a, sms);
+  else if (hd == 128) group == 64 ? launch_rows_type<128, 64>(st, a, sms) : group ? launch_rows_type<128, 128>(st, a, sms) : launch_rows_type<128, 0>(st, a, sms);
+  else group == 64 ? launch_rows_type<256, 64>(st, a, sms) : group ? launch_rows_type<256, 128>(st, a, sms) : launch_rows_type<256, 0>(st, a, sms);
+}
+
+template <int HD, int GROUP, int TYPE>
+static void launch_read_as(cudaStream_t st, dim3 grid, const Kv4Args& kv, const int* seq, const int* pos, int tokens, void* k, void* v, int* status) {
+  const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+  launch_pdl(kv4_read_kernel<HD, TYPE, GROUP>, grid, dim3(128), 0, st, kv, seq, pos, tokens, k, v, vec, status);
+}
+template <int HD, int GROUP, typename... A>
+static void launch_read(cudaStream_t st, dim3 grid, int type, const A&... x) {
+  if (type == kF32) launch_read_as<HD, GROUP, kF32>(st, grid, x...);
+  else if (type == kBf16) launch_read_as<HD, GROUP, kBf16>(st, grid, x...);
+  else launch_read_as<HD, GROUP, kF16>(st, grid, x...);
 }
 
 void launch_kv4_attn_64(cudaStream_t st, const Kv4AttnArgs& a, int rb);
@@ -171,7 +197,7 @@ extern "C" int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t
   require_device(device);
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
-  launch_rows<false>(reinterpret_cast<cudaStream_t>(stream), a, hd, device_sms(device));
+  launch_rows(reinterpret_cast<cudaStream_t>(stream), a, hd, 0, device_sms(device));
   KV4_END
 }
 
@@ -191,7 +217,7 @@ extern "C" int B200LmOps_QkNormRopeAppendKv4(int32_t device, const void* qkv_dev
   require_device(device);
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
-  launch_rows<true>(reinterpret_cast<cudaStream_t>(stream), a, hd, device_sms(device));
+  launch_rows(reinterpret_cast<cudaStream_t>(stream), a, hd, cache->group, device_sms(device));
   KV4_END
 }
 
@@ -210,15 +236,18 @@ extern "C" int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, co
   check_pointer(pos_dev, 4, "pos_dev");
   B2_CHECK(seq_dev || tokens <= cache->batch, kInvalidArgument, "more tokens than sequences: seq_dev says whose they are");
   const long long jobs = (long long)tokens * kv.hkv * ((k_out_dev != nullptr) + (v_out_dev != nullptr));
-  B2_CHECK((jobs + 3) / 4 <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
+  B2_CHECK(jobs <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
   require_device(device);
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)((jobs + 3) / 4));
-  if (kv.d.hd == 64) launch_pdl(kv4_read_kernel<64>, grid, dim3(128), 0, st, kv, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev);
-  else if (kv.d.hd == 128) launch_pdl(kv4_read_kernel<128>, grid, dim3(128), 0, st, kv, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev);
-  else launch_pdl(kv4_read_kernel<256>, grid, dim3(128), 0, st, kv, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev);
+  const auto read = kv.d.hd == 64 ? launch_read<64, 64, Kv4Args, const int*, const int*, int, void*, void*, int*>
+                    : kv.d.hd == 128 ? (kv.d.group == 64 ? launch_read<128, 64, Kv4Args, const int*, const int*, int, void*, void*, int*>
+                                                         : launch_read<128, 128, Kv4Args, const int*, const int*, int, void*, void*, int*>)
+                                     : (kv.d.group == 64 ? launch_read<256, 64, Kv4Args, const int*, const int*, int, void*, void*, int*>
+                                                         : launch_read<256, 128, Kv4Args, const int*, const int*, int, void*, void*, int*>);
+  read(st, grid, out_type, kv, seq_dev, pos_dev, tokens, k_out_dev, v_out_dev, status_dev);
   KV4_END
 }
 
