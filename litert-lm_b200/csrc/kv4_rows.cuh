@@ -5,9 +5,10 @@
 //   m = fp16(low), s = fp16((high - low) / 15), code = rint((x - m) / s) held to 0 .. 15
 //
 // Every byte is read and written once: what bounds it is HBM for many tokens, one chain of latencies (row, two warp sums,
-// table row) for a few.  A warp takes up to four heads of one kind and token, asks for their rows at once and keeps gain and
-// rotation multiplied in registers; a lane holds hd / 32 neighbouring elements, so that the other half of a pair lies at the
-// same place of a lane rot / hd * 16 further and comes from there as it lay in memory.
+// table row) for a few.  A lane holds eight neighbouring elements, so a pass of a warp takes 1, 2 or 4 heads (of 256, 128,
+// 64); the other halves of the pairs lie at the same place of a lane rot / 16 further and come from there as they lay in memory.  A
+// warp takes up to four passes over heads of one kind and token, asks for their rows at once and keeps gain and rotation
+// multiplied in registers.
 // Queries are computed in fp32.  Keys that go into the cache are computed in fp64 and rounded to fp32 before their
 // codes are decided: a code next to a border would otherwise depend on the order of the sum, and one step of a code is a
 // fifteenth of the group's range.
@@ -44,7 +45,6 @@ struct RowArgs {
   long long k_stride;
   const int* seq;
   Kv4Args kv;
-  bool vec, vec_q, vec_k;      // rows of qkv, q_out, k_out start on 16-byte boundaries
   int* status;
 };
 
@@ -52,10 +52,10 @@ __device__ __forceinline__ void set_status(int* status, int code) {
   if (status) atomicMax(status, code);
 }
 
-// V neighbouring elements of a row as they lie in memory: whole words where the row starts allow it (`vec`), else one by one.
-template <int TYPE, int V>
+// W neighbouring elements of a row as they lie in memory: whole words where the row starts allow it (`vec`), else one by one.
+template <int TYPE, int W>
 struct RawRow {
-  static constexpr int N = TYPE == kF32 ? V : V / 2;
+  static constexpr int N = TYPE == kF32 ? W : W / 2;
   uint32_t u[N];
   __device__ __forceinline__ void load(const void* p, long long i, bool vec) {
     const char* a = reinterpret_cast<const char*>(p) + i * elem_size(TYPE);
@@ -102,7 +102,7 @@ struct RawRow {
       }
     }
   }
-  __device__ __forceinline__ void get(float (&x)[V]) const {
+  __device__ __forceinline__ void get(float (&x)[W]) const {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if constexpr (TYPE == kF32) x[j] = __uint_as_float(u[j]);
@@ -113,7 +113,7 @@ struct RawRow {
       }
     }
   }
-  __device__ __forceinline__ void put(const float (&x)[V]) {
+  __device__ __forceinline__ void put(const float (&x)[W]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if constexpr (TYPE == kF32) u[j] = __float_as_uint(x[j]);
@@ -127,117 +127,143 @@ struct RawRow {
     }
   }
 };
-template <int V>
-__device__ __forceinline__ void row_load(const void* p, long long i, int type, float (&x)[V]) {
+template <int W>
+__device__ __forceinline__ void row_load(const void* p, long long i, int type, float (&x)[W]) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p) + i * elem_size(type);
   auto as = [&](auto raw) {
     constexpr int bytes = 4 * decltype(raw)::N;
     raw.load(p, i, at % (bytes < 16 ? bytes : 16) == 0);
     raw.get(x);
   };
-  if (type == kF32) as(RawRow<kF32, V>());
-  else if (type == kBf16) as(RawRow<kBf16, V>());
-  else as(RawRow<kF16, V>());
+  if (type == kF32) as(RawRow<kF32, W>());
+  else if (type == kBf16) as(RawRow<kBf16, W>());
+  else as(RawRow<kF16, W>());
 }
 
-// Norm and rotation of the V elements x that this lane holds of a head, `other` being those of the lane with the other halves of the
+constexpr int kVec = 8;             // elements of a lane
+
+// Norm and rotation of the elements x that this lane holds of a head, `other` being those of the lane with the other halves of the
 // pairs: y = inv (x ca + other sb), ca = gain * cos, sb = +- the other's gain * sin.
-template <typename T, int V>
-__device__ __forceinline__ void norm_rotate(const float (&x)[V], const float (&other)[V], bool norm, float eps, const T (&ca)[V], const T (&sb)[V], bool rotates, T (&y)[V]) {
-  constexpr int HD = 32 * V;
+template <typename T, int HD>
+__device__ __forceinline__ void norm_rotate(const float (&x)[kVec], const float (&other)[kVec], bool norm, float eps, const T (&ca)[kVec], const T (&sb)[kVec], bool rotates, T (&y)[kVec]) {
   T inv = 1;
   if (norm) {
     T sum = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum += (T)x[j] * (T)x[j];
+    for (int j = 0; j < kVec; ++j) sum += (T)x[j] * (T)x[j];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = HD / kVec / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const T mean = sum * (T)(1.0 / HD) + (T)eps;
     inv = rsqrtf((float)mean);
     if constexpr (sizeof(T) == 8) inv = inv * (1.5 - 0.5 * mean * inv * inv);      // 2^-22 -> 2^-43
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
+  for (int j = 0; j < kVec; ++j) {
     y[j] = (T)x[j] * ca[j];
     if (rotates) y[j] += (T)other[j] * sb[j];
     y[j] *= inv;
   }
 }
 
-// Codes of the group that this lane's V elements lie in (GL lanes of it); returns the pair (s, m) as fp16 bits.
-template <int V, int GL>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[V], uint32_t (&code)[V]) {
+// What fp64 says where fp32 leaves it open; kept out of the loops, which it would push out of the instruction cache.
+static __device__ __noinline__ float step64(float low, float high) { return (float)(((double)high - (double)low) / 15.0); }
+static __device__ __noinline__ uint32_t code64(float x, float m, float s) { return s == 0.f ? 0u : (uint32_t)fmin(fmax(rint(((double)x - (double)m) / (double)s), 0.0), 15.0); }
+
+// Codes, a byte each, of this lane's elements, GL lanes being a group; returns the pair (s, m) as fp16 bits.
+template <int GL>
+__device__ __forceinline__ uint32_t quantise(const float (&x)[kVec], uint32_t (&word)[2]) {
   float low = x[0], high = x[0];
   bool nan = x[0] != x[0];
 #pragma unroll
-  for (int j = 1; j < V; ++j) {
+  for (int j = 1; j < kVec; ++j) {
     low = fminf(low, x[j]);
     high = fmaxf(high, x[j]);
     nan = nan || x[j] != x[j];
   }
   if (nan) high = INFINITY;                                // the comparisons pass a NaN over
-  if constexpr (GL == 32) {                                // one instruction for the whole warp
-    asm volatile("redux.sync.min.f32 %0, %0, 0xffffffff;" : "+f"(low));
-    asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(high));
-  } else {
 #pragma unroll
-    for (int o = 1; o < GL; o <<= 1) {
-      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-    }
+  for (int o = 1; o < GL; o <<= 1) {
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
   }
   const bool bad = !isfinite(low) || !isfinite(high);
   constexpr float top = 65504.f;                           // fp16's largest
   const __half m = __float2half_rn(fminf(fmaxf(low, -top), top));
-  const __half s = __float2half_rn(fminf((float)(((double)high - (double)low) / 15.0), top));
-  const float mf = __half2float(m), sf = __half2float(s), inv = sf > 0.f ? 1.f / sf : 0.f;
+  // (high - low) / 15 in fp32 is off by at most 2^-22 of itself: where that could lead to another fp16 number, fp64 decides
+  const float step = (high - low) * (1.f / 15.f);
+  __half s = __float2half_rn(fminf(step, top));
+  if (!bad && (__half_as_ushort(__float2half_rn(step * (1.f - 3e-7f))) != __half_as_ushort(__float2half_rn(step * (1.f + 3e-7f)))))
+    s = __float2half_rn(fminf(step64(low, high), top));
+  const float mf = __half2float(m), sf = __half2float(s), inv = sf > 0.f ? __fdividef(1.f, sf) : 0.f;
+  constexpr float whole = 12582912.f;                      // 1.5 * 2^23: adding it rounds, and leaves a code in the lowest byte
+  float r[kVec], near = 0.f;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    // three roundings leave a code below 16 off by at most 3 * 2^-24 * 16 = 3e-6: nearer to a border than that fp64 decides
-    const float c = (x[j] - mf) * inv, whole = rintf(c);
-    float decided = whole;
-    if (fabsf(fabsf(c - whole) - 0.5f) < 1e-5f && sf > 0.f) decided = (float)rint(((double)x[j] - (double)mf) / (double)sf);
-    code[j] = bad ? 0u : (uint32_t)fminf(fmaxf(decided, 0.f), 15.f);
+  for (int j = 0; j < kVec; ++j) {
+    const float from = x[j] - mf;
+    r[j] = fmaf(from, inv, whole);
+    near = fmaxf(near, fabsf(fmaf(from, inv, whole - r[j])));
+    r[j] = fminf(fmaxf(r[j], whole), whole + 15.f);
   }
-  if (bad) return 0x7E007E00u;                             // NaN, NaN
-  return (uint32_t)__half_as_ushort(s) | (uint32_t)__half_as_ushort(m) << 16;
-}
-
-// Byte of element e0 + j (e0 = lane V) of a V row whose planes lie one behind the other.
-template <int V>
-__device__ __forceinline__ int v_place(int slot, int e0, int j) {
-  constexpr int PL = V >= 4 ? 128 : 64, ROW = PL / 2;
-  const int turn = PL == 128 ? 4 * (slot >> 1 & 1) : 0;
-  return e0 / PL * ROW + ((e0 + j) % 8 ^ turn) * (ROW / 8) + e0 % PL / 16;
-}
-
-// Writes a row's codes; `stage` is the warp's own.  Of K a lane has the bytes of whole words (elements 16 apart share a byte, four
-// neighbours a word).  Of V, neighbours lie in different units: the row is put together in shared memory first.
-template <int V>
-__device__ __forceinline__ void put_codes(uint8_t* codes, const Kv4Dims& d, int slot, bool is_v, int lane, const uint32_t (&code)[V], uint8_t* stage) {
-  const int e0 = lane * V, apart = (is_v ? 8 : 16) / V;
-  uint32_t byte[V];
+  // the quotient, three roundings off, is off by at most 2^-21 of 16: nearer to a border than 1e-5 fp64 decides.  (Far outside
+  // 0 .. 15, where fp16 could not tell m from its neighbours, it is held to the range either way.)
+  if (near > 0.5f - 1e-5f && !bad) {
+#pragma unroll 1
+    for (int j = 0; j < kVec; ++j) {
+      float v = x[0];
 #pragma unroll
-  for (int j = 0; j < V; ++j) byte[j] = code[j] | __shfl_down_sync(0xffffffffu, code[j], apart) << 4;
-  if (!is_v) {
-    if (d.k_high(e0)) return;
-    if constexpr (V == 2) {
-      *reinterpret_cast<uint16_t*>(codes + d.k_byte(slot, e0)) = (uint16_t)(byte[0] | byte[1] << 8);
-    } else {
+      for (int i = 1; i < kVec; ++i) v = i == j ? x[i] : v;
+      const float c = whole + (float)code64(v, mf, sf);
 #pragma unroll
-      for (int j = 0; j < V; j += 4)
-        *reinterpret_cast<uint32_t*>(codes + d.k_byte(slot, e0 + j)) = byte[j] | byte[j + 1] << 8 | byte[j + 2] << 16 | byte[j + 3] << 24;
+      for (int i = 0; i < kVec; ++i) r[i] = i == j ? c : r[i];
     }
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t lo = __byte_perm(__float_as_uint(r[4 * q]), __float_as_uint(r[4 * q + 1]), 0x0040), hi = __byte_perm(__float_as_uint(r[4 * q + 2]), __float_as_uint(r[4 * q + 3]), 0x0040);
+    word[q] = bad ? 0u : __byte_perm(lo, hi, 0x5410);
+  }
+  return bad ? 0x7E007E00u : (uint32_t)__half_as_ushort(s) | (uint32_t)__half_as_ushort(m) << 16;     // NaN, NaN
+}
+
+// Places of the element e0 = 8 i in a K or V row whose planes lie one behind the other: K has the bytes of its neighbours in two
+// words a quarter of a plane's row apart, V has them in the same byte of eight units (`place` of the first four, of the others).
+template <int HD>
+__device__ __forceinline__ uint32_t k_place(uint32_t e0) {
+  constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2;
+  return e0 / PL * ROW + e0 % 16 / 4 * (ROW / 4) + e0 % PL / 32 * 4;
+}
+template <int HD>
+__device__ __forceinline__ uint32_t v_place(uint32_t slot, uint32_t e0, uint32_t q) {
+  constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2;
+  return e0 / PL * ROW + (4 * q ^ (PL == 128 ? 4 * (slot >> 1 & 1) : 0)) * (ROW / 8) + e0 % PL / 16;
+}
+
+// Writes the codes of the warp's rows, those of lane / (HD / 8) = `sub`; `stage` is the warp's own.  Of K a lane has the bytes of whole
+// words (elements 16 apart share a byte, four neighbours a word).  Of V, neighbours lie in different units: the rows are put
+// together in shared memory first.
+template <int HD>
+__device__ __forceinline__ void put_codes(uint8_t* codes, uint32_t slot, bool is_v, bool active, uint32_t lane, uint32_t (&word)[2], uint8_t* stage) {
+  constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2, LH = HD / kVec;
+  const uint32_t e0 = lane % LH * kVec, apart = is_v ? 1 : 2;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) word[q] |= __shfl_down_sync(0xffffffffu, word[q], apart) << 4;
+  if (!is_v) {
+    if ((e0 & 16) || !active) return;
+    uint8_t* at = codes + slot * ROW + e0 / PL * (kKv4Page - 1) * ROW + k_place<HD>(e0);
+    *reinterpret_cast<uint32_t*>(at) = word[0];
+    *reinterpret_cast<uint32_t*>(at + ROW / 4) = word[1];
     return;
   }
-  constexpr int ROW = V >= 4 ? 64 : 32, HALF = 16 * V;               // bytes of a plane's row, of all planes'
-  __syncwarp();                                                      // the row before has been taken away
-  if (!d.v_high(e0)) {
+  __syncwarp();                                                      // the rows before have been taken away
+  if (!(e0 & 8)) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) stage[v_place<V>(slot, e0, j)] = (uint8_t)byte[j];
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stage[lane / LH * (HD / 2) + v_place<HD>(slot, e0, q) + j * (ROW / 8)] = (uint8_t)(word[q] >> (8 * j));
   }
   __syncwarp();
-  if (lane * 4 < HALF) *reinterpret_cast<uint32_t*>(codes + (lane * 4 / ROW * kKv4Page + slot) * ROW + lane * 4 % ROW) = *reinterpret_cast<const uint32_t*>(stage + lane * 4);
+  const uint32_t at = lane % LH * 4;                                 // a row has HD / 2 = 4 LH bytes
+  if (active) *reinterpret_cast<uint32_t*>(codes + (at / ROW * kKv4Page + slot) * ROW + at % ROW) = *reinterpret_cast<const uint32_t*>(stage + lane * 4);
 }
 
 // Physical page of (sequence, position), or null (and the status set) where there is none.
@@ -248,12 +274,20 @@ __device__ __forceinline__ uint8_t* kv4_page(const Kv4Args& kv, int seq, int pos
   return kv.pages + (long long)page * kv.hkv * kv.d.head_bytes();
 }
 
-// NH heads of one kind and token a warp; GROUP 0: keys are written out, else keys and values go into the cache.
-template <int HD, int TYPE, int GROUP, int NH>
-__global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
-  constexpr int V = HD / 32;
+template <bool VEC>
+__device__ __forceinline__ void table_row(const float* p, long long i, float (&x)[kVec]) {
+  RawRow<kF32, kVec> r;
+  r.load(p, i, VEC);
+  r.get(x);
+}
+
+// NP passes of 256 / HD heads of one kind and token a warp; GROUP 0: keys are written out, else keys and values go into the cache.
+// VEC: all rows and tables start on 16-byte boundaries.
+template <int HD, int TYPE, int GROUP, int NP, bool VEC>
+__global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const RowArgs a) {
+  constexpr int LH = HD / kVec, HP = 32 / LH, NH = NP * HP;             // lanes of a head, heads of a pass, of a warp
   constexpr bool APPEND = GROUP > 0;
-  __shared__ __align__(16) uint8_t stage[4][APPEND ? HD / 2 : 16];
+  __shared__ __align__(16) uint8_t stage[4][APPEND ? 128 : 16];
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -263,12 +297,14 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
   const int tok = (int)(job / per), part = (int)(job - tok * per);
   if (tok >= a.tokens) return;
   const bool is_q = part < jq, is_v = APPEND && part >= jq + jk;
-  const int h0 = (is_q ? part : is_v ? part - jq - jk : part - jq) * NH, hn = min(NH, (is_q ? a.hq : a.hkv) - h0), e0 = lane * V;
-  const long long row = tok * a.stride + ((is_q ? 0 : is_v ? a.hq + a.hkv : a.hq) + h0) * HD + e0;
-  RawRow<TYPE, V> raw[NH];
+  // this lane's first head; those behind the last compute the last one's and write nothing
+  const int heads = is_q ? a.hq : a.hkv, h0 = (is_q ? part : is_v ? part - jq - jk : part - jq) * NH, passes = min(NP, (heads - h0 + HP - 1) / HP), mine = h0 + lane / LH;
+  const int e0 = lane % LH * kVec;
+  const long long row = tok * a.stride + (is_q ? 0 : is_v ? a.hq + a.hkv : a.hq) * HD + e0;
+  RawRow<TYPE, kVec> raw[NP];
 #pragma unroll
-  for (int i = 0; i < NH; ++i)
-    if (i < hn) raw[i].load(a.qkv, row + i * HD, a.vec);
+  for (int i = 0; i < NP; ++i)
+    if (i < passes) raw[i].load(a.qkv, row + min(mine + i * HP, heads - 1) * HD, VEC);
   const int pos = a.pos[tok];
   if (pos < 0) return;
   if (a.rot > 0 && pos >= a.rope_rows) { set_status(a.status, kDevBadPosition); return; }
@@ -279,114 +315,124 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const RowArgs a) {
   }
   const int half = a.rot / 2, slot = pos % kKv4Page;
   const bool rotates = e0 < a.rot && !is_v, first = e0 < half;
-  const int other_lane = lane + (rotates ? (first ? half / V : -(half / V)) : 0);
+  const int other_lane = lane + (rotates ? (first ? half / kVec : -(half / kVec)) : 0);
   const bool norm = (is_q ? a.q_gain : a.k_gain) != nullptr && !is_v;
-  float ca[V], sb[V], gain[V];
+  float ca[kVec], sb[kVec], gain[kVec];
 #pragma unroll
-  for (int j = 0; j < V; ++j) ca[j] = gain[j] = 1.f, sb[j] = 0.f;
-  if (norm) row_load<V>(is_q ? a.q_gain : a.k_gain, e0, kF32, gain);
+  for (int j = 0; j < kVec; ++j) ca[j] = gain[j] = 1.f, sb[j] = 0.f;
+  if (norm) table_row<VEC>(is_q ? a.q_gain : a.k_gain, e0, gain);
   if (rotates) {
     const long long i = (long long)pos * half + e0 - (first ? 0 : half);
-    row_load<V>(a.cos, i, kF32, ca);
-    row_load<V>(a.sin, i, kF32, sb);
+    table_row<VEC>(a.cos, i, ca);
+    table_row<VEC>(a.sin, i, sb);
   }
-  auto heads = [&](auto one, auto&& done) {                          // one: a number of the type that norm and rotation are computed in
-    using T = decltype(one);
-    T c[V], s[V];
+  auto next = [&]() {                                                // the bodies of an appending kernel's loops stand once: unrolled, they miss the instruction cache
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int i = 0; i + 1 < NP; ++i) raw[i] = raw[i + 1];
+  };
+  constexpr int kUnroll = APPEND ? 1 : NP;
+  auto normed = [&](auto one, auto&& done) {                          // one: a number of the type that norm and rotation are computed in
+    using T = decltype(one);
+    T c[kVec], s[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
       const float other_gain = __shfl_sync(0xffffffffu, gain[j], other_lane);
       c[j] = (T)ca[j] * (T)gain[j];
       s[j] = (T)(first ? -sb[j] : sb[j]) * (T)other_gain;
     }
+#pragma unroll kUnroll
+    for (int i = 0; i < NP; ++i) {
+      if (i >= passes) break;
+      RawRow<TYPE, kVec> fellow;
 #pragma unroll
-    for (int i = 0; i < NH; ++i) {
-      if (i >= hn) break;
-      RawRow<TYPE, V> fellow;
-#pragma unroll
-      for (int j = 0; j < RawRow<TYPE, V>::N; ++j) fellow.u[j] = __shfl_sync(0xffffffffu, raw[i].u[j], other_lane);
-      float x[V], f[V];
-      raw[i].get(x);
+      for (int j = 0; j < RawRow<TYPE, kVec>::N; ++j) fellow.u[j] = __shfl_sync(0xffffffffu, raw[0].u[j], other_lane);
+      float x[kVec], f[kVec];
+      raw[0].get(x);
       fellow.get(f);
-      T y[V];
-      norm_rotate<T, V>(x, f, norm, a.eps, c, s, rotates, y);
+      T y[kVec];
+      norm_rotate<T, HD>(x, f, norm, a.eps, c, s, rotates, y);
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = (float)y[j];
+      for (int j = 0; j < kVec; ++j) x[j] = (float)y[j];
       done(i, x);
+      next();
     }
   };
   if (is_q || !APPEND) {
     void* out = is_q ? a.q_out : a.k_out;
-    const long long at = tok * (is_q ? a.q_stride : a.k_stride) + h0 * HD + e0;
-    const bool vec = is_q ? a.vec_q : a.vec_k;
-    heads(1.f, [&](int i, const float (&x)[V]) {
-      RawRow<TYPE, V> y;
+    const long long at = tok * (is_q ? a.q_stride : a.k_stride) + e0;
+    normed(1.f, [&](int i, const float (&x)[kVec]) {
+      RawRow<TYPE, kVec> y;
       y.put(x);
-      y.store(out, at + i * HD, vec);
+      if (mine + i * HP < heads) y.store(out, at + (mine + i * HP) * HD, VEC);
     });
   }
   if constexpr (APPEND) {
     constexpr Kv4Dims d{HD, GROUP};
-    constexpr int gl = GROUP / V;
-    auto put = [&](int i, const float (&x)[V]) {
-      uint8_t* head = page + (long long)(h0 + i) * d.head_bytes();
-      uint32_t code[V];
-      const uint32_t pair = quantise<V, gl>(x, code);
-      put_codes<V>(head + (is_v ? d.v_codes() : d.k_codes()), d, slot, is_v, lane, code, stage[threadIdx.x >> 5]);
-      if (lane % gl == 0) reinterpret_cast<uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + lane / gl] = pair;
+    constexpr int GL = GROUP / kVec;
+    auto put = [&](int i, const float (&x)[kVec]) {
+      const int h = mine + i * HP;
+      uint8_t* head = page + (long long)h * d.head_bytes();
+      uint32_t word[2];
+      const uint32_t pair = quantise<GL>(x, word);
+      put_codes<HD>(head + (is_v ? d.v_codes() : d.k_codes()), slot, is_v, h < heads, lane, word, stage[threadIdx.x >> 5]);
+      if (lane % GL == 0 && h < heads) reinterpret_cast<uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + lane % LH / GL] = pair;
     };
     if (is_v) {
-#pragma unroll
-      for (int i = 0; i < NH; ++i) {
-        if (i >= hn) break;
-        float x[V];
-        raw[i].get(x);
+#pragma unroll 1
+      for (int i = 0; i < passes; ++i) {
+        float x[kVec];
+        raw[0].get(x);
         put(i, x);
+        next();
       }
     } else if (!is_q) {
-      heads(1.0, put);
+      normed(1.0, put);
     }
   }
 }
 
-// A warp per (token, kv head, K or V); a lane reads the bytes of V elements and their fellows.
-template <int HD, int TYPE, int GROUP>
-__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const int* __restrict__ seq, const int* __restrict__ pos, int tokens, void* k_out, void* v_out, bool vec, int* status) {
-  constexpr int V = HD / 32;
+// 256 / HD kv heads of a token a warp, K and V of each.
+template <int HD, int TYPE, int GROUP, bool VEC>
+__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const int* __restrict__ seq, const int* __restrict__ pos, int tokens, void* k_out, void* v_out, int* status) {
+  constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2;
+  constexpr int LH = HD / kVec, HP = 32 / LH;
+  constexpr Kv4Dims d{HD, GROUP};
+  __shared__ __align__(16) uint8_t stage[4][128];
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, sides = (k_out != nullptr) + (v_out != nullptr);
-  const uint32_t per = sides * kv.hkv, job = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int tok = (int)(job / per), part = (int)(job - tok * per), h = sides == 2 ? part >> 1 : part;
+  const uint32_t lane = threadIdx.x & 31, e0 = lane % LH * kVec, per = (kv.hkv + HP - 1) / HP, job = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int tok = (int)(job / per), h = (int)(job - tok * per) * HP + lane / LH;
   if (tok >= tokens) return;
-  const bool is_v = k_out == nullptr || (sides == 2 && (part & 1));
   const int p = pos[tok];
   if (p < 0) return;
   const uint8_t* page = kv4_page(kv, seq ? seq[tok] : tok, p, status);
   if (!page) return;
-  constexpr Kv4Dims d{HD, GROUP};
-  const uint8_t* head = page + (long long)h * d.head_bytes();
-  const uint8_t* codes = head + (is_v ? d.v_codes() : d.k_codes());
-  const int slot = p % kKv4Page, e0 = lane * V;
-  const uint32_t pair = reinterpret_cast<const uint32_t*>(head + (is_v ? d.v_scales() : d.k_scales()))[slot * d.groups() + e0 / d.group];
-  const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&pair));
-  // the row's bytes come in words; V's neighbours lie in different units and are picked from shared memory
-  constexpr int ROW = V >= 4 ? 64 : 32;
-  __shared__ __align__(16) uint8_t stage[4][HD / 2];
-  uint8_t* row = stage[threadIdx.x >> 5];
-  if (lane * 8 < HD) reinterpret_cast<uint32_t*>(row)[lane] = *reinterpret_cast<const uint32_t*>(codes + (lane * 4 / ROW * kKv4Page + slot) * ROW + lane * 4 % ROW);
+  const uint32_t slot = p % kKv4Page, at = lane % LH * 4;
+  const uint8_t* head = page + (long long)min(h, kv.hkv - 1) * d.head_bytes();
+  const uint8_t* k = head + d.k_codes() + slot * ROW + e0 / PL * (kKv4Page - 1) * ROW + k_place<HD>(e0 & ~16u);
+  uint32_t kw[2] = {*reinterpret_cast<const uint32_t*>(k), *reinterpret_cast<const uint32_t*>(k + ROW / 4)};
+  uint8_t* row = stage[threadIdx.x >> 5] + lane / LH * (HD / 2);
+  *reinterpret_cast<uint32_t*>(row + at) = *reinterpret_cast<const uint32_t*>(head + d.v_codes() + (at / ROW * kKv4Page + slot) * ROW + at % ROW);
+  const uint32_t ks = reinterpret_cast<const uint32_t*>(head + d.k_scales())[slot * d.groups() + e0 / GROUP];
+  const uint32_t vs = reinterpret_cast<const uint32_t*>(head + d.v_scales())[slot * d.groups() + e0 / GROUP];
   __syncwarp();
-  float x[V];
-  const int k_at = e0 / (2 * ROW) * ROW + e0 % 16 / 4 * (ROW / 4) + e0 % (2 * ROW) / 32 * 4 + e0 % 4;     // and 4 neighbours, the next 4 a quarter row on
-  const bool high = is_v ? d.v_high(e0) : d.k_high(e0);
+  if (h >= kv.hkv) return;
+  auto write = [&](void* out, uint32_t pair, const uint32_t (&word)[2], uint32_t shift) {
+    const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    float x[kVec];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const uint32_t byte = row[is_v ? v_place<V>(slot, e0, j) : k_at + j / 4 * (ROW / 4) + j % 4];
-    x[j] = fmaf(sm.x, (float)(high ? byte >> 4 : byte & 15), sm.y);
+    for (int j = 0; j < kVec; ++j) x[j] = fmaf(sm.x, (float)(word[j / 4] >> (8 * (j % 4) + shift) & 15u), sm.y);
+    RawRow<TYPE, kVec> y;
+    y.put(x);
+    y.store(out, ((long long)tok * kv.hkv + h) * HD + e0, VEC);
+  };
+  if (k_out) write(k_out, ks, kw, e0 & 16 ? 4 : 0);
+  if (v_out) {                                             // neighbours lie in different units: a byte of each
+    uint32_t word[2] = {};
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) word[j / 4] |= (uint32_t)row[v_place<HD>(slot, e0, j / 4) + j % 4 * (ROW / 8)] << (8 * (j % 4));
+    write(v_out, vs, word, e0 & 8 ? 4 : 0);
   }
-  RawRow<TYPE, V> y;
-  y.put(x);
-  y.store(is_v ? v_out : k_out, ((long long)tok * kv.hkv + h) * HD + e0, vec);
 }
 
 }  // namespace b200lm

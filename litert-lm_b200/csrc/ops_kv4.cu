@@ -56,7 +56,7 @@ static RowArgs row_args(const void* qkv, int type, int64_t stride, int tokens, i
   check_query_heads(hq);
   B2_CHECK(tokens >= 0, kInvalidArgument, "tokens is negative");
   B2_CHECK(stride >= (int64_t)(hq + 2 * hkv) * hd && q_stride >= (int64_t)hq * hd, kInvalidArgument, "a row stride is shorter than its row");
-  B2_CHECK(rot >= 0 && rot <= hd && rot % (hd / 16) == 0, kInvalidArgument, "rot must be a multiple of hd / 16 up to hd");
+  B2_CHECK(rot >= 0 && rot <= hd && rot % 16 == 0, kInvalidArgument, "rot must be a multiple of 16 up to hd");
   B2_CHECK(eps >= 0.f, kInvalidArgument, "eps must not be negative");
   check_pointer(qkv, elem_size(type), "qkv_dev");
   check_pointer(q_out, elem_size(type), "q_out_dev");
@@ -76,15 +76,22 @@ static RowArgs row_args(const void* qkv, int type, int64_t stride, int tokens, i
   return a;
 }
 
+template <int HD, int TYPE, int GROUP, int NP, bool VEC>
+static void launch_rows_at(cudaStream_t st, const RowArgs& a) {
+  const int n = NP * (256 / HD);
+  const long long jobs = (long long)a.tokens * ((a.hq + n - 1) / n + (GROUP ? 2 : 1) * ((a.hkv + n - 1) / n));
+  B2_CHECK(jobs <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
+  launch_pdl(qk_norm_rope_kernel<HD, TYPE, GROUP, NP, VEC>, dim3((unsigned)((jobs + 3) / 4)), dim3(128), 0, st, a);
+}
 template <int HD, int TYPE, int GROUP>
 static void launch_rows_as(cudaStream_t st, const RowArgs& a, int sms) {
-  auto jobs = [&](int n) { return (long long)a.tokens * ((a.hq + n - 1) / n + (GROUP ? 2 : 1) * ((a.hkv + n - 1) / n)); };
-  B2_CHECK(jobs(1) <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
-  // one head a warp while that leaves room on the GPU (a token's chain of latencies), else four: rotation and gains are read less often
-  const bool few = jobs(1) <= 16ll * sms;
-  const dim3 grid((unsigned)((jobs(few ? 1 : 4) + 3) / 4));
-  if (few) launch_pdl(qk_norm_rope_kernel<HD, TYPE, GROUP, 1>, grid, dim3(128), 0, st, a);
-  else launch_pdl(qk_norm_rope_kernel<HD, TYPE, GROUP, 4>, grid, dim3(128), 0, st, a);
+  const int esz = elem_size(a.type);
+  const uintptr_t all = (uintptr_t)a.qkv | (uintptr_t)(a.stride * esz) | (uintptr_t)a.q_out | (uintptr_t)(a.q_stride * esz) | (uintptr_t)a.k_out | (uintptr_t)(a.k_stride * esz) |
+                        (uintptr_t)a.q_gain | (uintptr_t)a.k_gain | (a.rot ? (uintptr_t)a.cos | (uintptr_t)a.sin : 0);
+  // one pass a warp while that leaves room on the GPU (a token's chain of latencies), else four: rotation and gains are read less often
+  if (all % 16 != 0) launch_rows_at<HD, TYPE, GROUP, 1, false>(st, a);
+  else if ((long long)a.tokens * (a.hq + 2 * a.hkv) <= 16ll * sms) launch_rows_at<HD, TYPE, GROUP, 1, true>(st, a);
+  else launch_rows_at<HD, TYPE, GROUP, 4, true>(st, a);
 }
 template <int HD, int GROUP>
 static void launch_rows_type(cudaStream_t st, const RowArgs& a, int sms) {
@@ -93,27 +100,26 @@ static void launch_rows_type(cudaStream_t st, const RowArgs& a, int sms) {
   else launch_rows_as<HD, kF16, GROUP>(st, a, sms);
 }
 // group 0: keys are written out.
-static void launch_rows(cudaStream_t st, RowArgs a, int hd, int group, int sms) {
-  const int esz = elem_size(a.type);
-  auto aligned = [&](const void* p, long long stride) { return ((uintptr_t)p | (uintptr_t)(stride * esz)) % 16 == 0; };
-  a.vec = aligned(a.qkv, a.stride);
-  a.vec_q = aligned(a.q_out, a.q_stride);
-  a.vec_k = aligned(a.k_out, a.k_stride);
+static void launch_rows(cudaStream_t st, const RowArgs& a, int hd, int group, int sms) {
   if (hd == 64) group ? launch_rows_type<64, 64>(st, a, sms) : launch_rows_type<64, 0>(st, a, sms);
   else if (hd == 128) group == 64 ? launch_rows_type<128, 64>(st, a, sms) : group ? launch_rows_type<128, 128>(st, a, sms) : launch_rows_type<128, 0>(st, a, sms);
   else group == 64 ? launch_rows_type<256, 64>(st, a, sms) : group ? launch_rows_type<256, 128>(st, a, sms) : launch_rows_type<256, 0>(st, a, sms);
 }
 
 template <int HD, int GROUP, int TYPE>
-static void launch_read_as(cudaStream_t st, dim3 grid, const Kv4Args& kv, const int* seq, const int* pos, int tokens, void* k, void* v, int* status) {
-  const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
-  launch_pdl(kv4_read_kernel<HD, TYPE, GROUP>, grid, dim3(128), 0, st, kv, seq, pos, tokens, k, v, vec, status);
+static void launch_read_as(cudaStream_t st, const Kv4Args& kv, const int* seq, const int* pos, int tokens, void* k, void* v, int* status) {
+  const int n = 256 / HD;
+  const long long jobs = (long long)tokens * ((kv.hkv + n - 1) / n);
+  B2_CHECK(jobs <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
+  const dim3 grid((unsigned)((jobs + 3) / 4));
+  if (((uintptr_t)k | (uintptr_t)v) % 16 == 0) launch_pdl(kv4_read_kernel<HD, TYPE, GROUP, true>, grid, dim3(128), 0, st, kv, seq, pos, tokens, k, v, status);
+  else launch_pdl(kv4_read_kernel<HD, TYPE, GROUP, false>, grid, dim3(128), 0, st, kv, seq, pos, tokens, k, v, status);
 }
-template <int HD, int GROUP, typename... A>
-static void launch_read(cudaStream_t st, dim3 grid, int type, const A&... x) {
-  if (type == kF32) launch_read_as<HD, GROUP, kF32>(st, grid, x...);
-  else if (type == kBf16) launch_read_as<HD, GROUP, kBf16>(st, grid, x...);
-  else launch_read_as<HD, GROUP, kF16>(st, grid, x...);
+template <int HD, int GROUP>
+static void launch_read(cudaStream_t st, int type, const Kv4Args& kv, const int* seq, const int* pos, int tokens, void* k, void* v, int* status) {
+  if (type == kF32) launch_read_as<HD, GROUP, kF32>(st, kv, seq, pos, tokens, k, v, status);
+  else if (type == kBf16) launch_read_as<HD, GROUP, kBf16>(st, kv, seq, pos, tokens, k, v, status);
+  else launch_read_as<HD, GROUP, kF16>(st, kv, seq, pos, tokens, k, v, status);
 }
 
 void launch_kv4_attn_64(cudaStream_t st, const Kv4AttnArgs& a, int rb);
@@ -235,19 +241,12 @@ extern "C" int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, co
   check_optional(status_dev, 4, "status_dev");
   check_pointer(pos_dev, 4, "pos_dev");
   B2_CHECK(seq_dev || tokens <= cache->batch, kInvalidArgument, "more tokens than sequences: seq_dev says whose they are");
-  const long long jobs = (long long)tokens * kv.hkv * ((k_out_dev != nullptr) + (v_out_dev != nullptr));
-  B2_CHECK(jobs <= 0x7FFFFFFF, kInvalidArgument, "too many tokens for one call");
   require_device(device);
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid((unsigned)((jobs + 3) / 4));
-  const auto read = kv.d.hd == 64 ? launch_read<64, 64, Kv4Args, const int*, const int*, int, void*, void*, int*>
-                    : kv.d.hd == 128 ? (kv.d.group == 64 ? launch_read<128, 64, Kv4Args, const int*, const int*, int, void*, void*, int*>
-                                                         : launch_read<128, 128, Kv4Args, const int*, const int*, int, void*, void*, int*>)
-                                     : (kv.d.group == 64 ? launch_read<256, 64, Kv4Args, const int*, const int*, int, void*, void*, int*>
-                                                         : launch_read<256, 128, Kv4Args, const int*, const int*, int, void*, void*, int*>);
-  read(st, grid, out_type, kv, seq_dev, pos_dev, tokens, k_out_dev, v_out_dev, status_dev);
+  const auto read = kv.d.hd == 64 ? launch_read<64, 64> : kv.d.hd == 128 ? (kv.d.group == 64 ? launch_read<128, 64> : launch_read<128, 128>) : kv.d.group == 64 ? launch_read<256, 64> : launch_read<256, 128>;
+  read(st, out_type, kv, seq_dev, pos_dev, tokens, k_out_dev, v_out_dev, status_dev);
   KV4_END
 }
 

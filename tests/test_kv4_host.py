@@ -76,7 +76,7 @@ def test_gemv_refusals(pkg):
 def test_rows_refusals(pkg):
     ok = dict(qkv_dev=P, type=1, qkv_stride=768, tokens=3, hq=4, hkv=1, hd=128, rot=128, q_gain_dev=P, k_gain_dev=P, eps=1e-6, cos_dev=P, sin_dev=P, rope_rows=10, pos_dev=P, q_out_dev=P, q_stride=512)
     f = lambda **kw: pkg.ops.qk_norm_rope(**{**ok, "k_out_dev": P, "k_stride": 128, **kw})          # noqa: E731
-    for bad, code in [(dict(qkv_dev=0), 3), (dict(type=4), 3), (dict(qkv_stride=767), 3), (dict(tokens=-1), 3), (dict(hq=0), 3), (dict(hkv=0), 3), (dict(hd=96), 12), (dict(rot=130), 3), (dict(rot=12), 3),
+    for bad, code in [(dict(qkv_dev=0), 3), (dict(type=4), 3), (dict(qkv_stride=767), 3), (dict(tokens=-1), 3), (dict(hq=0), 3), (dict(hkv=0), 3), (dict(hd=96), 12), (dict(rot=144), 3), (dict(rot=24), 3),
                       (dict(rot=-8), 3), (dict(eps=-1.0), 3), (dict(eps=float("nan")), 3), (dict(cos_dev=0), 3), (dict(sin_dev=0), 3), (dict(rope_rows=0), 3), (dict(pos_dev=0), 3), (dict(q_out_dev=0), 3),
                       (dict(q_stride=511), 3), (dict(k_out_dev=0), 3), (dict(k_stride=127), 3), (dict(qkv_dev=P + 1), 3), (dict(q_gain_dev=P + 2), 3), (dict(status_dev=P + 2), 3)]:
         refused(pkg, code, f, **bad)
