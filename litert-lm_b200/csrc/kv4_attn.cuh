@@ -6,10 +6,13 @@
 // The codes go from the cache into the A operands of mma.sync as they are, and the precision lies in the other operand:
 //   S  int8 products (m16n8k32, unsigned codes): a row of q is cut into four digits of seven bits below its largest power of
 //      two, the eight columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
-//   O  bf16 products (m16n8k16) with the codes as bf16 numbers c - 8 (exact) and P s in two bf16 terms (16-bit rows: 2^-17 of
-//      each weight) or three (fp32 rows, 2^-25).  Codes centred at zero keep the sums small; uncentred ones (16 + c, one
-//      instruction less for two codes) would cancel against their offset and lose five bits.  The tensor core cuts its sums off:
-//      fp32 rows take them out after every product, 16-bit rows at the end (at most 2^-24 an add).
+//   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in fp16 terms: one for bf16 rows (2^-12 of each
+//      weight, an eighth of what storing the row costs), two for fp16 and fp32 rows (2^-23).  P s is held in a power of two below
+//      fp16's range: its reference is the largest scale that the warp has met, so small weights are off by 2^-31 of that.
+//      Two nibbles of a half word come out of a mask each (1024 + c and 1024 + 16 c) and a fused product makes them c - 8; as
+//      bf16 numbers they would need a shift each, and the logic pipe, half as wide as the others, is what bounds this kernel.
+//      Codes centred at zero keep the sums small; the tensor core cuts its sums off, so fp32 rows take them out after every
+//      product, 16-bit rows at the end (at most 2^-24 an add).
 //
 // A warp walks its own tiles of keys (16 at head size 256, else 32) with a ring of its own that it fills by 16-byte asynchronous
 // copies: K and V rows lie in the cache in the order in which the fragments want them, so a lane's loads are 8 or 16 bytes
@@ -44,6 +47,7 @@ constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps;
 constexpr int kKaTickets = 4096;          // words at the start of a workspace
 constexpr int kKaStages = 3;
 
+// TV terms of P s.
 template <int HD, int GROUP, int RB, int TV>
 struct KaShape {
   static constexpr int PL = HD < 128 ? HD : 128, P = HD / PL;        // plane, planes
@@ -56,8 +60,7 @@ struct KaShape {
   static constexpr int kRing = kKaWarps * kKaStages * kStage;
   static constexpr int kDigits = HD / 64 * NB * 512;
   static constexpr int kUnit = kRing + kDigits;                      // [RB], then the group sums [RB][NG]
-  static constexpr int OR = TV == 2 ? RB : CV;                       // rows of a warp's O as it is handed over
-  static constexpr int kMergeO = kKaWarps * OR * HD * 4, kMergeOff = kKaWarps * RB * NG * 4;
+  static constexpr int kMergeO = kKaWarps * RB * HD * 4, kMergeOff = kKaWarps * RB * NG * 4;
   static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 <= kRing, "the exchange fits over the ring");
   static_assert(RB * KT * 4 <= kCodes, "P of a tile fits over its K codes");
   static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
@@ -68,7 +71,7 @@ __device__ __forceinline__ void ka_mma_s(int (&c)[4], uint32_t a0, uint32_t a1, 
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ka_mma_o(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float ka_ex2(float x) {
@@ -79,20 +82,19 @@ __device__ __forceinline__ float ka_ex2(float x) {
 __device__ __forceinline__ void ka_copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
-// Nibble p of both halves of x, as bf16 numbers c - 8: 16 + c has its code in the mantissa's upper bits.
+// The lowest (p = 0) or second nibble of both halves of x as fp16 numbers c - 8.
 template <int p>
 __device__ __forceinline__ uint32_t ka_codes(uint32_t x) {
-  const uint32_t y = ((p == 0 ? x << 3 : x >> (4 * p - 3)) & 0x00780078u) | 0x41804180u;
-  const uint32_t off = 0x41C041C0u;                                  // 24
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&off));
+  const uint32_t y = (x & (p ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;       // 1024 + c, or 1024 + 16 c
+  const __half2 h = *reinterpret_cast<const __half2*>(&y);
+  const __half2 r = p ? __hfma2(h, __float2half2_rn(1.f / 16), __float2half2_rn(-72.f)) : __hadd2(h, __float2half2_rn(-1032.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float ka_lo(uint32_t u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float ka_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+__device__ __forceinline__ float2 ka_unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
 template <int N>
 __device__ __forceinline__ void ka_words(const unsigned char* p, uint32_t (&d)[N]) {
@@ -107,7 +109,7 @@ __device__ __forceinline__ void ka_words(const unsigned char* p, uint32_t (&d)[N
   }
 }
 
-template <int HD, int GROUP, int RB, int TV>
+template <int HD, int GROUP, int RB, int TV, bool EXACT>
 __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a) {
   using S = KaShape<HD, GROUP, RB, TV>;
   constexpr int NG = S::NG, NB = S::NB, NBV = S::NBV, KT = S::KT, SUB = S::SUB, W4 = S::PL / 32;
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     if (lane == 0) unit_s[r] = spoilt ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 5) << 23) * a.qscale;
   }
   __syncthreads();
-  float unit[NB], qsum[NB][NG], m[NB], l[NB];
+  float unit[NB], qsum[NB][NG], m[NB], mz[NB], l[NB];                  // mz: m, or 0 while there is none
   int hi[NB], lo[NB];                                                // the keys that this lane's rows see
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -232,8 +234,10 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     hi[nb] = r < rows ? at : -1;
     lo[nb] = a.window > 0 ? at - a.window + 1 : 0;
     m[nb] = -INFINITY;
-    l[nb] = 0.f;
+    mz[nb] = l[nb] = 0.f;
   }
+  float wk = 1.f;                                                    // P s is held times this power of two
+  uint32_t limit = 1;                                                // and this scale (fp16 bits) is past it
   float o[S::MT][NBV][4], off[NBV][NG];
 #pragma unroll
   for (int c = 0; c < NBV; ++c) {
@@ -243,10 +247,11 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     for (int i = 0; i < NG; ++i) off[c][i] = 0.f;
   }
   // keys that every row sees, so that tiles within them need no mask
+  const int seen0 = a.window > 0 ? max(0, first - a.window + 1) : 0;
   const int open1 = rows == RB ? first + 1 : 0, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
 
   auto add = [](float (&acc)[4], const uint32_t (&x)[4], const uint32_t (&y)[2]) {
-    if constexpr (TV == 2) {
+    if constexpr (!EXACT) {
       ka_mma_o(acc, x, y[0], y[1]);
     } else {
       float part[4] = {0.f, 0.f, 0.f, 0.f};
@@ -307,11 +312,12 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
               const float low = t & 1 ? s1.y : s0.y;
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) {
-                constexpr float big = 12582912.f;
-                const float d0 = __int_as_float(c[u][nb][0]) - big, d1 = __int_as_float(c[u][nb][1]) - big;
-                const float d2 = __int_as_float(c[u][nb][2]) - big, d3 = __int_as_float(c[u][nb][3]) - big;
-                s[u][nb][0] = fmaf(s0.x, fmaf(d1, 1.f / 128, d0), s[u][nb][0]);
-                s[u][nb][1] = fmaf(s1.x, fmaf(d3, 1.f / 128, d2), s[u][nb][1]);
+                // both digits' sums carry 1.5 * 2^23; every step is exact
+                constexpr float big = 12582912.f * (1.f + 1.f / 128);
+                const float d0 = fmaf(__int_as_float(c[u][nb][1]), 1.f / 128, __int_as_float(c[u][nb][0]) - big);
+                const float d1 = fmaf(__int_as_float(c[u][nb][3]), 1.f / 128, __int_as_float(c[u][nb][2]) - big);
+                s[u][nb][0] = fmaf(s0.x, d0, s[u][nb][0]);
+                s[u][nb][1] = fmaf(s1.x, d1, s[u][nb][1]);
                 smin[u][nb] = fmaf(low, qsum[nb][grp], smin[u][nb]);
               }
             }
@@ -322,6 +328,19 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     // ---- whole scores: lane keeps key g + 8 (t & 1); softmax against the row's reference
     float p[SUB][NB];
     bool over = false;
+    uint32_t largest = 0;
+    {
+      constexpr int WL = KT * NG / 32;                               // every scale of V once in the warp
+      uint32_t w[WL];
+      ka_words<WL>(st + 2 * S::kCodes + S::kScales + lane * WL * 4, w);
+#pragma unroll
+      for (int i = 0; i < WL; ++i) {
+        const uint32_t x = w[i] & 0xFFFFu;
+        const int key = tl * KT + (lane * WL + i) / NG;
+        if (x < 0x7C00u && (!edge || (key >= seen0 && key < key1))) largest = max(largest, x);
+      }
+      over = largest >= limit;
+    }
     const float digit = t & 1 ? 1.f / 16384 : 1.f;
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
@@ -337,7 +356,15 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
         over = over || x > m[nb] + 8.f;
       }
     if (__any_sync(0xffffffffu, over)) {
-      float f[NB];
+      float f[NB], fk = 1.f;
+      largest = __reduce_max_sync(0xffffffffu, largest);
+      if (largest >= limit) {                                        // largest 2^k in [2^6, 2^7); with P <= 2^8 within fp16's range
+        const float top = __half2float(__ushort_as_half((unsigned short)largest));
+        const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = 64.f / power;
+        fk = k / wk;
+        wk = k;
+        limit = power >= 32768.f ? 0x7C00u : (uint32_t)__half_as_ushort(__float2half_rn(2.f * power));
+      }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float top = m[nb];
@@ -348,7 +375,9 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
         for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
         f[nb] = m[nb] == top ? 1.f : ka_ex2(m[nb] - top);            // equal: both may be -inf
         m[nb] = top;
+        mz[nb] = top == -INFINITY ? 0.f : top;
         l[nb] *= f[nb];
+        f[nb] *= fk;
       }
       auto of_row = [&](int r) {                                     // factor of row r, from a lane that holds it
         float v = 1.f;
@@ -375,10 +404,10 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const float x = ka_ex2(p[u][nb] - (m[nb] == -INFINITY ? 0.f : m[nb]));
+        const float x = ka_ex2(p[u][nb] - mz[nb]);
         l[nb] += x;
         const int key = g + 8 * (t & 1);
-        ps[(2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4] = x;
+        ps[(2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4] = x * wk;
       }
     __syncwarp();
 
@@ -427,12 +456,10 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
                 off[c][grp] += y;
               }
               uint32_t b0 = ka_pack(x[0], x[1]), b1 = ka_pack(x[2], x[3]);
-              const int term = (c * 8 + g) % TV;
-#pragma unroll
-              for (int k = 1; k < TV; ++k) {                         // the next term, in the lanes whose column is one
-                x[0] -= ka_lo(b0); x[1] -= ka_hi(b0); x[2] -= ka_lo(b1); x[3] -= ka_hi(b1);
-                const uint32_t n0 = ka_pack(x[0], x[1]), n1 = ka_pack(x[2], x[3]);
-                if (term >= k) { b0 = n0; b1 = n1; }
+              if constexpr (TV == 2) {                               // what the first term left, in the odd columns
+                const float2 y0 = ka_unpack(b0), y1 = ka_unpack(b1);
+                const uint32_t n0 = ka_pack(x[0] - y0.x, x[1] - y0.y), n1 = ka_pack(x[2] - y1.x, x[3] - y1.y);
+                if (g & 1) { b0 = n0; b1 = n1; }
               }
               bt[c][0] = b0;
               bt[c][1] = b1;
@@ -442,7 +469,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
           for (int h = 0; h < 2; ++h) {                              // 32 dims: a half of the units' words
             const uint32_t x = __byte_perm(v[0][j], v[1][j], h ? 0x7632 : 0x5410), y = __byte_perm(v[2][j], v[3][j], h ? 0x7632 : 0x5410);
             const uint32_t a0[4] = {ka_codes<0>(x), ka_codes<1>(x), ka_codes<0>(y), ka_codes<1>(y)};
-            const uint32_t a1[4] = {ka_codes<2>(x), ka_codes<3>(x), ka_codes<2>(y), ka_codes<3>(y)};
+            const uint32_t a1[4] = {ka_codes<0>(x >> 8), ka_codes<1>(x >> 8), ka_codes<0>(y >> 8), ka_codes<1>(y >> 8)};
             const int mt = dim / 16 + 2 * h;
 #pragma unroll
             for (int c = 0; c < NBV; ++c) {
@@ -456,7 +483,8 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
   }
 
   // ---- the warps' sums
-  float* mo = reinterpret_cast<float*>(ka_sm);                       // [warp][OR][HD]
+  const float back = 1.f / wk;                                       // a power of two
+  float* mo = reinterpret_cast<float*>(ka_sm);                       // [warp][RB][HD]
   float* moff = mo + S::kMergeO / 4;                                 // [warp][RB][NG]
   float* ml = moff + S::kMergeOff / 4;                               // [warp][RB][2]
   const bool spoilt = __syncthreads_or(bad) != 0;                    // every warp is done with its ring, too
@@ -478,7 +506,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       float x = off[c][i];
       x += __shfl_xor_sync(0xffffffffu, x, 1);
       x += __shfl_xor_sync(0xffffffffu, x, 2);
-      if (t == 0 && (c * 8 + g) % TV == 0 && c * 8 + g < S::CV) moff[(warp * RB + (c * 8 + g) / TV) * NG + i] = x;
+      if (t == 0 && (c * 8 + g) % TV == 0 && c * 8 + g < S::CV) moff[(warp * RB + (c * 8 + g) / TV) * NG + i] = x * back;
     }
 #pragma unroll
     for (int i = 0; i < S::MT; ++i)
@@ -486,11 +514,11 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       for (int h = 0; h < 2; ++h) {
         const int dim = i * 16 + h * 8 + g;
         if constexpr (TV == 2) {                                     // the two terms of row 4 c + t
-          if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + dim] = o[i][c][2 * h] + o[i][c][2 * h + 1];
+          if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + dim] = (o[i][c][2 * h] + o[i][c][2 * h + 1]) * back;
         } else {
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            if (c * 8 + 2 * t + k < S::CV) mo[(warp * S::OR + c * 8 + 2 * t + k) * HD + dim] = o[i][c][2 * h + k];
+            if (2 * t + k < RB) mo[(warp * RB + 2 * t + k) * HD + dim] = o[i][c][2 * h + k] * back;
         }
       }
   }
@@ -509,9 +537,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
 #pragma unroll
     for (int w = 0; w < kKaWarps; ++w) {
       const float mw = ml[(w * RB + r) * 2], f = mw == top ? 1.f : ka_ex2(mw - top);
-      float x = moff[(w * RB + r) * NG + dim / GROUP];
-      if constexpr (TV == 2) x += mo[(w * RB + r) * HD + dim];
-      else x += mo[(w * S::OR + r * 3) * HD + dim] + (mo[(w * S::OR + r * 3 + 1) * HD + dim] + mo[(w * S::OR + r * 3 + 2) * HD + dim]);
+      const float x = moff[(w * RB + r) * NG + dim / GROUP] + mo[(w * RB + r) * HD + dim];
       sum += f * ml[(w * RB + r) * 2 + 1];
       v += f * x;
     }
@@ -559,8 +585,8 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
   }
 }
 
-// Rows of a CTA for `rows` query rows of a kv head: the fewest that hold them, and four at head size 256, where O of eight would
-// not fit the registers.
+// Rows of a CTA for `rows` query rows of a kv head: the fewest that hold them, and four at head size 256, where O of eight in two
+// terms would not fit the registers.
 constexpr int ka_rows(int hd, long long rows) { return rows <= 2 ? 2 : rows <= 4 || hd == 256 ? 4 : 8; }
 
 }  // namespace b200lm
