@@ -5,7 +5,7 @@
 //
 // The codes go from the cache into the A operands of mma.sync as they are, and the precision lies in the other operand:
 //   S  int8 products (m16n8k32, unsigned codes): a row of q is cut into four digits of seven bits below its largest power of
-//      two, the eight columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
+//      two (of three bits and three times seven where the codes enter as 16 c: upper nibbles are masked, not shifted), the eight columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
 //   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in fp16 terms: one for bf16 rows (2^-12 of each
 //      weight, an eighth of what storing the row costs), two for fp16 and fp32 rows (2^-23).  P s is held in a power of two below
 //      fp16's range: its reference is the largest scale that the warp has met, so small weights are off by 2^-31 of that.
@@ -22,6 +22,8 @@
 // A CTA serves RB rows over a share of the keys; shares of a sequence are joined by the last CTA to arrive.  How many
 // keys a share has is decided on the host from the largest length, how many shares a sequence has on the device from its own.
 #pragma once
+#include <type_traits>
+
 #include "kv4_rows.cuh"
 #include "split_ticket.h"
 
@@ -66,9 +68,10 @@ struct KaShape {
   static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
 };
 
-__device__ __forceinline__ void ka_mma_s(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void ka_mma_s(int (&d)[4], const int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 __device__ __forceinline__ void ka_mma_o(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -191,7 +194,8 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     }
     const uint32_t bits = __reduce_max_sync(0xffffffffu, odd ? 0x7F800000u : __float_as_uint(top));
     const int e = max((int)(bits >> 23), 30);
-    const float f = __uint_as_float((uint32_t)(254 + 5 - e) << 23);
+    // elements with bit 4 set meet their codes as 16 c: their digits are of a sixteenth, 2^-23 of the row's largest
+    const float f = __uint_as_float((uint32_t)(254 + 5 - e - ((lane * V & 16) ? 4 : 0)) << 23);
     const bool spoilt = bits >= 0x7F800000u;
     uint32_t word[4][(V + 3) / 4] = {};
 #pragma unroll
@@ -260,6 +264,79 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       for (int i = 0; i < 4; ++i) acc[i] += part[i];
     }
   };
+  // O += (P s) codes of a tile: lane (g, t) holds column g of P s for the keys t + 4 i, and the codes of unit g of those keys.
+  // ODD: rows may not see keys whose scales are NaN.
+  auto products = [&](const unsigned char* st, const float* ps, auto odd) {
+    constexpr bool ODD = decltype(odd)::value;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      float w[NBV][4];
+#pragma unroll
+      for (int c = 0; c < NBV; ++c) {
+        const int r = (c * 8 + g) / TV;
+        const float4 v = *reinterpret_cast<const float4*>(ps + (r < RB ? r : 0) * KT + u * 16 + 4 * t);
+        w[c][0] = v.x; w[c][1] = v.y; w[c][2] = v.z; w[c][3] = v.w;
+      }
+      uint32_t vs[4][NG];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ka_words<NG>(st + 2 * S::kCodes + S::kScales + (u * 16 + t + 4 * i) * NG * 4, vs[i]);
+      uint32_t bt[NBV][2];
+#pragma unroll
+      for (int pl = 0; pl < S::P; ++pl) {
+        constexpr int WU = S::ROW / 32;                              // words of a unit: 2, at head size 64 one
+        uint32_t v[4][WU];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int unit_at = S::PL == 128 ? g ^ (4 * (t >> 1)) : g;
+          ka_words<WU>(st + S::kCodes + pl * KT * S::ROW + (u * 16 + t + 4 * i) * S::ROW + unit_at * (S::ROW / 8), v[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < WU; ++j) {                               // 64 dims
+          const int dim = pl * S::PL + j * 64, grp = dim / GROUP;
+          if (dim % GROUP == 0) {
+            float sc[4], mn[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vs[i][grp]));
+              sc[i] = f.x;
+              mn[i] = fmaf(8.f, f.x, f.y);
+            }
+#pragma unroll
+            for (int c = 0; c < NBV; ++c) {
+              float x[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                x[i] = w[c][i] * sc[i];
+                if (ODD && w[c][i] == 0.f) x[i] = 0.f;               // 0 times NaN
+                else off[c][grp] = fmaf(w[c][i], mn[i], off[c][grp]);
+              }
+              uint32_t b0 = ka_pack(x[0], x[1]), b1 = ka_pack(x[2], x[3]);
+              if constexpr (TV == 2) {                               // what the first term left, in the odd columns
+                const float2 y0 = ka_unpack(b0), y1 = ka_unpack(b1);
+                const uint32_t n0 = ka_pack(x[0] - y0.x, x[1] - y0.y), n1 = ka_pack(x[2] - y1.x, x[3] - y1.y);
+                if (g & 1) { b0 = n0; b1 = n1; }
+              }
+              bt[c][0] = b0;
+              bt[c][1] = b1;
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {                              // 32 dims: a half of the units' words
+            const uint32_t x = __byte_perm(v[0][j], v[1][j], h ? 0x7632 : 0x5410), y = __byte_perm(v[2][j], v[3][j], h ? 0x7632 : 0x5410);
+            const uint32_t a0[4] = {ka_codes<0>(x), ka_codes<1>(x), ka_codes<0>(y), ka_codes<1>(y)};
+            const uint32_t a1[4] = {ka_codes<0>(x >> 8), ka_codes<1>(x >> 8), ka_codes<0>(y >> 8), ka_codes<1>(y >> 8)};
+            const int mt = dim / 16 + 2 * h;
+#pragma unroll
+            for (int c = 0; c < NBV; ++c) {
+              add(o[mt][c], a0, bt[c]);
+              add(o[mt + 1][c], a1, bt[c]);
+            }
+          }
+        }
+      }
+    }
+  };
+  const int zero[4] = {kGgMagic, kGgMagic, kGgMagic, kGgMagic};
   int slot = 0;
 #pragma unroll 1
   for (int tl = t0 + warp; tl < t1; tl += kKaWarps) {
@@ -298,10 +375,10 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
             const uint2 q = *reinterpret_cast<const uint2*>(digits + ((dim / 64 * NB + nb) * 32 + lane) * 4 + (j & 1) * 2);
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
-              if (dim % GROUP == 0) c[u][nb][0] = c[u][nb][1] = c[u][nb][2] = c[u][nb][3] = kGgMagic;
               const uint32_t x = k[u][0][j], y = k[u][1][j];
-              constexpr uint32_t n = 0x0F0F0F0Fu;
-              ka_mma_s(c[u][nb], x & n, y & n, (x >> 4) & n, (y >> 4) & n, q.x, q.y);
+              constexpr uint32_t n = 0x0F0F0F0Fu;                    // the upper nibbles enter as 16 c, their digits a sixteenth
+              if (dim % GROUP == 0) ka_mma_s(c[u][nb], zero, x & n, y & n, x & ~n, y & ~n, q.x, q.y);
+              else ka_mma_s(c[u][nb], c[u][nb], x & n, y & n, x & ~n, y & ~n, q.x, q.y);
             }
           }
           if ((dim + 32) % GROUP == 0) {
@@ -327,7 +404,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
     }
     // ---- whole scores: lane keeps key g + 8 (t & 1); softmax against the row's reference
     float p[SUB][NB];
-    bool over = false;
+    bool over = false, odd = false;
     uint32_t largest = 0;
     {
       constexpr int WL = KT * NG / 32;                               // every scale of V once in the warp
@@ -336,8 +413,20 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
         const uint32_t x = w[i] & 0xFFFFu;
-        const int key = tl * KT + (lane * WL + i) / NG;
-        if (x < 0x7C00u && (!edge || (key >= seen0 && key < key1))) largest = max(largest, x);
+        if (x < 0x7C00u) largest = max(largest, x);
+      }
+      if (edge) {                                                    // rows that no one sees may hold anything: zeros do no harm
+        largest = 0;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < WL; ++i) {
+          const uint32_t x = w[i] & 0xFFFFu;
+          const int key = tl * KT + (lane * WL + i) / NG;
+          if (key < seen0 || key >= key1) reinterpret_cast<uint32_t*>(st + 2 * S::kCodes + S::kScales)[lane * WL + i] = 0u;
+          else if (x < 0x7C00u) largest = max(largest, x);
+          else nan = true;
+        }
+        odd = __any_sync(0xffffffffu, nan);
       }
       over = largest >= limit;
     }
@@ -411,75 +500,9 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       }
     __syncwarp();
 
-    // ---- O: lane (g, t) holds column g of P s for the keys t + 4 i, and the codes of unit g of those keys
-#pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      float w[NBV][4];
-#pragma unroll
-      for (int c = 0; c < NBV; ++c) {
-        const int r = (c * 8 + g) / TV;
-        const float4 v = *reinterpret_cast<const float4*>(ps + (r < RB ? r : 0) * KT + u * 16 + 4 * t);
-        w[c][0] = v.x; w[c][1] = v.y; w[c][2] = v.z; w[c][3] = v.w;
-      }
-      uint32_t vs[4][NG];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ka_words<NG>(st + 2 * S::kCodes + S::kScales + (u * 16 + t + 4 * i) * NG * 4, vs[i]);
-      uint32_t bt[NBV][2];
-#pragma unroll
-      for (int pl = 0; pl < S::P; ++pl) {
-        constexpr int WU = S::ROW / 32;                              // words of a unit: 2, at head size 64 one
-        uint32_t v[4][WU];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int unit_at = S::PL == 128 ? g ^ (4 * (t >> 1)) : g;
-          ka_words<WU>(st + S::kCodes + pl * KT * S::ROW + (u * 16 + t + 4 * i) * S::ROW + unit_at * (S::ROW / 8), v[i]);
-        }
-#pragma unroll
-        for (int j = 0; j < WU; ++j) {                               // 64 dims
-          const int dim = pl * S::PL + j * 64, grp = dim / GROUP;
-          if (dim % GROUP == 0) {
-            float sc[4], mn[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vs[i][grp]));
-              sc[i] = f.x;
-              mn[i] = fmaf(8.f, f.x, f.y);
-            }
-#pragma unroll
-            for (int c = 0; c < NBV; ++c) {
-              float x[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                x[i] = w[c][i] * sc[i];
-                float y = w[c][i] * mn[i];
-                if (edge && w[c][i] == 0.f) x[i] = y = 0.f;          // a row that is not seen may hold anything
-                off[c][grp] += y;
-              }
-              uint32_t b0 = ka_pack(x[0], x[1]), b1 = ka_pack(x[2], x[3]);
-              if constexpr (TV == 2) {                               // what the first term left, in the odd columns
-                const float2 y0 = ka_unpack(b0), y1 = ka_unpack(b1);
-                const uint32_t n0 = ka_pack(x[0] - y0.x, x[1] - y0.y), n1 = ka_pack(x[2] - y1.x, x[3] - y1.y);
-                if (g & 1) { b0 = n0; b1 = n1; }
-              }
-              bt[c][0] = b0;
-              bt[c][1] = b1;
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {                              // 32 dims: a half of the units' words
-            const uint32_t x = __byte_perm(v[0][j], v[1][j], h ? 0x7632 : 0x5410), y = __byte_perm(v[2][j], v[3][j], h ? 0x7632 : 0x5410);
-            const uint32_t a0[4] = {ka_codes<0>(x), ka_codes<1>(x), ka_codes<0>(y), ka_codes<1>(y)};
-            const uint32_t a1[4] = {ka_codes<0>(x >> 8), ka_codes<1>(x >> 8), ka_codes<0>(y >> 8), ka_codes<1>(y >> 8)};
-            const int mt = dim / 16 + 2 * h;
-#pragma unroll
-            for (int c = 0; c < NBV; ++c) {
-              add(o[mt][c], a0, bt[c]);
-              add(o[mt + 1][c], a1, bt[c]);
-            }
-          }
-        }
-      }
-    }
+    // ---- O
+    if (odd) products(st, ps, std::true_type());
+    else products(st, ps, std::false_type());
   }
 
   // ---- the warps' sums
