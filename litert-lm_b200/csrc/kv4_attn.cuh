@@ -42,7 +42,7 @@ struct Kv4AttnArgs {
   int* status;
   int row_tiles, share, splits;           // row tiles of a kv head, keys of a share, most shares of a sequence
   unsigned* tickets;                      // one per (sequence, kv head, row tile), zero between calls
-  float* parts;                           // [unit][split][RB][HD + 2]: O, maximum, sum (negative: a page outside the pool)
+  float* parts;                           // [unit][split]: O [RB][HD], then maximum and sum (negative: a page outside the pool) of each row
 };
 
 constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps;
@@ -63,7 +63,7 @@ struct KaShape {
   static constexpr int kDigits = HD / 64 * NB * 512;
   static constexpr int kUnit = kRing + kDigits;                      // [RB], then the group sums [RB][NG]
   static constexpr int kMergeO = kKaWarps * RB * HD * 4, kMergeOff = kKaWarps * RB * NG * 4;
-  static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 <= kRing, "the exchange fits over the ring");
+  static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 + RB * 8 <= kRing, "the exchange fits over the ring");
   static_assert(RB * KT * 4 <= kCodes, "P of a tile fits over its K codes");
   static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
 };
@@ -546,38 +546,56 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       }
   }
   __syncthreads();
-  auto out_at = [&](int r) {
-    const int row = r0 + r;
-    return (long long)(tok0 + row / G) * a.out_stride + (long long)(kvh * G + row % G) * HD;
-  };
-  const long long u = ((long long)b * a.kv.hkv + kvh) * a.row_tiles + tile;
-  float* rec = a.parts + (u * a.splits + split) * (RB * (HD + 2));
-  for (int i = threadIdx.x; i < RB * HD; i += kKaThreads) {
-    const int r = i / HD, dim = i % HD;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
+  // weights of the warps' sums (eight neighbouring lanes a row), the CTA's maximum and sum
+  float* total = ml + kKaWarps * RB * 2;                             // [RB][2]
+  if (warp * 32 < RB * kKaWarps) {                                   // whole warps: with two rows, lanes 16 .. 31 repeat the second
+    const int w = threadIdx.x % kKaWarps, r = min((int)threadIdx.x / kKaWarps, RB - 1);
+    const float mw = ml[(w * RB + r) * 2];
+    float top = mw, sum = ml[(w * RB + r) * 2 + 1];
 #pragma unroll
-    for (int w = 0; w < kKaWarps; ++w) top = fmaxf(top, ml[(w * RB + r) * 2]);
+    for (int k = 1; k < kKaWarps; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    const float f = mw == top ? 1.f : ka_ex2(mw - top);
+    sum *= f;
 #pragma unroll
-    for (int w = 0; w < kKaWarps; ++w) {
-      const float mw = ml[(w * RB + r) * 2], f = mw == top ? 1.f : ka_ex2(mw - top);
-      const float x = moff[(w * RB + r) * NG + dim / GROUP] + mo[(w * RB + r) * HD + dim];
-      sum += f * ml[(w * RB + r) * 2 + 1];
-      v += f * x;
-    }
-    if (nsplit == 1) {
-      if (r < rows && !spoilt) gg_store1(a.out, out_at(r) + dim, a.q_type, sum == 0.f ? 0.f : v / sum);
-    } else {
-      rec[r * (HD + 2) + dim] = v;
-      if (dim == 0) {
-        rec[r * (HD + 2) + HD] = top;
-        rec[r * (HD + 2) + HD + 1] = spoilt ? -1.f : sum;
+    for (int k = 1; k < kKaWarps; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (threadIdx.x < RB * kKaWarps) {
+      ml[(w * RB + r) * 2] = f;
+      if (w == 0) {
+        total[2 * r] = top;
+        total[2 * r + 1] = sum;
       }
     }
+  }
+  __syncthreads();
+  const long long u = ((long long)b * a.kv.hkv + kvh) * a.row_tiles + tile;
+  constexpr int REC = RB * (HD + 2);                                 // a share's record: O, then maximum and sum of its rows
+  float* rec = a.parts + (u * a.splits + split) * REC;
+  // a thread's elements are four neighbours of a row
+  auto store = [&](int r, int dim, const float (&v)[4], float sum) {
+    const int row = r0 + r;
+    const long long at = (long long)(tok0 + row / G) * a.out_stride + (long long)(kvh * G + row % G) * HD + dim;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) gg_store1(a.out, at + k, a.q_type, sum == 0.f ? 0.f : v[k] * inv);
+  };
+#pragma unroll 1
+  for (int i = threadIdx.x; i < RB * HD / 4; i += kKaThreads) {
+    const int r = i / (HD / 4), dim = i % (HD / 4) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kKaWarps; ++w) {
+      const float f = ml[(w * RB + r) * 2], add_all = moff[(w * RB + r) * NG + dim / GROUP];
+      const float4 x = *reinterpret_cast<const float4*>(mo + (w * RB + r) * HD + dim);
+      v[0] = fmaf(f, x.x + add_all, v[0]); v[1] = fmaf(f, x.y + add_all, v[1]); v[2] = fmaf(f, x.z + add_all, v[2]); v[3] = fmaf(f, x.w + add_all, v[3]);
+    }
+    if (nsplit > 1) *reinterpret_cast<float4*>(rec + r * HD + dim) = make_float4(v[0], v[1], v[2], v[3]);
+    else if (r < rows && !spoilt) store(r, dim, v, total[2 * r + 1]);
   }
   if (nsplit == 1) {
     if (spoilt && threadIdx.x == 0) set_status(a.status, kDevBadPosition);
     return;
   }
+  if (threadIdx.x < 2 * RB) rec[RB * HD + threadIdx.x] = spoilt && (threadIdx.x & 1) ? -1.f : total[threadIdx.x];
   // ---- the shares' sums: the last CTA of the unit to arrive
   __shared__ int last_s;
   __threadfence();
@@ -586,25 +604,43 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
   __syncthreads();
   if (!last_s) return;
   __threadfence();
-  const float* all = a.parts + u * a.splits * (RB * (HD + 2));
-  for (int i = threadIdx.x; i < rows * HD; i += kKaThreads) {
-    const int r = i / HD, dim = i % HD;
-    const float* at = all + r * (HD + 2);
-    float top = -INFINITY, sum = 0.f, v = 0.f;
-    bool lost = false;
-    for (int k = 0; k < nsplit; ++k) {
-      const float* x = at + k * (RB * (HD + 2));
-      top = fmaxf(top, __ldcg(x + HD));
-      lost = lost || __ldcg(x + HD + 1) < 0.f;
+  const float* all = a.parts + u * a.splits * REC;
+  float* weight = reinterpret_cast<float*>(ka_sm);                   // [RB][nsplit] (the host keeps RB * splits below the ring's size)
+  bool lost = false;
+  for (int i = threadIdx.x; i < RB * nsplit; i += kKaThreads) {
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(all + (long long)(i / RB) * REC + RB * HD) + i % RB);
+    lost = lost || x.y < 0.f;
+    weight[i % RB * nsplit + i / RB] = x.x;
+    weight[(RB + i % RB) * nsplit + i / RB] = x.y;
+  }
+  if (__syncthreads_or(lost)) {
+    if (threadIdx.x == 0) set_status(a.status, kDevBadPosition);
+    return;
+  }
+  for (int r = warp; r < RB; r += kKaWarps) {
+    float top = -INFINITY, sum = 0.f;
+    for (int k = lane; k < nsplit; k += 32) top = fmaxf(top, weight[r * nsplit + k]);
+    top = warp_max(top);
+    for (int k = lane; k < nsplit; k += 32) {
+      const float mk = weight[r * nsplit + k], f = mk == top ? 1.f : ka_ex2(mk - top);
+      weight[r * nsplit + k] = f;
+      sum = fmaf(f, weight[(RB + r) * nsplit + k], sum);
     }
+    sum = warp_sum(sum);
+    if (lane == 0) unit_s[r] = sum;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < rows * HD / 4; i += kKaThreads) {
+    const int r = i / (HD / 4), dim = i % (HD / 4) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int k = 0; k < nsplit; ++k) {
-      const float* x = at + k * (RB * (HD + 2));
-      const float mk = __ldcg(x + HD), f = mk == top ? 1.f : ka_ex2(mk - top);
-      sum += f * __ldcg(x + HD + 1);
-      v += f * __ldcg(x + dim);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(all + (long long)k * REC + r * HD + dim));
+      const float f = weight[r * nsplit + k];
+      v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
     }
-    if (lost) { if (i == 0) set_status(a.status, kDevBadPosition); }
-    else gg_store1(a.out, out_at(r) + dim, a.q_type, sum == 0.f ? 0.f : v / sum);
+    store(r, dim, v, unit_s[r]);
   }
 }
 

@@ -139,16 +139,18 @@ static Kv4Plan plan_attention(int batch, int hkv, int hd, int hq, int max_q, int
   p.units = tiles * hkv * batch;
   B2_CHECK(tiles * hkv <= 0x7FFFFFFF, kInvalidArgument, "too many query rows for one call");
   p.row_tiles = (int)tiles;
-  // Shares of 2 CTAs an SM four times over, so that sequences of different lengths even out; none shorter than a round of
-  // the CTA's warps.
+  // Shares for 2 CTAs an SM four times over, so that sequences of different lengths even out (64 of 300 .. 8192: 90 us against 129
+  // with one share a CTA), but none shorter than four rounds of the CTA's warps where the GPU is full without (16 x 5 rows
+  // over a window of 1024: 27 us against 32), as a share costs its set-up and its part of the join.
   const int round = (hd == 256 ? 16 : 32) * kKaWarps;
-  const long long most = std::max<long long>(1, 8ll * sms / p.units);
   const long long keys = (window > 0 ? std::min<long long>(max_kv, (long long)window + max_q) : max_kv) + 32;
-  p.share = (int)std::min<long long>((keys / most + round) / round * round, 1 << 30);
-  p.splits = (int)std::min<long long>(std::max<long long>(1, (keys + p.share - 1) / p.share), most);
+  auto shares = [&](long long ctas) { return std::min<long long>(512, std::max<long long>(1, ctas * sms / p.units)); };
+  auto length = [&](long long n) { return (keys / n + round) / round * round; };
+  p.share = (int)std::min<long long>(std::max(length(shares(8)), std::min<long long>(4 * round, length(shares(2)))), 1 << 30);
+  p.splits = (int)((keys + p.share - 1) / p.share);
   B2_CHECK(tiles * hkv * p.splits <= 0x7FFFFFFF, kInvalidArgument, "too many query rows for one call");
   // what a call of any length up to these sizes may need
-  p.bytes = most == 1 ? 0 : kKaTickets * 4 + p.units * most * p.rb * (hd + 2) * 4;
+  p.bytes = shares(8) == 1 ? 0 : kKaTickets * 4 + p.units * shares(8) * p.rb * (hd + 2) * 4;
   return p;
 }
 
