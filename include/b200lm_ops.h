@@ -207,8 +207,8 @@ int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t type, int6
 /* A paged cache in 4 bits.  For each page and kv head lie, in this order, the K
  * codes, K scales, V codes and V scales of 256 positions.  A row of hd elements is
  * cut into groups of 64 or 128; of each group are kept m = its lowest value,
- * s = (highest - lowest) / 15, both rounded to fp16 (rounded to fp32 before, and
- * held within the fp16 range), and a code of 4 bits for each element,
+ * s = (highest - lowest) / 15, both rounded to fp32 and then fp16 (lowest and
+ * highest are held to -64000 .. 64000), and a code of 4 bits for each element,
  * c = rint((x - m) / s) held to 0 .. 15, which stands for s c + m.  A group with an
  * infinity or NaN stands for NaN.
  * Scales are [256][hd/group] pairs (s, m).  Codes lie in planes of 128 elements

@@ -6,8 +6,8 @@
 // The codes go from the cache into the A operands of mma.sync as they are, and the precision lies in the other operand:
 //   S  int8 products (m16n8k32, unsigned codes): a row of q is cut into four digits of seven bits below its largest power of
 //      two (of three bits and three times seven where the codes enter as 16 c: upper nibbles are masked, not shifted), the eight columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
-//   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in fp16 terms: one for bf16 rows (2^-12 of each
-//      weight, an eighth of what storing the row costs), two for fp16 and fp32 rows (2^-23).  P s is held in a power of two below
+//   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in fp16 terms: one for bf16 rows (2^-11 of each
+//      weight, an eighth of what storing the row costs), two for fp16 and fp32 rows (2^-22).  P s is held in a power of two below
 //      fp16's range: its reference is the largest scale that the warp has met, so small weights are off by 2^-31 of that.
 //      Two nibbles of a half word come out of a mask each (1024 + c and 1024 + 16 c) and a fused product makes them c - 8; as
 //      bf16 numbers they would need a shift each, and the logic pipe, half as wide as the others, is what bounds this kernel.

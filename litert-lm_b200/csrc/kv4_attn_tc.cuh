@@ -1,0 +1,465 @@
+// Attention over the cache in 4 bits for many bf16 query rows of a kv head (a prompt's chunk), on the 5th-generation tensor cores.
+//
+// A CTA owns 128 query rows of a kv head and a range of keys, walked in tiles of 64.  Codes become fp16 numbers
+// s (c - 8) + (m + 8 s) on the way (the quantiser keeps them inside fp16's range), two roundings of at most 2^-11 of the group's
+// largest (storing a bf16 row costs 2^-8); queries are bf16 numbers times a power of two of their row, exact in fp16.
+//
+//   warps 9 - 16  expand: codes from global memory a tile ahead, K and V rows into swizzled shared memory (two stages each)
+//   warp 8        issues the products: S = Q K^T with Q in tensor memory (read from shared memory it would take half of the
+//                 bandwidth that the expanded rows need), O += P V with P in tensor memory, over the scores it was made from
+//   warps 0 - 7   softmax, two threads a row (half of the keys, half of O each).  A row's reference moves when a score passes it
+//                 by 8 powers of two; only then is O read, scaled and written back, behind the products of the tile before.
+//
+// Order of issue: S(j + 1), then O(j), so that the softmax of a tile runs beside the products of its neighbours.
+// Scores of tile j + 1 may overwrite the probabilities of j - 1 when O(j - 1) is complete.
+//
+// What bounds it: shared memory.  Per tile (head size 256) 64 KB of expanded rows are written and read once by the products (1024
+// cycles at 128 B), the products themselves take 1024.
+//
+// A NaN in a group of K or V makes the key's scores NaN, so it spoils the rows that see the key and no others; V's own row is
+// zero then, as is what no row sees.  All waits are bounded; after one that gave up the CTA's threads run to its end without
+// the products, and the status says so.
+#pragma once
+#include "kv4_attn.cuh"
+#include "prefill_gemm_ts.cuh"
+#include "prefill_ops.cuh"
+#include "attn_tc.cuh"
+
+namespace b200lm {
+
+constexpr int kKcRows = 128, kKcSoft = 256, kKcExpand = 256, kKcThreads = kKcSoft + 32 + kKcExpand;
+
+template <int HD>
+struct KcShape {
+  static constexpr int KT = 64;                                      // keys of a tile
+  static constexpr int kTile = KT * HD * 2;                          // K or V of a tile
+  static constexpr int kMax = 4 * kTile;                             // [2][128] floats
+  static constexpr int kBars = kMax + 2 * 128 * 4;
+  static constexpr int kSmem = kBars + 256;
+  static constexpr uint32_t kO = 0, kQ = HD, kS = HD + HD / 2;       // tensor memory columns; P of a tile over its scores
+  static_assert(kS + 2 * KT <= 512 && kSmem <= 227 * 1024, "budgets");
+};
+__host__ __device__ constexpr uint32_t kc_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }      // fp16 x fp16 -> fp32
+
+// Two neighbouring codes (nibbles of two bytes, `low` or high) as values.
+template <int p>
+__device__ __forceinline__ uint32_t kc_values(uint32_t x, __half2 s, __half2 mid) {
+  const uint32_t c = ka_codes<p>(x);
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c), s, mid);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int HD, int GROUP>
+__global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnArgs a) {
+  using S = KcShape<HD>;
+  constexpr int KT = S::KT, P = HD / 128, HK = KT / 2;
+  constexpr Kv4Dims d{HD, GROUP};
+  extern __shared__ __align__(1024) unsigned char kc_sm[];
+  float* row_x = reinterpret_cast<float*>(kc_sm + S::kMax);          // [half][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(kc_sm + S::kBars);
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10, *o_full = bars + 12, *q_ready = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  int* gave_up = reinterpret_cast<int*>(bars + 15);
+  __shared__ int last_s;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  // ---- which rows and keys
+  const int tile = blockIdx.x % a.row_tiles, split = blockIdx.x / a.row_tiles % a.splits, kvh = blockIdx.x / a.row_tiles / a.splits, b = blockIdx.y;
+  const int G = a.hq / a.kv.hkv;
+  const int tok0 = a.q_start ? a.q_start[b] : b, nq = a.q_start ? a.q_start[b + 1] - tok0 : 1, len = a.kv_len[b];
+  if (tok0 < 0 || nq < 0 || nq > a.max_q || tok0 > a.tokens - nq || len < 0 || len > a.max_kv) {
+    if (threadIdx.x == 0) set_status(a.status, kDevBadPosition);
+    return;
+  }
+  const int r0 = tile * kKcRows, rows = min(kKcRows, nq * G - r0);
+  if (rows <= 0) return;
+  const int first = len - nq + r0 / G, lastp = len - nq + (r0 + rows - 1) / G;
+  const int seen0 = a.window > 0 ? max(0, first - a.window + 1) : 0, key0 = seen0 & ~(KT - 1), key1 = lastp + 1;
+  const int nsplit = max(1, (key1 - key0 + a.share - 1) / a.share);
+  if (split >= nsplit) return;
+  const int t0 = (key0 + split * a.share) / KT, n = max(0, (min(key1, key0 + (split + 1) * a.share) + KT - 1) / KT - t0);
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], P * 128);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], P * 128);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 8);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(q_ready, 8);
+    *gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  bool ok = true, bad = false;                                       // none of this thread's waits has given up; a page outside the pool
+  const int quarter = warp & 3, half = (warp >> 2) & 1, row = quarter * 32 + lane;     // softmax
+  const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+  float m = -INFINITY, l = 0.f;
+  if (n > 0 && warp >= 9) {
+    // ---- expansion: thread (key, plane, q): 32 bytes of a K row (64 elements), 32 of a V row
+    // (at head size 128 the first four warps have the K rows, the others the V rows)
+    const int w = warp - 9, key = (P == 2 ? w / 2 : w % 4) * 16 + (lane & 15), plane = P == 2 ? w % 2 : 0, q = lane >> 4;
+    const bool has_k = P == 2 || w < 4, has_v = P == 2 || w >= 4;
+    const int* table = a.kv.table + b * a.kv.table_stride;
+    const long long page_bytes = (long long)a.kv.hkv * d.head_bytes(), head = (long long)kvh * d.head_bytes();
+    uint4 kr[2], vr[2];
+    uint32_t ks[2], vs[2];
+    int page_ahead = __ldg(table + t0 * KT / kKv4Page);               // of the next tile to load: its number is a tile ahead of its rows
+    auto load = [&](int j) {
+      const int at = (t0 + j) * KT, page = page_ahead, slot = at % kKv4Page + key;
+      if (j + 1 < n) page_ahead = __ldg(table + (at + KT) / kKv4Page);
+      if (page < 0 || page >= a.kv.num_pages) {
+        bad = true;
+        return;
+      }
+      const uint8_t* h = a.kv.pages + page * page_bytes + head;
+      const uint8_t* k = h + d.k_codes() + (plane * kKv4Page + slot) * 64 + q * 32;
+      const uint8_t* v = h + d.v_codes() + (plane * kKv4Page + slot) * 64 + q * 32;
+      if (has_k) {
+        kr[0] = ldg_nc_v4(reinterpret_cast<const uint4*>(k));
+        kr[1] = ldg_nc_v4(reinterpret_cast<const uint4*>(k) + 1);
+      }
+      if (has_v) {
+        vr[0] = ldg_nc_v4(reinterpret_cast<const uint4*>(v));
+        vr[1] = ldg_nc_v4(reinterpret_cast<const uint4*>(v) + 1);
+      }
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(h + d.k_scales()) + slot * d.groups() + plane * 128 / GROUP;
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(h + d.v_scales()) + slot * d.groups() + plane * 128 / GROUP;
+      ks[0] = __ldg(kp);
+      vs[0] = __ldg(vp);
+      ks[1] = GROUP == 64 ? __ldg(kp + 1) : ks[0];
+      vs[1] = GROUP == 64 ? __ldg(vp + 1) : vs[0];
+    };
+    kr[0] = kr[1] = vr[0] = vr[1] = make_uint4(0u, 0u, 0u, 0u);
+    ks[0] = ks[1] = vs[0] = vs[1] = 0u;
+    load(0);
+    auto pair = [](uint32_t u, __half2& s, __half2& mid) {
+      const __half2 x = *reinterpret_cast<const __half2*>(&u);
+      s = __half2half2(__low2half(x));
+      mid = __half2half2(__hfma(__low2half(x), __float2half(8.f), __high2half(x)));
+    };
+    auto nan = [](uint32_t u) { return (u & 0x7C00u) == 0x7C00u; };
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int st = j & 1, use = j >> 1;
+      uint32_t kw[8] = {kr[0].x, kr[0].y, kr[0].z, kr[0].w, kr[1].x, kr[1].y, kr[1].z, kr[1].w};
+      uint32_t vw[8] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w, vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+      uint32_t k2[2] = {ks[0], ks[1]}, v2[2] = {vs[0], vs[1]};
+      if (j + 1 < n) load(j + 1);
+      const int slot = (t0 + j) * KT % kKv4Page + key, where = (t0 + j) * KT + key;
+      if (where < seen0 || where >= key1) v2[0] = v2[1] = 0u, k2[0] = k2[1] = 0u;    // what no row sees: zeros
+      else if (nan(v2[0]) || nan(v2[1])) {
+        k2[0] = 0x7E007E00u;
+        if (nan(v2[0])) v2[0] = 0u;
+        if (nan(v2[1])) v2[1] = 0u;
+      }
+      if (has_k && use > 0) ok = ok && mbar_wait(&k_empty[st], (use - 1) & 1, gave_up);
+      if (has_k && ok) {
+        unsigned char* line = kc_sm + st * S::kTile + key * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                                // 32 elements: 8 q .. and 16 more, of the words 2 q and 2 q + 1
+          __half2 s, mid;
+          pair(k2[i / 2], s, mid);
+          const uint32_t x0 = __byte_perm(kw[i], 0, 0x4140), x1 = __byte_perm(kw[i], 0, 0x4342), x2 = __byte_perm(kw[4 + i], 0, 0x4140), x3 = __byte_perm(kw[4 + i], 0, 0x4342);
+          unsigned char* at = line + (plane * 2 + i / 2) * KT * 128;
+          const int c = 4 * (i & 1) + q;
+          *reinterpret_cast<uint4*>(at + ((c ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
+          *reinterpret_cast<uint4*>(at + (((c + 2) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
+        }
+      }
+      fence_async_smem();
+      if (has_k) mbar_arrive(&k_full[st]);
+      // V: this thread has two words of four units; it wants word q of all eight, the partner (lane ^ 16) the other words
+      uint32_t mine[4], got[4], unit[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mine[i] = q ? vw[2 * i + 1] : vw[2 * i];
+        got[i] = __shfl_xor_sync(0xffffffffu, q ? vw[2 * i] : vw[2 * i + 1], 16);
+      }
+      const bool low = q == (slot >> 1 & 1);                         // the units that it has are the first four
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unit[i] = low ? mine[i] : got[i];
+        unit[4 + i] = low ? got[i] : mine[i];
+      }
+      if (has_v && use > 0) ok = ok && mbar_wait(&v_empty[st], (use - 1) & 1, gave_up);
+      if (has_v && ok) {
+        unsigned char* line = kc_sm + (2 + st) * S::kTile + (plane * 2 + q) * KT * 128 + key * 128;
+        __half2 s, mid;
+        pair(v2[GROUP == 64 ? q : 0], s, mid);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                                // byte i of the words: 16 neighbours
+          const uint32_t sel = i | (4 + i) << 8;
+          const uint32_t x0 = __byte_perm(unit[0], unit[1], sel), x1 = __byte_perm(unit[2], unit[3], sel), x2 = __byte_perm(unit[4], unit[5], sel), x3 = __byte_perm(unit[6], unit[7], sel);
+          *reinterpret_cast<uint4*>(line + (((2 * i) ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
+          *reinterpret_cast<uint4*>(line + (((2 * i + 1) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
+        }
+      }
+      fence_async_smem();
+      if (has_v) mbar_arrive(&v_full[st]);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+  } else if (n > 0 && warp == 8) {
+    // ---- products
+    constexpr uint32_t idesc_s = kc_idesc(128, KT), idesc_o = kc_idesc(128, HD) | 1u << 16;      // V: hd contiguous
+    const bool leader = elect_one();
+    const uint32_t ring = smem_u32(kc_sm);
+    auto scores = [&](int j) {
+      const uint32_t k = ring + (j & 1) * S::kTile;
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i)
+        umma_bf16_ts(tmem + S::kS + (j & 1) * KT, tmem + S::kQ + i * 8, umma_desc_sw128(k + i / 4 * KT * 128) + (uint64_t)(i % 4 * 2), idesc_s, i > 0);
+      umma_commit(&s_full[j & 1]);
+      umma_commit(&k_empty[j & 1]);
+    };
+    ok = __all_sync(0xffffffffu, mbar_wait2(q_ready, 0, &k_full[0], 0, gave_up));
+    if (ok) {
+      tc_fence_after();
+      if (leader) scores(0);
+      __syncwarp();
+    }
+#pragma unroll 1
+    for (int j = 0; j < n && ok; ++j) {
+      if (j + 1 < n) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, gave_up) && (j == 0 || mbar_wait(o_full, (j - 1) & 1, gave_up)));
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) scores(j + 1);
+        __syncwarp();
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait2(&v_full[j & 1], (j >> 1) & 1, &p_full[j & 1], (j >> 1) & 1, gave_up));
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        const uint32_t v = ring + (2 + (j & 1)) * S::kTile;
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k)
+          umma_bf16_ts(tmem + S::kO, tmem + S::kS + (j & 1) * KT + k * 8, atc_desc_mn(v + k * 2048, KT * 128), idesc_o, j > 0 || k > 0);
+        umma_commit(o_full);
+        umma_commit(&v_empty[j & 1]);
+      }
+      __syncwarp();
+    }
+  } else if (n > 0) {
+    // ---- this thread's half of a query row, times a power of two, into tensor memory
+    const int at = len - nq + (r0 + row) / G, hi = row < rows ? at : -1, lo = a.window > 0 ? at - a.window + 1 : 0;
+    float unit;
+    {
+      constexpr int V = HD / 2;
+      const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.q) + (long long)(tok0 + (r0 + row) / G) * a.q_stride + (long long)(kvh * G + (r0 + row) % G) * HD + half * V;
+      const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+      auto get = [&](int i, float (&x)[8]) {
+        RawRow<kBf16, 8> raw;
+        if (row < rows) raw.load(src, i, vec);
+        else raw.u[0] = raw.u[1] = raw.u[2] = raw.u[3] = 0u;
+        raw.get(x);
+      };
+      float top = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < V; i += 8) {
+        float x[8];
+        get(i, x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = isfinite(x[k]) ? fmaxf(top, fabsf(x[k])) : INFINITY;
+      }
+      row_x[half * 128 + row] = top;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const uint32_t bits = __float_as_uint(fmaxf(row_x[row], row_x[128 + row]));
+      const int e = max((int)(bits >> 23), 30);
+      const bool spoilt = bits >= 0x7F800000u;
+      const float f = spoilt ? 0.f : __uint_as_float((uint32_t)(254 + 7 - e) << 23);             // largest |q| f in [2^7, 2^8)
+      unit = spoilt ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 7) << 23) * a.qscale;
+#pragma unroll 1
+      for (int i = 0; i < V; i += 32) {                              // the second time from the cache
+        uint32_t y[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          float x[8];
+          get(i + k, x);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) y[k / 2 + c] = spoilt ? 0u : ka_pack(x[2 * c] * f, x[2 * c + 1] * f);
+        }
+        tmem_st16(lane_addr + S::kQ + half * (HD / 4) + i / 2, y);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    // keys that every row of the tile sees
+    const int open1 = rows == kKcRows ? first + 1 : 0, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
+    float mz = 0.f;
+    bool late = false;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int base = (t0 + j) * KT, mykeys = base + half * HK;
+      const bool got = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (j >> 1) & 1, gave_up)) && !late;
+      float s[HK], mx = -INFINITY;
+      if (got) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < HK; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(lane_addr + S::kS + (j & 1) * KT + half * HK + c, x);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(x[i]) * unit;
+        }
+        if (base < open0 || base + KT > open1) {
+#pragma unroll
+          for (int i = 0; i < HK; ++i)
+            if (mykeys + i > hi || mykeys + i < lo) s[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < HK; ++i) mx = fmaxf(mx, s[i]);
+      }
+      if (bar_or<1, 256>(!got || mx > m + 8.f)) {
+        // the eight warps leave the loop together, or move the references of all rows
+        row_x[half * 128 + row] = mx;
+        ok = !block_gave_up([&] { return !got; }, bar_or<1, 256>);
+        if (!ok) break;
+        const float mn = fmaxf(m, fmaxf(row_x[row], row_x[128 + row])), f = mn == m ? 1.f : ka_ex2(m - mn);
+        m = mn;
+        mz = mn == -INFINITY ? 0.f : mn;
+        l *= f;
+        if (j > 0) {
+          late = !__all_sync(0xffffffffu, mbar_wait(o_full, (j - 1) & 1, gave_up));
+          if (!late && __any_sync(0xffffffffu, f != 1.f)) {
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 32) {
+              uint32_t x[32];
+              tmem_ld32(lane_addr + S::kO + half * (HD / 2) + c, x);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+              tmem_st16(lane_addr + S::kO + half * (HD / 2) + c, *reinterpret_cast<const uint32_t(*)[16]>(x));
+              tmem_st16(lane_addr + S::kO + half * (HD / 2) + c + 16, *reinterpret_cast<const uint32_t(*)[16]>(x + 16));
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < HK; c += 32) {
+        uint32_t y[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float p0 = ka_ex2(s[c + i] - mz), p1 = ka_ex2(s[c + i + 1] - mz);
+          l += p0 + p1;
+          y[i / 2] = ka_pack(p0, p1);
+        }
+        tmem_st16(lane_addr + S::kS + (j & 1) * KT + half * (HK / 2) + c / 2, y);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
+    }
+    ok = ok && !late && __all_sync(0xffffffffu, mbar_wait(o_full, (n - 1) & 1, gave_up));
+    tc_fence_after();
+  }
+  // ---- row sums meet; O out of tensor memory
+  const bool spoilt = __syncthreads_or(bad) != 0, failed = __syncthreads_or(!ok) != 0;
+  const long long u = ((long long)b * a.kv.hkv + kvh) * a.row_tiles + tile;
+  constexpr int REC = kKcRows * (HD + 2);
+  float* rec = a.parts + (u * a.splits + split) * REC;
+  if (warp < 8) row_x[half * 128 + row] = l;
+  __syncthreads();
+  if (warp < 8 && !failed) {
+    const float sum = row_x[row] + row_x[128 + row], inv = sum == 0.f ? 0.f : 1.f / sum;
+    const long long out = (long long)(tok0 + (r0 + row) / G) * a.out_stride + (long long)(kvh * G + (r0 + row) % G) * HD + half * (HD / 2);
+    const bool vec = (reinterpret_cast<uintptr_t>(reinterpret_cast<__nv_bfloat16*>(a.out) + out) & 15) == 0;
+#pragma unroll 1
+    for (int c = 0; c < HD / 2; c += 32) {
+      uint32_t x[32];
+      if (n > 0) tmem_ld32(lane_addr + S::kO + half * (HD / 2) + c, x);
+      else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = 0u;
+      }
+      if (row < rows && nsplit > 1) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<uint4*>(rec + row * HD + half * (HD / 2) + c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      } else if (row < rows && !spoilt) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          RawRow<kBf16, 8> y;
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = sum == 0.f ? 0.f : __uint_as_float(x[i + k]) * inv;
+          y.put(v);
+          y.store(a.out, out + c + i, vec);
+        }
+      }
+      __syncwarp();                                                  // the next load is the whole warp's
+    }
+    if (nsplit > 1 && half == 0) *reinterpret_cast<float2*>(rec + kKcRows * HD + 2 * row) = make_float2(m, spoilt ? -1.f : sum);
+  }
+  tc_fence_before();
+  sync_after_waits(ok);
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (failed) {
+    // the other shares of the unit still count this one: its record says that it is lost
+    if (nsplit > 1 && threadIdx.x < kKcRows) *reinterpret_cast<float2*>(rec + kKcRows * HD + 2 * threadIdx.x) = make_float2(0.f, -1.f);
+    if (threadIdx.x == 0) set_status(a.status, kDevBarrierTimeout);
+  } else if (spoilt && threadIdx.x == 0) {
+    set_status(a.status, kDevBadPosition);
+  }
+  if (nsplit == 1) return;
+  // ---- the shares' sums: the last CTA of the unit to arrive
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last_s = ticket_last(a.tickets + u, nsplit, [](unsigned* p, unsigned k) { return atomicInc(p, k); });
+  __syncthreads();
+  if (!last_s) return;
+  __threadfence();
+  const float* all = a.parts + u * a.splits * REC;
+  float* weight = reinterpret_cast<float*>(kc_sm);                   // [nsplit][row], then the rows' sums
+  bool lost = false;
+  if (threadIdx.x < kKcRows) {
+    const float* ml = all + kKcRows * HD + 2 * threadIdx.x;
+    float top = -INFINITY, sum = 0.f;
+    for (int k = 0; k < nsplit; ++k) top = (int)threadIdx.x < rows ? fmaxf(top, __ldcg(ml + (long long)k * REC)) : 0.f;
+    for (int k = 0; k < nsplit; ++k) {
+      const float mk = (int)threadIdx.x < rows ? __ldcg(ml + (long long)k * REC) : 0.f, lk = (int)threadIdx.x < rows ? __ldcg(ml + (long long)k * REC + 1) : 1.f, f = mk == top ? 1.f : ka_ex2(mk - top);
+      lost = lost || lk < 0.f;
+      weight[k * kKcRows + threadIdx.x] = f;
+      sum = fmaf(f, lk, sum);
+    }
+    weight[nsplit * kKcRows + threadIdx.x] = sum;
+  }
+  if (__syncthreads_or(lost)) return;                                // the CTA that lost it has said so
+#pragma unroll 1
+  for (int i = threadIdx.x; i < rows * HD / 8; i += kKcThreads) {
+    const int r = i / (HD / 8), dim = i % (HD / 8) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < nsplit; ++k) {
+      const float4* p = reinterpret_cast<const float4*>(all + (long long)k * REC + r * HD + dim);
+      const float4 x = __ldcg(p), y = __ldcg(p + 1);
+      const float f = weight[k * kKcRows + r];
+      v[0] = fmaf(f, x.x, v[0]); v[1] = fmaf(f, x.y, v[1]); v[2] = fmaf(f, x.z, v[2]); v[3] = fmaf(f, x.w, v[3]);
+      v[4] = fmaf(f, y.x, v[4]); v[5] = fmaf(f, y.y, v[5]); v[6] = fmaf(f, y.z, v[6]); v[7] = fmaf(f, y.w, v[7]);
+    }
+    const float sum = weight[nsplit * kKcRows + r], inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = sum == 0.f ? 0.f : v[k] * inv;
+    const long long out = (long long)(tok0 + (r0 + r) / G) * a.out_stride + (long long)(kvh * G + (r0 + r) % G) * HD + dim;
+    RawRow<kBf16, 8> y;
+    y.put(v);
+    y.store(a.out, out, (reinterpret_cast<uintptr_t>(reinterpret_cast<__nv_bfloat16*>(a.out) + out) & 15) == 0);
+  }
+}
+
+}  // namespace b200lm

@@ -187,13 +187,15 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[kVec], uint32_t (&
     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
   }
   const bool bad = !isfinite(low) || !isfinite(high);
-  constexpr float top = 65504.f;                           // fp16's largest
-  const __half m = __float2half_rn(fminf(fmaxf(low, -top), top));
+  constexpr float top = 64000.f;                           // with every rounding, m + 15 s stays inside fp16's range
+  low = fminf(fmaxf(low, -top), top);
+  high = fminf(fmaxf(high, -top), top);
+  const __half m = __float2half_rn(low);
   // (high - low) / 15 in fp32 is off by at most 2^-22 of itself: where that could lead to another fp16 number, fp64 decides
   const float step = (high - low) * (1.f / 15.f);
-  __half s = __float2half_rn(fminf(step, top));
+  __half s = __float2half_rn(step);
   if (!bad && (__half_as_ushort(__float2half_rn(step * (1.f - 3e-7f))) != __half_as_ushort(__float2half_rn(step * (1.f + 3e-7f)))))
-    s = __float2half_rn(fminf(step64(low, high), top));
+    s = __float2half_rn(step64(low, high));
   const float mf = __half2float(m), sf = __half2float(s), inv = sf > 0.f ? __fdividef(1.f, sf) : 0.f;
   constexpr float whole = 12582912.f;                      // 1.5 * 2^23: adding it rounds, and leaves a code in the lowest byte
   float r[kVec], near = 0.f;

@@ -126,11 +126,37 @@ void launch_kv4_attn_64(cudaStream_t st, const Kv4AttnArgs& a, int rb);
 void launch_kv4_attn_128(cudaStream_t st, const Kv4AttnArgs& a, int rb);
 void launch_kv4_attn_256(cudaStream_t st, const Kv4AttnArgs& a, int rb);
 
+void launch_kv4_chunk(cudaStream_t st, const Kv4AttnArgs& a);
+
 // How a call's keys are shared out.  A unit is a (sequence, kv head, row tile).
 struct Kv4Plan {
   int rb, row_tiles, share, splits;
   int64_t units, bytes;
 };
+#ifndef KCR
+#define KCR 32
+#endif
+constexpr int kChunkRows = KCR;             // query rows of a kv head from which the tensor-core kernel takes a bf16 call
+static bool chunk_call(int hd, int hq, int hkv, int max_q, int type) { return type == kBf16 && hd >= 128 && (long long)max_q * (hq / hkv) >= kChunkRows; }
+
+// The tensor-core kernel: one CTA an SM, tiles of 64 keys.
+static Kv4Plan plan_chunk(int batch, int hkv, int hd, int hq, int max_q, int max_kv, int window, int sms) {
+  Kv4Plan p;
+  const long long rows = (long long)max_q * (hq / hkv);
+  p.rb = 128;
+  const long long tiles = (rows + 127) / 128;
+  p.units = tiles * hkv * batch;
+  B2_CHECK(tiles * hkv * 16 <= 0x7FFFFFFF, kInvalidArgument, "too many query rows for one call");
+  p.row_tiles = (int)tiles;
+  const int round = 64;
+  const long long keys = (window > 0 ? std::min<long long>(max_kv, (long long)window + max_q) : max_kv) + round;
+  long long best = std::min<long long>(std::max<long long>(1, sms / p.units), 16);      // one round of CTAs
+  best = std::max<long long>(1, std::min(best, keys / (4 * round)));                    // of at least four tiles each
+  p.share = (int)std::min<long long>((keys / best + round) / round * round, 1 << 30);
+  p.splits = (int)((keys + p.share - 1) / p.share);
+  p.bytes = p.units * 2 > sms ? 0 : kKaTickets * 4 + std::min<int64_t>(sms, p.units * 16) * 128 * (hd + 2) * 4;
+  return p;
+}
 static Kv4Plan plan_attention(int batch, int hkv, int hd, int hq, int max_q, int max_kv, int window, int sms) {
   Kv4Plan p;
   const long long rows = (long long)max_q * (hq / hkv);
@@ -267,7 +293,9 @@ extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, in
   check_attention(batch, hkv, hd, hq, max_q, max_kv);
   require_device(device);
   DeviceScope scope(device);
-  *bytes = plan_attention(batch, hkv, hd, hq, max_q, max_kv, 0, device_sms(device)).bytes;
+  const int sms = device_sms(device);
+  *bytes = plan_attention(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes;
+  if (chunk_call(hd, hq, hkv, max_q, kBf16)) *bytes = std::max(*bytes, plan_chunk(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes);
   KV4_END
 }
 
@@ -298,13 +326,15 @@ extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cach
   a.qscale = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)cache->hd));
   a.out = out_dev; a.out_stride = out_stride; a.status = status_dev;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const Kv4Plan p = plan_attention(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv, window, device_sms(device));
+  const bool chunk = chunk_call(cache->hd, hq, cache->hkv, max_q, q_type);
+  const Kv4Plan p = (chunk ? plan_chunk : plan_attention)(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv, window, device_sms(device));
   B2_CHECK(p.splits == 1 || (workspace_dev && workspace_bytes >= p.bytes), kInvalidArgument,
            "the workspace is smaller than AttentionKv4Workspace says: " + std::to_string(p.bytes) + " bytes");
   a.row_tiles = p.row_tiles; a.share = p.share; a.splits = p.splits;
   a.tickets = reinterpret_cast<unsigned*>(workspace_dev);
   a.parts = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(workspace_dev) + kKaTickets * 4);
-  if (cache->hd == 64) launch_kv4_attn_64(st, a, p.rb);
+  if (chunk) launch_kv4_chunk(st, a);
+  else if (cache->hd == 64) launch_kv4_attn_64(st, a, p.rb);
   else if (cache->hd == 128) launch_kv4_attn_128(st, a, p.rb);
   else launch_kv4_attn_256(st, a, p.rb);
   KV4_END

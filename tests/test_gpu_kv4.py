@@ -7,8 +7,12 @@ Tolerances.  u = 2^-24.  A stored value is off by half a step: eps / 2 of it, an
   norm       sum of hd / 32 + 5 adds, a root, a quotient: at most 16 u on the factor, four roundings behind it: 24 u (|a| + |b|)
   cache      codes are decided in 64 bits from values rounded once to 32: equal
   attention  a score is off by dS = 8 u sum |q k| scale + 2^-20 (the exponent's own error, 2^-22, and its argument's rounding among it),
-             a weight by 2 dS and what it is held in, one fp16 term (half a step: 2^-12) for bf16 rows, two (2^-23) else; with the sums' own error of 64 u that
-             times the largest |v| bounds the result's
+             a weight by 2 dS and what it is held in, one fp16 term (half a step: 2^-11) for bf16 rows, two (2^-22) else; with the
+             sums' own error of 64 u that times the largest |v| bounds the result's.
+             Chunks of bf16 rows (32 rows of a kv head and more, head sizes 128 and 256) meet K and V as fp16 numbers
+             s (c - 8) + (m + 8 s), two roundings of at most 2^-11 of the largest |k| or |v| each.  The roundings of a key's elements
+             are independent: by Hoeffding's bound the score is off by more than 6 * 2^-10 max |k| |q| scale (|q| the 2-norm) with
+             probability 2 exp(-18) = 3e-8; that is added to dS, and 2^-10 to what multiplies the largest |v|
 """
 import math
 
@@ -347,7 +351,10 @@ class Attention:
             p = torch.where(seen, torch.softmax(x.masked_fill(~seen, -math.inf), -1), 0.0) if n else x
             want = torch.einsum("hgts,shd->thgd", p, v)
             d = 8 * U * (size.amax() if n else 0) + 2.0 ** -20
-            held_in = 2.0 ** -12 if self.typ == torch.bfloat16 else 2.0 ** -23
+            held_in = 2.0 ** -11 if self.typ == torch.bfloat16 else 2.0 ** -22
+            if self.typ == torch.bfloat16 and hd >= 128 and self.max_q * (hq // hkv) >= 32 and n:
+                d = d + 6 * 2.0 ** -10 * k.abs().amax() * q.norm(dim=-1).amax() * used
+                held_in += 2.0 ** -10
             bound = (2 * d + held_in + 64 * U) * (v.abs().amax() if n else 0)
             got = self.out[rows, :hq * hd].double().view_as(want)
             err = (got - want).abs()
