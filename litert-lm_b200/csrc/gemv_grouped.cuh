@@ -4,15 +4,17 @@
 //
 // What has to move is the weights' image, read once (n k / 2 bytes and the scales); the products themselves are small.  So
 // the codes go from global memory into the A operand of mma.sync (m16n8k32, int8) with three logic instructions for eight
-// of them, and the precision lies in the other operand: x is cut, for each column and block of 128 k, into four digits of
-// seven bits, x = 2^e (t0 + t1 / 2^7 + t2 / 2^14 + t3 / 2^21) with |t| <= 64, exact to 2^-28 of the block's largest value.
-// The eight columns of a product are four digits of two columns of x; its integer sums are exact.  They enter fp32 once a
-// group: an accumulator that starts at the bits of 1.5 * 2^23 is read as a float and 1.5 * 2^23 taken off (|sum| <=
-// 128 * 64 * 128 < 2^22, so nothing is rounded).
+// of them, and the precision lies in the other operand: x is cut, for each column and block of 128 k, into digits of seven bits,
+// x = 2^e (t0 + t1 / 2^7 + t2 / 2^14 [+ t3 / 2^21]) with |t| <= 64, exact to 2^-20 (three) or 2^-27 (four) of the block's
+// largest value.  A product of eight columns takes four digits of two columns of x; five to eight columns of a 16-bit type take
+// three products, one a digit (their numbers are exact in three unless they are below 2^-9 of the largest).  The integer sums are exact.  They enter fp32 once a group: an accumulator that starts at the bits of
+// 1.5 * 2^23 is read as a float and 1.5 * 2^23 taken off (|sum| <= 128 * 64 * 128 < 2^22, so nothing is rounded).
 //
-// A CTA has eight warps: RS strips of 16 rows times 8 / RS shares of its blocks of k.  Where the strips are fewer than the
-// GPU needs, a cluster of CTAs shares the blocks of the same strips and adds up through distributed shared memory: no
-// workspace, and a fixed order of sums.
+// The GPU's CTAs (two an SM) are clusters of `cs` that share the blocks of k and take an equal run of strips (16 rows) each.  A
+// CTA cuts its part of x into digits once (done for every strip it cost 17 us of 43008 x 5376 with eight columns), then its warps
+// stream strips without meeting, with blocks of weights on their way ahead; sums stay in shared memory and meet once, over
+// distributed shared memory: no workspace, a fixed order.  Where a run has fewer strips than warps, kw warps share the blocks
+// of a strip.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -33,23 +35,24 @@ struct GgArgs {
   void* y;
   long long ldy;
   int x_type, y_type, scale_bf16;
-  int rs, cs, chunk;            // strips of a CTA, CTAs of a cluster, blocks of k whose digits are held at once
+  int kw, cs, chunk, run;       // warps of a strip, CTAs of a cluster, blocks of k whose digits are held at once, strips of a cluster
 };
 
-constexpr int kGgThreads = 256;
+constexpr int kGgThreads = 256, kGgWarps = 8;
 constexpr int kGgMagic = 0x4B400000;                       // 1.5 * 2^23
 
-template <int GROUP, bool OFF, int NB>
+// MM products of a step: 1, 2 and 4 are two columns of four digits each, 3 is eight columns of three digits.
+template <int GROUP, bool OFF, int MM>
 struct GgShape {
   static constexpr int kGroups = 128 / GROUP;              // of a block
   static constexpr int kBlock = 1024 + 32 * kGroups * (OFF ? 2 : 1);
-  static constexpr int kAhead = NB == 4 ? 2 : 4;           // blocks of a warp on their way
-  static constexpr int kCols = 2 * NB;
+  static constexpr int kAhead = MM >= 3 ? 2 : 4;           // blocks of a warp on their way
+  static constexpr int kCols = MM == 3 ? 8 : 2 * MM;
   // shared memory of a chunk's block: digits, the columns' powers of two, their group sums
-  static constexpr int kPerBlock = NB * 1024 + kCols * 4 + (OFF ? kCols * kGroups * 4 : 0);
-  static constexpr int kRed = 8 * kCols * 16 * 4;
-  static size_t smem(int chunk) { return (size_t)chunk * kPerBlock + kRed; }
+  static constexpr int kPerBlock = MM * 1024 + kCols * 4 + (OFF ? kCols * kGroups * 4 : 0);
+  static constexpr int kChunk = 64 / MM;                   // most blocks held at once
 };
+inline size_t gg_out_bytes(int run, int ncols, int kw) { return (size_t)run * kw * ncols * 64; }
 
 __device__ __forceinline__ float gg_load1(const void* p, long long i, int type) {
   if (type == kF32) return reinterpret_cast<const float*>(p)[i];
@@ -104,45 +107,53 @@ struct GgBlock {
   }
 };
 
+__device__ __forceinline__ void gg_mma(int (&d)[4], const int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
 __device__ __forceinline__ float2 gg_pair(uint32_t u, bool bf16) {
   if (bf16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
 
-template <int GROUP, bool OFF, int NB>
-__global__ void __launch_bounds__(kGgThreads) gemv_grouped_kernel(const GgArgs a) {
-  using S = GgShape<GROUP, OFF, NB>;
-  constexpr int G = S::kGroups, AH = S::kAhead;
+template <int GROUP, bool OFF, int MM>
+__global__ void __launch_bounds__(kGgThreads, 2) gemv_grouped_kernel(const GgArgs a) {
+  using S = GgShape<GROUP, OFF, MM>;
+  constexpr int G = S::kGroups, AH = S::kAhead, LC = MM == 3 ? 2 : MM;        // columns of a lane
   extern __shared__ __align__(16) unsigned char gg_sm[];
-  uint32_t* digits = reinterpret_cast<uint32_t*>(gg_sm);                                       // [block][tile][nb][lane][4]
-  float* unit = reinterpret_cast<float*>(gg_sm + (size_t)a.chunk * NB * 1024);                 // [block][col]
+  uint32_t* digits = reinterpret_cast<uint32_t*>(gg_sm);                                       // [block][tile][product][lane][4]
+  float* unit = reinterpret_cast<float*>(gg_sm + (size_t)a.chunk * MM * 1024);                 // [block][col]
   float* sums = unit + a.chunk * S::kCols;                                                     // [block][col][group]
-  float* red = reinterpret_cast<float*>(gg_sm + (size_t)a.chunk * S::kPerBlock);               // [warp][col][16]
+  float* out = reinterpret_cast<float*>(gg_sm + (size_t)a.chunk * S::kPerBlock);               // [share of k][strip][col][16]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane & 3;
-  const int rank = blockIdx.x % a.cs, tile = blockIdx.x / a.cs;
-  const int kw = 8 / a.rs, ks = warp / a.rs;
-  const int strip = tile * a.rs + warp % a.rs;
+  const int rank = blockIdx.x % a.cs, first = blockIdx.x / a.cs * a.run, strips = min(a.run, a.strips - first);
+  const int rs = kGgWarps / a.kw, ks = warp / rs;                                              // strips at a time, this warp's share
   const int b0 = (int)((long long)a.blocks * rank / a.cs), b1 = (int)((long long)a.blocks * (rank + 1) / a.cs);
-  const int last = strip < a.strips ? b1 : b0;                                                 // a warp without a strip has no blocks
-  const uint8_t* w = a.w + (long long)strip * a.blocks * S::kBlock;
   pdl_wait();
   pdl_launch_dependents();
-
-  GgBlock<GROUP, OFF> ahead[AH];
-#pragma unroll
-  for (int i = 0; i < AH; ++i)
-    if (b0 + ks + i * kw < last) ahead[i].load(w + (long long)(b0 + ks + i * kw) * S::kBlock, lane);
-
-  float acc[NB][2];
-#pragma unroll
-  for (int i = 0; i < NB; ++i) acc[i][0] = acc[i][1] = 0.f;
 
 #pragma unroll 1
   for (int c0 = b0; c0 < b1; c0 += a.chunk) {
     const int c1 = min(c0 + a.chunk, b1);
+    // this warp's blocks: of strip warp % rs, warp % rs + rs, ... those from c0 + ks on in steps of kw
+    int strip_in = warp % rs, block_in = c0 + ks;
+    GgBlock<GROUP, OFF> ahead[AH];
+    auto load = [&](GgBlock<GROUP, OFF>& q) {
+      if (strip_in < strips && block_in < c1) {
+        q.load(a.w + ((long long)(first + strip_in) * a.blocks + block_in) * S::kBlock, lane);
+        block_in += a.kw;
+        if (block_in >= c1) {
+          block_in = c0 + ks;
+          strip_in += rs;
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < AH; ++i) load(ahead[i]);
     if (c0 > b0) __syncthreads();                          // the chunk before has been read
 #pragma unroll 1
-    for (int item = warp; item < (c1 - c0) * a.ncols; item += 8) {
+    for (int item = warp; item < (c1 - c0) * a.ncols; item += kGgWarps) {
       const int blk = item / a.ncols, c = item % a.ncols;
       const long long k = (long long)(c0 + blk) * 128 + 4 * lane;
       const float4 x = gg_load4(a.x, c * a.ldx + k, c * a.ldx + a.k, a.x_type);
@@ -154,17 +165,18 @@ __global__ void __launch_bounds__(kGgThreads) gemv_grouped_kernel(const GgArgs a
       const float f = __uint_as_float((uint32_t)(254 + 5 - e) << 23);
       float r[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
       if (bits >= 0x7F800000u) r[0] = r[1] = r[2] = r[3] = 0.f;
-      uint32_t* d = digits + ((blk * 2 + (lane >> 4)) * NB + (c >> 1)) * 128 + ((c & 1) * 16 + t) * 4 + ((lane >> 2) & 3);
+      constexpr int ND = MM == 3 ? 3 : 4;
+      uint32_t* d = digits + ((blk * 2 + (lane >> 4)) * MM + (MM == 3 ? 0 : c >> 1)) * 128 + ((MM == 3 ? 4 * c : (c & 1) * 16) + t) * 4 + ((lane >> 2) & 3);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t word = 0;
+      for (int i = 0; i < ND; ++i) {
+        uint32_t b[4];                                     // rint(r) in the lowest byte of r + 1.5 * 2^23
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float q = rintf(r[j]);
-          word |= ((uint32_t)(int)q & 0xFFu) << (8 * j);
-          r[j] = (r[j] - q) * 128.f;
+          const float q = r[j] + 12582912.f;
+          b[j] = __float_as_uint(q);
+          r[j] = (r[j] - (q - 12582912.f)) * 128.f;
         }
-        d[i * 16] = word;
+        d[i * (MM == 3 ? 128 : 16)] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
       }
       if (lane == 0) unit[blk * S::kCols + c] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 9) << 23);      // 1/16 of the digits' unit: codes enter as 16 q
       if constexpr (OFF) {
@@ -175,99 +187,137 @@ __global__ void __launch_bounds__(kGgThreads) gemv_grouped_kernel(const GgArgs a
       }
     }
     __syncthreads();
-    const int end = min(c1, last);
+    const int magic[4] = {kGgMagic, kGgMagic, kGgMagic, kGgMagic};
+    // strips and blocks as one sequence, a slot of the ring behind the other
+    const int mine = strips > warp % rs ? (strips - warp % rs + rs - 1) / rs : 0, each = c1 - c0 > ks ? (c1 - c0 - ks + a.kw - 1) / a.kw : 0, total = mine * each;
+    int s = warp % rs, b = c0 + ks;
+    float acc[LC][2];
+#pragma unroll
+    for (int i = 0; i < LC; ++i) acc[i][0] = acc[i][1] = 0.f;
 #pragma unroll 1
-    for (int base = c0 + ks; base < end; base += AH * kw) {
+    for (int it = 0; it < total; it += AH) {
 #pragma unroll
-      for (int i = 0; i < AH; ++i) {
-        const int b = base + i * kw;
-        if (b >= end) break;
+      for (int slot = 0; slot < AH; ++slot) {
+        if (it + slot >= total) break;
+        const GgBlock<GROUP, OFF>& q = ahead[slot];
         const int at = b - c0;
-        const GgBlock<GROUP, OFF>& q = ahead[i];
         constexpr uint32_t m = 0xF0F0F0F0u;
-        uint4 x[2][NB];
+        float part[LC][2];                                 // in units of the column's power of two
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < LC; ++i) part[i][0] = part[i][1] = 0.f;
+        float off[LC][2];
+        if constexpr (OFF) {
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) x[h][nb] = *reinterpret_cast<const uint4*>(digits + ((at * 2 + h) * NB + nb) * 128 + lane * 4);
-        float u[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) u[nb] = unit[at * S::kCols + nb * 2 + (t >> 1)];
-        int c[NB][4];
+          for (int i = 0; i < LC; ++i) off[i][0] = off[i][1] = 0.f;
+        }
+        int c[MM][4];
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
           const uint4& v = step < 2 ? q.a : q.b;
           const uint32_t lo = step & 1 ? v.z : v.x, hi = step & 1 ? v.w : v.y;
+          const uint32_t a0 = (lo << 4) & m, a1 = lo & m, a2 = (hi << 4) & m, a3 = hi & m;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (step * 32 % GROUP == 0) c[nb][0] = c[nb][1] = c[nb][2] = c[nb][3] = kGgMagic;
-            const uint4& d = x[step >> 1][nb];
-            mma_s8s8(c[nb], (lo << 4) & m, lo & m, (hi << 4) & m, hi & m, step & 1 ? d.z : d.x, step & 1 ? d.w : d.y);
+          for (int p = 0; p < MM; ++p) {
+            const uint2 d = *reinterpret_cast<const uint2*>(digits + ((at * 2 + (step >> 1)) * MM + p) * 128 + lane * 4 + (step & 1) * 2);
+            if (step * 32 % GROUP == 0) gg_mma(c[p], magic, a0, a1, a2, a3, d.x, d.y);
+            else gg_mma(c[p], c[p], a0, a1, a2, a3, d.x, d.y);
           }
           if ((step + 1) * 32 % GROUP == 0) {
             const int grp = step * 32 / GROUP;
-            const float2 s = gg_pair(q.s[grp], a.scale_bf16);
-            float2 o;
-            if constexpr (OFF) o = gg_pair(q.o[grp], a.scale_bf16);
+            const float2 sc = gg_pair(q.s[grp], a.scale_bf16);
+            constexpr float big = 12582912.f, two = big + big / 128, three = two + big / 16384;
+            if constexpr (MM == 3) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              constexpr float big = 12582912.f;
-              const float d0 = __int_as_float(c[nb][0]) - big, d1 = __int_as_float(c[nb][1]) - big;
-              const float d2 = __int_as_float(c[nb][2]) - big, d3 = __int_as_float(c[nb][3]) - big;
-              acc[nb][0] = fmaf(s.x * u[nb], fmaf(d1, 1.f / 128, d0), acc[nb][0]);
-              acc[nb][1] = fmaf(s.y * u[nb], fmaf(d3, 1.f / 128, d2), acc[nb][1]);
-              if constexpr (OFF) {
-                const float gs = t & 1 ? 0.f : sums[(at * S::kCols + nb * 2 + (t >> 1)) * G + grp];
-                acc[nb][0] = fmaf(o.x, gs, acc[nb][0]);
-                acc[nb][1] = fmaf(o.y, gs, acc[nb][1]);
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int x = 2 * h + i;
+                  const float v0 = fmaf(__int_as_float(c[1][x]), 1.f / 128, __int_as_float(c[0][x]) - three);
+                  part[i][h] = fmaf(h ? sc.y : sc.x, fmaf(__int_as_float(c[2][x]), 1.f / 16384, v0), part[i][h]);
+                }
+            } else {
+#pragma unroll
+              for (int p = 0; p < MM; ++p)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  part[p][h] = fmaf(h ? sc.y : sc.x, fmaf(__int_as_float(c[p][2 * h + 1]), 1.f / 128, __int_as_float(c[p][2 * h]) - two), part[p][h]);
+            }
+            if constexpr (OFF) {
+              const float2 of = gg_pair(q.o[grp], a.scale_bf16);
+#pragma unroll
+              for (int i = 0; i < LC; ++i) {
+                const float gs = sums[(at * S::kCols + (MM == 3 ? 2 * t + i : 2 * i + (t >> 1))) * G + grp];
+                off[i][0] = fmaf(of.x, gs, off[i][0]);
+                off[i][1] = fmaf(of.y, gs, off[i][1]);
               }
             }
           }
         }
-        if (b + AH * kw < last) ahead[i].load(w + (long long)(b + AH * kw) * S::kBlock, lane);
+#pragma unroll
+        for (int i = 0; i < LC; ++i) {
+          const float u = unit[at * S::kCols + (MM == 3 ? 2 * t + i : 2 * i + (t >> 1))];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            acc[i][h] = fmaf(u, part[i][h], acc[i][h]);
+            if constexpr (OFF) {
+              if (MM == 3 || !(t & 1)) acc[i][h] += off[i][h];       // the other lane of a column has its lower digits only
+            }
+          }
+        }
+        load(ahead[slot]);
+        b += a.kw;
+        if (b < c1) continue;
+        // the strip's sums: rows g and g + 8
+        float* o = out + (size_t)(ks * a.run + s) * a.ncols * 16 + (lane >> 2);
+#pragma unroll
+        for (int i = 0; i < LC; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v = acc[i][h];
+            int col = 2 * t + i;
+            if constexpr (MM != 3) {                       // the two digit pairs of a column sit in neighbouring lanes
+              v = t & 1 ? v * (1.f / 16384) : v;
+              v += __shfl_xor_sync(0xffffffffu, v, 1);
+              col = t & 1 ? a.ncols : 2 * i + (t >> 1);
+            }
+            if (col < a.ncols) {
+              float* at2 = o + col * 16 + 8 * h;
+              *at2 = c0 > b0 ? *at2 + v : v;
+            }
+            acc[i][h] = 0.f;
+          }
+        b = c0 + ks;
+        s += rs;
       }
     }
   }
-  // the two digit pairs of a column sit in neighbouring lanes
-  const float f = t & 1 ? 1.f / 16384 : 1.f;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v = acc[nb][h] * f;
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      if (!(t & 1)) red[(warp * S::kCols + nb * 2 + (t >> 1)) * 16 + h * 8 + (lane >> 2)] = v;
-    }
-  const int rows = a.rs * 16, outs = rows * a.ncols;
-  auto share = [&](const float* r, int c, int row) {       // a CTA's sum for column c, row `row` of its strips
-    float v = 0.f;
-    for (int i = 0; i < kw; ++i) v += r[((i * a.rs + row / 16) * S::kCols + c) * 16 + row % 16];
-    return v;
+  const int outs = strips * a.ncols * 16;
+  auto store = [&](int i, float v) {
+    const int row = (first + i / (16 * a.ncols)) * 16 + i % 16, c = i / 16 % a.ncols;
+    if (row < a.n) gg_store1(a.y, c * a.ldy + row, a.y_type, v);
   };
   if (a.cs == 1) {
     __syncthreads();
     for (int i = threadIdx.x; i < outs; i += kGgThreads) {
-      const int c = i / rows, row = i % rows;
-      if (tile * rows + row < a.n) gg_store1(a.y, c * a.ldy + tile * rows + row, a.y_type, share(red, c, row));
+      float v = out[i];
+      for (int j = 1; j < a.kw; ++j) v += out[j * a.run * a.ncols * 16 + i];
+      store(i, v);
     }
     return;
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   for (int i = rank * kGgThreads + threadIdx.x; i < outs; i += a.cs * kGgThreads) {
-    const int c = i / rows, row = i % rows;
     float v = 0.f;
     for (int r = 0; r < a.cs; ++r) {
       uint32_t base;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(base) : "r"((uint32_t)__cvta_generic_to_shared(red)), "r"(r));
-      float part = 0.f;
-      for (int j = 0; j < kw; ++j) {
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(base) : "r"((uint32_t)__cvta_generic_to_shared(out + i)), "r"(r));
+      for (int j = 0; j < a.kw; ++j) {
         float x;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(base + (uint32_t)(((j * a.rs + row / 16) * S::kCols + c) * 16 + row % 16) * 4) : "memory");
-        part += x;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(base + (uint32_t)(j * a.run * a.ncols) * 64) : "memory");
+        v += x;
       }
-      v += part;
     }
-    if (tile * rows + row < a.n) gg_store1(a.y, c * a.ldy + tile * rows + row, a.y_type, v);
+    store(i, v);
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // nobody leaves while its sums are read
 }

@@ -15,20 +15,40 @@ static void check_grouped(int64_t n, int64_t k, int32_t group) {
 static int64_t grouped_block(int group, bool off) { return 1024 + 32 * (128 / group) * (off ? 2 : 1); }
 static int64_t grouped_bytes(int64_t n, int64_t k, int group, bool off) { return (n + 15) / 16 * ((k + 127) / 128) * grouped_block(group, off); }
 
-template <int GROUP, bool OFF, int NB>
+// Runs of strips, clusters and warps a strip: the fewest blocks for the longest warp, where cutting x into digits counts 1/8 of a
+// block for each column and block of a CTA, and a cluster's meeting as many blocks as it has CTAs.
+template <typename S>
+static size_t plan_gg(GgArgs& a, int sms) {
+  long long best = -1;
+  const int room = 40 << 10;                                // bytes of sums in a CTA
+  for (int cs = 1; cs <= 8; cs *= 2)
+    for (int kw = 1; kw <= 8; kw *= 2) {
+      const int own = (a.blocks + cs - 1) / cs, rs = kGgWarps / kw;
+      if (cs > a.blocks || kw > a.blocks / cs) continue;       // every warp has a block
+      // clusters that are on the GPU at once: those of four and eight do not fill every GPC (73 of four took two rounds, 68 one)
+      const int slots = cs <= 2 ? 2 * sms / cs : cs == 4 ? sms * 46 / 100 : sms * 22 / 100;
+      int run = (a.strips + slots - 1) / slots;
+      run = std::min(run, room / (64 * a.ncols * kw));
+      if (kw > 1 && run > rs) continue;                     // shares of k are for runs shorter than the warps
+      const long long waves = ((a.strips + run - 1) / run + slots - 1) / slots;
+      const long long cost = waves * (8ll * ((run + rs - 1) / rs) * ((own + kw - 1) / kw) + (long long)own * a.ncols + (cs > 1 ? 8 * cs : 0));
+      if (best >= 0 && cost >= best) continue;
+      best = cost;
+      a.cs = cs;
+      a.kw = kw;
+      a.run = run;
+      a.chunk = std::min(own, S::kChunk);
+    }
+  return (size_t)a.chunk * S::kPerBlock + gg_out_bytes(a.run, a.ncols, a.kw);
+}
+
+template <int GROUP, bool OFF, int MM>
 static void launch_gg(cudaStream_t st, GgArgs a, int sms) {
-  using S = GgShape<GROUP, OFF, NB>;
-  // Strips of a CTA and CTAs of a cluster: the fewest CTAs' rounds of blocks, then the fewest times that x is cut into digits.
-  a.rs = 8;
-  a.cs = 1;
-  while (a.rs > 1 && (a.strips + a.rs - 1) / a.rs < 2 * sms) a.rs /= 2;
-  while (a.cs < 8 && (a.strips + a.rs - 1) / a.rs * a.cs < 2 * sms && a.blocks / (a.cs * 2) >= 8 / a.rs) a.cs *= 2;
-  const int round = 8 / a.rs * S::kAhead, own = (a.blocks + a.cs - 1) / a.cs;
-  a.chunk = std::min(own, std::max(1, 64 / NB / round) * round);
-  const size_t smem = S::smem(a.chunk);
-  raise_dyn_smem(gemv_grouped_kernel<GROUP, OFF, NB>, S::smem(64 / NB > 8 * S::kAhead ? 64 / NB : 8 * S::kAhead));
+  using S = GgShape<GROUP, OFF, MM>;
+  const size_t smem = plan_gg<S>(a, sms);
+  raise_dyn_smem(gemv_grouped_kernel<GROUP, OFF, MM>, (size_t)S::kChunk * S::kPerBlock + (40 << 10));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.strips + a.rs - 1) / a.rs * a.cs));
+  cfg.gridDim = dim3((unsigned)((a.strips + a.run - 1) / a.run * a.cs));
   cfg.blockDim = dim3(kGgThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -39,15 +59,16 @@ static void launch_gg(cudaStream_t st, GgArgs a, int sms) {
   at[1].val.clusterDim.x = (unsigned)a.cs;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
-  B2_CUDA(cudaLaunchKernelEx(&cfg, gemv_grouped_kernel<GROUP, OFF, NB>, (const GgArgs)a));
+  cfg.numAttrs = a.cs > 1 ? 2 : 1;
+  B2_CUDA(cudaLaunchKernelEx(&cfg, gemv_grouped_kernel<GROUP, OFF, MM>, (const GgArgs)a));
 }
 
 template <int GROUP, bool OFF>
 static void launch_gg_cols(cudaStream_t st, const GgArgs& a, int sms) {
   if (a.ncols <= 2) launch_gg<GROUP, OFF, 1>(st, a, sms);
   else if (a.ncols <= 4) launch_gg<GROUP, OFF, 2>(st, a, sms);
-  else launch_gg<GROUP, OFF, 4>(st, a, sms);
+  else if (a.x_type == kF32) launch_gg<GROUP, OFF, 4>(st, a, sms);
+  else launch_gg<GROUP, OFF, 3>(st, a, sms);
 }
 
 }  // namespace b200lm

@@ -2,7 +2,8 @@
 64 bits, at the sizes and masks where they can go wrong.
 
 Tolerances.  u = 2^-24.  A stored value is off by half a step: eps / 2 of it, and of the smallest normal number below that.
-  product    every term is exact to 2^-28 of its block's largest |x|; a column is added up in fp32 along one chain of at most
+  product    x enters in digits of seven bits, the largest |x| of a block of 128 at least 2^5 of the first one's unit: four digits are
+             off by half of 2^-21 units, 2^-27 of that |x|, three (more than four columns of a 16-bit type) by 2^-20; a column is added up in fp32 along one chain of at most
              ceil(k / 32) + 2 adds a lane, joined by at most 12 more, each term behind two roundings: (ceil(k / 32) + 18) u sum |w x|
   norm       sum of hd / 32 + 5 adds, a root, a quotient: at most 16 u on the factor, four roundings behind it: 24 u (|a| + |b|)
   cache      codes are decided in 64 bits from values rounded once to 32: equal
@@ -70,7 +71,7 @@ def product(pkg, n, k, group, cols, x_type, y_type, s_type, offset, seed, ldx=0,
         w, size = w + o, size + o.abs()
     blocks = torch.nn.functional.pad(rows.abs(), (0, -k % 128)).view(cols, -1, 128).amax(-1).repeat_interleave(128, 1)[:, :k]
     want = rows @ w.T
-    bound = (-(-k // 32) + 18) * U * (rows.abs() @ size.T) + 2.0 ** -28 * (blocks @ size.T)
+    bound = (-(-k // 32) + 18) * U * (rows.abs() @ size.T) + (2.0 ** -20 if cols > 4 and x_type != torch.float32 else 2.0 ** -27) * (blocks @ size.T)
     got = y.view(cols, ldy)
     assert (got[:, n:] == 7.0).all()
     err = (got[:, :n].double() - want).abs()
