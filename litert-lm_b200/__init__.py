@@ -14,6 +14,7 @@ CUDA device every device entry point reports ``FAILED_PRECONDITION``.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 from typing import List, Optional, Sequence, Tuple
 
@@ -24,6 +25,7 @@ from . import sharding  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200lm.so")
+CALLS_PATH = os.path.join(_HERE, "_calls.so")
 
 # absl::StatusCode
 OK, CANCELLED, INVALID_ARGUMENT, DEADLINE_EXCEEDED, NOT_FOUND = 0, 1, 3, 4, 5
@@ -61,13 +63,13 @@ class Kv4Cache:
     """A paged cache in 4 bits in the caller's device memory (raw addresses): pages of ``page_bytes()`` each and a page
     table [batch][table_stride].  The memory has to outlive the calls that it is passed to."""
 
-    __slots__ = ("desc", "ref")
+    __slots__ = ("desc", "addr")
 
     def __init__(self, pages_dev: int, num_pages: int, page_table_dev: int, table_stride: int, batch: int, hkv: int, hd: int,
                  group: int = 64) -> None:
         self.desc = B200LmKv4Cache(C.sizeof(B200LmKv4Cache), batch, hkv, hd, group, 0, pages_dev, num_pages, page_table_dev,
                                    table_stride)
-        self.ref = C.byref(self.desc)
+        self.addr = C.addressof(self.desc)
 
     @staticmethod
     def page_bytes(hkv: int, hd: int, group: int = 64) -> int:
@@ -170,6 +172,22 @@ def tp_unique_id() -> bytes:
     buf = C.create_string_buffer(128)
     _call("B200Lm_TpUniqueId", C.cast(buf, C.c_void_p))
     return buf.raw
+
+
+_calls_module = None
+
+
+def _calls():
+    """The extension module over the operators that are called once per layer and step (ctypes takes 4 us for their arguments)."""
+    global _calls_module
+    if _calls_module is None:
+        load_library()
+        if not os.path.exists(CALLS_PATH):
+            raise RuntimeError(f"{CALLS_PATH} is missing: build it with `python litert-lm_b200/build.py`")
+        spec = importlib.util.spec_from_file_location("_calls", CALLS_PATH)
+        _calls_module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_calls_module)
+    return _calls_module
 
 
 _libc = C.CDLL(None)
@@ -515,24 +533,20 @@ class ops:
                         stream: int = 0, device: int = 0) -> None:
         """y[c] = W x[c] for 1 .. 8 columns, W int4 with a scale (and offset) for each group of k; rows of x and y are ldx
         and ldy elements apart (0: k and n)."""
-        err = C.c_char_p()
-        code = (_lib or load_library()).B200LmOps_GemvW4Grouped(
-            device, w_dev, scale_type, has_offset, n, k, group, x_dev, x_type, ldx or k, ncols, y_dev, y_type, ldy or n, stream or None,
-            C.byref(err))
-        if code != OK:
-            _check(code, err)
+        failed = (_calls_module or _calls()).gemv_w4_grouped(device, w_dev, scale_type, has_offset, n, k, group, x_dev, x_type, ldx or k, ncols, y_dev,
+                                                             y_type, ldy or n, stream)
+        if failed:
+            raise StatusError(*failed)
 
     @staticmethod
     def qk_norm_rope(qkv_dev: int, type: int, qkv_stride: int, tokens: int, hq: int, hkv: int, hd: int, rot: int, q_gain_dev: int,
                      k_gain_dev: int, eps: float, cos_dev: int, sin_dev: int, rope_rows: int, pos_dev: int, q_out_dev: int, q_stride: int,
                      k_out_dev: int, k_stride: int, status_dev: int = 0, stream: int = 0, device: int = 0) -> None:
         """RMSNorm of each query and key head and the rotation, in one pass over rows of a fused QKV projection."""
-        err = C.c_char_p()
-        code = (_lib or load_library()).B200LmOps_QkNormRope(
-            device, qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev,
-            q_out_dev, q_stride, k_out_dev, k_stride, status_dev, stream or None, C.byref(err))
-        if code != OK:
-            _check(code, err)
+        failed = (_calls_module or _calls()).qk_norm_rope(device, qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev,
+                                                          sin_dev, rope_rows, pos_dev, q_out_dev, q_stride, k_out_dev, k_stride, status_dev, stream)
+        if failed:
+            raise StatusError(*failed)
 
     @staticmethod
     def qk_norm_rope_append_kv4(qkv_dev: int, type: int, qkv_stride: int, tokens: int, hq: int, hkv: int, hd: int, rot: int,
@@ -540,22 +554,19 @@ class ops:
                                 q_out_dev: int, q_stride: int, cache: Kv4Cache, seq_dev: int = 0, status_dev: int = 0, stream: int = 0,
                                 device: int = 0) -> None:
         """`qk_norm_rope` whose keys, with the rows' values, go into the cache in 4 bits."""
-        err = C.c_char_p()
-        code = (_lib or load_library()).B200LmOps_QkNormRopeAppendKv4(
-            device, qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev,
-            q_out_dev, q_stride, cache.ref, seq_dev, status_dev, stream or None, C.byref(err))
-        if code != OK:
-            _check(code, err)
+        failed = (_calls_module or _calls()).qk_norm_rope_append_kv4(device, qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps,
+                                                                     cos_dev, sin_dev, rope_rows, pos_dev, q_out_dev, q_stride, cache.addr, seq_dev, status_dev,
+                                                                     stream)
+        if failed:
+            raise StatusError(*failed)
 
     @staticmethod
     def kv4_read(cache: Kv4Cache, seq_dev: int, pos_dev: int, tokens: int, out_type: int, k_out_dev: int, v_out_dev: int,
                  status_dev: int = 0, stream: int = 0, device: int = 0) -> None:
         """The values that cached positions stand for, [tokens][hkv][hd]."""
-        err = C.c_char_p()
-        code = (_lib or load_library()).B200LmOps_Kv4Read(device, cache.ref, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev,
-                                                          status_dev, stream or None, C.byref(err))
-        if code != OK:
-            _check(code, err)
+        failed = (_calls_module or _calls()).kv4_read(device, cache.addr, seq_dev, pos_dev, tokens, out_type, k_out_dev, v_out_dev, status_dev, stream)
+        if failed:
+            raise StatusError(*failed)
 
     @staticmethod
     def attention_kv4_workspace(batch: int, hkv: int, hd: int, hq: int, max_q: int, max_kv: int, device: int = 0) -> int:
@@ -569,9 +580,7 @@ class ops:
                       max_kv: int, hq: int, out_dev: int, out_stride: int, workspace_dev: int = 0, workspace_bytes: int = 0,
                       window: int = 0, scale: float = 0.0, status_dev: int = 0, stream: int = 0, device: int = 0) -> None:
         """Attention of ragged sequences over the cache: causal, windowed, one query token a sequence or many."""
-        err = C.c_char_p()
-        code = (_lib or load_library()).B200LmOps_AttentionKv4(
-            device, cache.ref, q_dev, q_type, q_stride, kv_len_dev, q_start_dev, tokens, max_q, max_kv, hq, window, scale, out_dev, out_stride,
-            workspace_dev, workspace_bytes, status_dev, stream or None, C.byref(err))
-        if code != OK:
-            _check(code, err)
+        failed = (_calls_module or _calls()).attention_kv4(device, cache.addr, q_dev, q_type, q_stride, kv_len_dev, q_start_dev, tokens, max_q, max_kv, hq, window,
+                                                           scale, out_dev, out_stride, workspace_dev, workspace_bytes, status_dev, stream)
+        if failed:
+            raise StatusError(*failed)

@@ -2,6 +2,7 @@
 
     python litert-lm_b200/build.py [--force]
 
+Beside it lies `_calls.so`, the Python binding of the operators that are called once per layer and step.
 The shared library is self-contained (static CUDA runtime) and exports the C ABI
 declared in include/b200lm.h and include/b200lm_ops.h.
 """
@@ -11,12 +12,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200lm.so")
+CALLS = os.path.join(HERE, "_calls.so")      # the per-step operators as a Python extension module, bound to the library beside it
 # one translation unit per kernel family and cache type, compiled side by side
 SOURCES = ["lib.cu", "decode_step.cu", "ops_gemv_grouped.cu", "ops_kv4.cu"] + [f"kv4_attn_{s}.cu" for s in ("64", "128", "256", "tc")] + [f"{k}_{t}.cu" for k in ("decode_stream", "decode_wide", "attn_mma") for t in ("f32", "bf16")]
 
@@ -24,7 +27,7 @@ SOURCES = ["lib.cu", "decode_step.cu", "ops_gemv_grouped.cu", "ops_kv4.cu"] + [f
 def _deps():
     """Every file the translation unit can include."""
     inc = os.path.join(HERE, "..", "include")
-    files = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h"))]
+    files = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h", ".c"))]
     files += [os.path.join(inc, f) for f in os.listdir(inc) if f.endswith(".h")]
     return files
 
@@ -37,9 +40,9 @@ def nvcc_path() -> str:
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(CALLS):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(CALLS))
     return any(os.path.getmtime(d) > t for d in _deps())
 
 
@@ -66,6 +69,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
             list(pool.map(run, [[nvcc] + flags + ["-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(SOURCES, objs)]))
         run([nvcc] + flags + ["-shared", "-o", LIB] + objs)
+    run(["gcc", "-O2", "-Wall", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"], os.path.join(CSRC, "calls.c"), "-o", CALLS, "-L", HERE, "-lb200lm",
+         "-Wl,-rpath,$ORIGIN"])
     return LIB
 
 
