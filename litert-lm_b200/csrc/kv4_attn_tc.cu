@@ -6,7 +6,7 @@ namespace b200lm {
 template <int HD, int GROUP>
 static void launch_kv4_chunk_as(cudaStream_t st, const Kv4AttnArgs& a) {
   raise_dyn_smem(kv4_chunk_kernel<HD, GROUP>, KcShape<HD>::kSmem);
-  launch_pdl(kv4_chunk_kernel<HD, GROUP>, dim3((unsigned)(a.row_tiles * a.splits * a.kv.hkv), (unsigned)a.kv.batch), dim3(kKcThreads), KcShape<HD>::kSmem, st, a);
+  launch_pdl(kv4_chunk_kernel<HD, GROUP>, dim3((unsigned)(a.row_tiles * a.splits * a.kv.hkv), (unsigned)a.kv.batch), dim3(KcShape<HD>::kThreads), KcShape<HD>::kSmem, st, a);
 }
 
 void launch_kv4_chunk(cudaStream_t st, const Kv4AttnArgs& a) {

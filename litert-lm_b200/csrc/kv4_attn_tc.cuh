@@ -4,7 +4,7 @@
 // s (c - 8) + (m + 8 s) on the way (the quantiser keeps them inside fp16's range), two roundings of at most 2^-11 of the group's
 // largest (storing a bf16 row costs 2^-8); queries are bf16 numbers times a power of two of their row, exact in fp16.
 //
-//   warps 9 - 16  expand: codes from global memory a tile ahead, K and V rows into swizzled shared memory (two stages each)
+//   the others    expand: codes from global memory a tile ahead, K and V rows into swizzled shared memory (two stages each)
 //   warp 8        issues the products: S = Q K^T with Q in tensor memory (read from shared memory it would take half of the
 //                 bandwidth that the expanded rows need), O += P V with P in tensor memory, over the scores it was made from
 //   warps 0 - 7   softmax, two threads a row (half of the keys, half of O each).  A row's reference moves when a score passes it
@@ -27,11 +27,12 @@
 
 namespace b200lm {
 
-constexpr int kKcRows = 128, kKcSoft = 256, kKcExpand = 256, kKcThreads = kKcSoft + 32 + kKcExpand;
+constexpr int kKcRows = 128, kKcSoft = 256;
 
 template <int HD>
 struct KcShape {
   static constexpr int KT = 64;                                      // keys of a tile
+  static constexpr int kThreads = kKcSoft + 32 + HD * 2;             // 4 warps for K, 4 for V of every 128 elements
   static constexpr int kTile = KT * HD * 2;                          // K or V of a tile
   static constexpr int kMax = 4 * kTile;                             // [2][128] floats
   static constexpr int kBars = kMax + 2 * 128 * 4;
@@ -50,7 +51,7 @@ __device__ __forceinline__ uint32_t kc_values(uint32_t x, __half2 s, __half2 mid
 }
 
 template <int HD, int GROUP>
-__global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(const Kv4AttnArgs a) {
   using S = KcShape<HD>;
   constexpr int KT = S::KT, P = HD / 128, HK = KT / 2;
   constexpr Kv4Dims d{HD, GROUP};
@@ -105,13 +106,12 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
   const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
   float m = -INFINITY, l = 0.f;
   if (n > 0 && warp >= 9) {
-    // ---- expansion: thread (key, plane, q): 32 bytes of a K row (64 elements), 32 of a V row
-    // (at head size 128 the first four warps have the K rows, the others the V rows)
-    const int w = warp - 9, key = (P == 2 ? w / 2 : w % 4) * 16 + (lane & 15), plane = P == 2 ? w % 2 : 0, q = lane >> 4;
-    const bool has_k = P == 2 || w < 4, has_v = P == 2 || w >= 4;
+    // ---- expansion: the first half of the warps has K rows, the other V rows; thread (key, plane, q): 32 bytes, 64 elements
+    const int w = (warp - 9) % (4 * P), key = w / P * 16 + (lane & 15), plane = w % P, q = lane >> 4;
+    const bool has_k = warp - 9 < 4 * P;
     const int* table = a.kv.table + b * a.kv.table_stride;
     const long long page_bytes = (long long)a.kv.hkv * d.head_bytes(), head = (long long)kvh * d.head_bytes();
-    uint4 kr[2], vr[2];
+    uint4 raw[2];
     uint32_t ks[2], vs[2];
     int page_ahead = __ldg(table + t0 * KT / kKv4Page);               // of the next tile to load: its number is a tile ahead of its rows
     auto load = [&](int j) {
@@ -122,16 +122,9 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
         return;
       }
       const uint8_t* h = a.kv.pages + page * page_bytes + head;
-      const uint8_t* k = h + d.k_codes() + (plane * kKv4Page + slot) * 64 + q * 32;
-      const uint8_t* v = h + d.v_codes() + (plane * kKv4Page + slot) * 64 + q * 32;
-      if (has_k) {
-        kr[0] = ldg_nc_v4(reinterpret_cast<const uint4*>(k));
-        kr[1] = ldg_nc_v4(reinterpret_cast<const uint4*>(k) + 1);
-      }
-      if (has_v) {
-        vr[0] = ldg_nc_v4(reinterpret_cast<const uint4*>(v));
-        vr[1] = ldg_nc_v4(reinterpret_cast<const uint4*>(v) + 1);
-      }
+      const uint8_t* src = h + (has_k ? d.k_codes() : d.v_codes()) + (plane * kKv4Page + slot) * 64 + q * 32;
+      raw[0] = ldg_nc_v4(reinterpret_cast<const uint4*>(src));
+      raw[1] = ldg_nc_v4(reinterpret_cast<const uint4*>(src) + 1);
       const uint32_t* kp = reinterpret_cast<const uint32_t*>(h + d.k_scales()) + slot * d.groups() + plane * 128 / GROUP;
       const uint32_t* vp = reinterpret_cast<const uint32_t*>(h + d.v_scales()) + slot * d.groups() + plane * 128 / GROUP;
       ks[0] = __ldg(kp);
@@ -139,7 +132,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
       ks[1] = GROUP == 64 ? __ldg(kp + 1) : ks[0];
       vs[1] = GROUP == 64 ? __ldg(vp + 1) : vs[0];
     };
-    kr[0] = kr[1] = vr[0] = vr[1] = make_uint4(0u, 0u, 0u, 0u);
+    raw[0] = raw[1] = make_uint4(0u, 0u, 0u, 0u);
     ks[0] = ks[1] = vs[0] = vs[1] = 0u;
     load(0);
     auto pair = [](uint32_t u, __half2& s, __half2& mid) {
@@ -151,8 +144,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int st = j & 1, use = j >> 1;
-      uint32_t kw[8] = {kr[0].x, kr[0].y, kr[0].z, kr[0].w, kr[1].x, kr[1].y, kr[1].z, kr[1].w};
-      uint32_t vw[8] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w, vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+      const uint32_t word[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
       uint32_t k2[2] = {ks[0], ks[1]}, v2[2] = {vs[0], vs[1]};
       if (j + 1 < n) load(j + 1);
       const int slot = (t0 + j) * KT % kKv4Page + key, where = (t0 + j) * KT + key;
@@ -162,50 +154,49 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
         if (nan(v2[0])) v2[0] = 0u;
         if (nan(v2[1])) v2[1] = 0u;
       }
-      if (has_k && use > 0) ok = ok && mbar_wait(&k_empty[st], (use - 1) & 1, gave_up);
+      if (use > 0) ok = ok && mbar_wait(has_k ? &k_empty[st] : &v_empty[st], (use - 1) & 1, gave_up);
       if (has_k && ok) {
         unsigned char* line = kc_sm + st * S::kTile + key * 128;
+        __half2 s, mid;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                                // 32 elements: 8 q .. and 16 more, of the words 2 q and 2 q + 1
-          __half2 s, mid;
-          pair(k2[i / 2], s, mid);
-          const uint32_t x0 = __byte_perm(kw[i], 0, 0x4140), x1 = __byte_perm(kw[i], 0, 0x4342), x2 = __byte_perm(kw[4 + i], 0, 0x4140), x3 = __byte_perm(kw[4 + i], 0, 0x4342);
+          if (i == 0 || (GROUP == 64 && i == 2)) pair(k2[i / 2], s, mid);
+          const uint32_t x0 = __byte_perm(word[i], 0, 0x4140), x1 = __byte_perm(word[i], 0, 0x4342), x2 = __byte_perm(word[4 + i], 0, 0x4140), x3 = __byte_perm(word[4 + i], 0, 0x4342);
           unsigned char* at = line + (plane * 2 + i / 2) * KT * 128;
           const int c = 4 * (i & 1) + q;
           *reinterpret_cast<uint4*>(at + ((c ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
           *reinterpret_cast<uint4*>(at + (((c + 2) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
         }
       }
-      fence_async_smem();
-      if (has_k) mbar_arrive(&k_full[st]);
       // V: this thread has two words of four units; it wants word q of all eight, the partner (lane ^ 16) the other words
-      uint32_t mine[4], got[4], unit[8];
+      if (!has_k) {
+        uint32_t mine[4], got[4], unit[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mine[i] = q ? vw[2 * i + 1] : vw[2 * i];
-        got[i] = __shfl_xor_sync(0xffffffffu, q ? vw[2 * i] : vw[2 * i + 1], 16);
-      }
-      const bool low = q == (slot >> 1 & 1);                         // the units that it has are the first four
+        for (int i = 0; i < 4; ++i) {
+          mine[i] = q ? word[2 * i + 1] : word[2 * i];
+          got[i] = __shfl_xor_sync(0xffffffffu, q ? word[2 * i] : word[2 * i + 1], 16);
+        }
+        const bool low = q == (slot >> 1 & 1);                         // the units that it has are the first four
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        unit[i] = low ? mine[i] : got[i];
-        unit[4 + i] = low ? got[i] : mine[i];
-      }
-      if (has_v && use > 0) ok = ok && mbar_wait(&v_empty[st], (use - 1) & 1, gave_up);
-      if (has_v && ok) {
-        unsigned char* line = kc_sm + (2 + st) * S::kTile + (plane * 2 + q) * KT * 128 + key * 128;
-        __half2 s, mid;
-        pair(v2[GROUP == 64 ? q : 0], s, mid);
+        for (int i = 0; i < 4; ++i) {
+          unit[i] = low ? mine[i] : got[i];
+          unit[4 + i] = low ? got[i] : mine[i];
+        }
+        if (ok) {
+          unsigned char* line = kc_sm + (2 + st) * S::kTile + (plane * 2 + q) * KT * 128 + key * 128;
+          __half2 s, mid;
+          pair(v2[GROUP == 64 ? q : 0], s, mid);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                                // byte i of the words: 16 neighbours
-          const uint32_t sel = i | (4 + i) << 8;
-          const uint32_t x0 = __byte_perm(unit[0], unit[1], sel), x1 = __byte_perm(unit[2], unit[3], sel), x2 = __byte_perm(unit[4], unit[5], sel), x3 = __byte_perm(unit[6], unit[7], sel);
-          *reinterpret_cast<uint4*>(line + (((2 * i) ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
-          *reinterpret_cast<uint4*>(line + (((2 * i + 1) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
+          for (int i = 0; i < 4; ++i) {                                // byte i of the words: 16 neighbours
+            const uint32_t sel = i | (4 + i) << 8;
+            const uint32_t x0 = __byte_perm(unit[0], unit[1], sel), x1 = __byte_perm(unit[2], unit[3], sel), x2 = __byte_perm(unit[4], unit[5], sel), x3 = __byte_perm(unit[6], unit[7], sel);
+            *reinterpret_cast<uint4*>(line + (((2 * i) ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
+            *reinterpret_cast<uint4*>(line + (((2 * i + 1) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
+          }
         }
       }
       fence_async_smem();
-      if (has_v) mbar_arrive(&v_full[st]);
+      mbar_arrive(has_k ? &k_full[st] : &v_full[st]);
       ok = __all_sync(0xffffffffu, ok);
     }
   } else if (n > 0 && warp == 8) {
@@ -311,7 +302,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
           uint32_t x[32];
           tmem_ld32(lane_addr + S::kS + (j & 1) * KT + half * HK + c, x);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(x[i]) * unit;
+          for (int i = 0; i < 32; ++i) s[c + i] = __uint_as_float(x[i]);
         }
         if (base < open0 || base + KT > open1) {
 #pragma unroll
@@ -320,6 +311,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
         }
 #pragma unroll
         for (int i = 0; i < HK; ++i) mx = fmaxf(mx, s[i]);
+        mx *= unit;                                                  // positive, or NaN
       }
       if (bar_or<1, 256>(!got || mx > m + 8.f)) {
         // the eight warps leave the loop together, or move the references of all rows
@@ -351,7 +343,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
         uint32_t y[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float p0 = ka_ex2(s[c + i] - mz), p1 = ka_ex2(s[c + i + 1] - mz);
+          const float p0 = ka_ex2(fmaf(s[c + i], unit, -mz)), p1 = ka_ex2(fmaf(s[c + i + 1], unit, -mz));
           l += p0 + p1;
           y[i / 2] = ka_pack(p0, p1);
         }
@@ -441,7 +433,7 @@ __global__ void __launch_bounds__(kKcThreads, 1) kv4_chunk_kernel(const Kv4AttnA
   }
   if (__syncthreads_or(lost)) return;                                // the CTA that lost it has said so
 #pragma unroll 1
-  for (int i = threadIdx.x; i < rows * HD / 8; i += kKcThreads) {
+  for (int i = threadIdx.x; i < rows * HD / 8; i += S::kThreads) {
     const int r = i / (HD / 8), dim = i % (HD / 8) * 8;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
