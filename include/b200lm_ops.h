@@ -262,8 +262,9 @@ int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, const int32_t
  * max_kv, max_kv at most 256 * table_stride.  scale <= 0 means 1/sqrt(hd).  out_dev
  * is of q's type; rows behind the last sequence's are left as they were.
  *
- * workspace_dev (16-byte boundary; NULL where AttentionKv4Workspace says 0) holds the
- * partial results of sequences whose keys are shared out.  Zero it once before its
+ * workspace_dev (16-byte boundary) holds the partial results of sequences whose
+ * keys are shared out; AttentionKv4Workspace says how many bytes calls up to the
+ * given sizes may need (10 MB for single tokens, up to 20 MB for chunks).  Zero it once before its
  * first use; every call leaves the part that has to be zero at zero.  It serves one
  * call at a time: calls, or replays of captured ones, that may overlap need
  * workspaces of their own. */

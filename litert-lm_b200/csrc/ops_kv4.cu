@@ -133,11 +133,7 @@ struct Kv4Plan {
   int rb, row_tiles, share, splits;
   int64_t units, bytes;
 };
-#ifndef KCR
-#define KCR 32
-#endif
-constexpr int kChunkRows = KCR;             // query rows of a kv head from which the tensor-core kernel takes a bf16 call
-static bool chunk_call(int hd, int hq, int hkv, int max_q, int type) { return type == kBf16 && hd >= 128 && (long long)max_q * (hq / hkv) >= kChunkRows; }
+constexpr int kChunkRows = 16;             // fewer query rows of a kv head never pay for the tensor-core kernel
 
 // The tensor-core kernel: one CTA an SM, tiles of 64 keys.
 static Kv4Plan plan_chunk(int batch, int hkv, int hd, int hq, int max_q, int max_kv, int window, int sms) {
@@ -154,7 +150,7 @@ static Kv4Plan plan_chunk(int batch, int hkv, int hd, int hq, int max_q, int max
   best = std::max<long long>(1, std::min(best, keys / (4 * round)));                    // of at least four tiles each
   p.share = (int)std::min<long long>((keys / best + round) / round * round, 1 << 30);
   p.splits = (int)((keys + p.share - 1) / p.share);
-  p.bytes = p.units * 2 > sms ? 0 : kKaTickets * 4 + std::min<int64_t>(sms, p.units * 16) * 128 * (hd + 2) * 4;
+  p.bytes = kKaTickets * 4 + std::min<int64_t>(sms, p.units * 16) * 128 * (hd + 2) * 4;
   return p;
 }
 static Kv4Plan plan_attention(int batch, int hkv, int hd, int hq, int max_q, int max_kv, int window, int sms) {
@@ -175,9 +171,19 @@ static Kv4Plan plan_attention(int batch, int hkv, int hd, int hq, int max_q, int
   p.share = (int)std::min<long long>(std::max(length(shares(8)), std::min<long long>(4 * round, length(shares(2)))), 1 << 30);
   p.splits = (int)((keys + p.share - 1) / p.share);
   B2_CHECK(tiles * hkv * p.splits <= 0x7FFFFFFF, kInvalidArgument, "too many query rows for one call");
-  // what a call of any length up to these sizes may need
-  p.bytes = shares(8) == 1 ? 0 : kKaTickets * 4 + p.units * shares(8) * p.rb * (hd + 2) * 4;
+  // What a call up to these sizes may need: fewer units can have more shares, but all of them at most these.
+  p.bytes = kKaTickets * 4 + std::min<int64_t>(512 * p.units, 8 * sms) * p.rb * (hd + 2) * 4;
   return p;
+}
+
+// Which of the two a call takes, by what they would cost in us.  Fitted to 2 .. 1024 rows over 2048 and 4096 keys of 1, 16 and 64
+// sequences: mma.sync grows with rows x keys (64 sequences x 4 kv heads x 16 rows x 4096 keys of 256: 243 us, 32 rows 434),
+// the tensor-core kernel with tiles of 128 rows (261 and 263, and 25 us at the least, where four rows over 4096 keys take 11).
+static bool chunk_pays(const Kv4Plan& few, const Kv4Plan& many, int hd, int max_kv, int window, int max_q, int sms) {
+  const double keys = window > 0 ? std::min<double>(max_kv, (double)window + max_q) : max_kv;
+  const double simple = 8 + 0.25e-6 * (double)few.units * keys * hd;
+  const double tiles = (double)((many.units * many.splits + sms - 1) / sms) * many.share / 64;
+  return 20 + tiles * (hd == 256 ? 1.45 : 0.8) < simple;
 }
 
 }  // namespace b200lm
@@ -283,6 +289,7 @@ static void check_attention(int batch, int hkv, int hd, int hq, int max_q, int m
   check_query_heads(hq);
   B2_CHECK(batch > 0 && batch <= 65535, kInvalidArgument, "batch must be 1 .. 65535");
   B2_CHECK(hq % hkv == 0, kInvalidArgument, "hq must be a multiple of hkv");
+  B2_CHECK((long long)max_q * (hq / hkv) <= (1 << 30), kInvalidArgument, "too many query rows for one call");
   B2_CHECK(max_q >= 1 && max_q <= (1 << 30) && max_kv >= 0 && max_kv <= (1 << 30), kInvalidArgument, "max_q must be 1 .. 2^30, max_kv 0 .. 2^30");
 }
 
@@ -295,7 +302,7 @@ extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, in
   DeviceScope scope(device);
   const int sms = device_sms(device);
   *bytes = plan_attention(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes;
-  if (chunk_call(hd, hq, hkv, max_q, kBf16)) *bytes = std::max(*bytes, plan_chunk(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes);
+  if (hd >= 128 && (long long)max_q * (hq / hkv) >= kChunkRows) *bytes = std::max(*bytes, plan_chunk(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes);
   KV4_END
 }
 
@@ -326,8 +333,14 @@ extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cach
   a.qscale = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)cache->hd));
   a.out = out_dev; a.out_stride = out_stride; a.status = status_dev;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool chunk = chunk_call(cache->hd, hq, cache->hkv, max_q, q_type);
-  const Kv4Plan p = (chunk ? plan_chunk : plan_attention)(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv, window, device_sms(device));
+  const int sms = device_sms(device);
+  Kv4Plan p = plan_attention(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv, window, sms);
+  bool chunk = false;
+  if (q_type == kBf16 && cache->hd >= 128 && (long long)max_q * (hq / cache->hkv) >= kChunkRows) {
+    const Kv4Plan many = plan_chunk(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv, window, sms);
+    chunk = chunk_pays(p, many, cache->hd, max_kv, window, max_q, sms);
+    if (chunk) p = many;
+  }
   B2_CHECK(p.splits == 1 || (workspace_dev && workspace_bytes >= p.bytes), kInvalidArgument,
            "the workspace is smaller than AttentionKv4Workspace says: " + std::to_string(p.bytes) + " bytes");
   a.row_tiles = p.row_tiles; a.share = p.share; a.splits = p.splits;

@@ -10,7 +10,7 @@ Tolerances.  u = 2^-24.  A stored value is off by half a step: eps / 2 of it, an
   attention  a score is off by dS = 8 u sum |q k| scale + 2^-20 (the exponent's own error, 2^-22, and its argument's rounding among it),
              a weight by 2 dS and what it is held in, one fp16 term (half a step: 2^-11) for bf16 rows, two (2^-22) else; with the
              sums' own error of 64 u that times the largest |v| bounds the result's.
-             Chunks of bf16 rows (32 rows of a kv head and more, head sizes 128 and 256) meet K and V as fp16 numbers
+             Chunks of bf16 rows (head sizes 128 and 256, 16 rows of a kv head and more) may meet K and V as fp16 numbers
              s (c - 8) + (m + 8 s), two roundings of at most 2^-11 of the largest |k| or |v| each.  The roundings of a key's elements
              are independent: by Hoeffding's bound the score is off by more than 6 * 2^-10 max |k| |q| scale (|q| the 2-norm) with
              probability 2 exp(-18) = 3e-8; that is added to dS, and 2^-10 to what multiplies the largest |v|
@@ -353,7 +353,7 @@ class Attention:
             want = torch.einsum("hgts,shd->thgd", p, v)
             d = 8 * U * (size.amax() if n else 0) + 2.0 ** -20
             held_in = 2.0 ** -11 if self.typ == torch.bfloat16 else 2.0 ** -22
-            if self.typ == torch.bfloat16 and hd >= 128 and self.max_q * (hq // hkv) >= 32 and n:
+            if self.typ == torch.bfloat16 and hd >= 128 and self.max_q * (hq // hkv) >= 16 and n:
                 d = d + 6 * 2.0 ** -10 * k.abs().amax() * q.norm(dim=-1).amax() * used
                 held_in += 2.0 ** -10
             bound = (2 * d + held_in + 64 * U) * (v.abs().amax() if n else 0)
@@ -397,9 +397,9 @@ def test_attention_of_several_tokens(pkg, hq, hkv, hd, group, typ):
 @pytest.mark.parametrize("hq,hkv,hd,group", HEADS)
 @pytest.mark.parametrize("typ", TYPES)
 def test_attention_of_chunks(pkg, hq, hkv, hd, group, typ):
-    lens, counts = [700, 130, 1025], [700, 129, 300]
+    lens, counts = [700, 130, 5, 1025, 0, 64, 300], [700, 129, 5, 300, 9, 100, 1]
     a = Attention(pkg, lens, counts, hq, hkv, hd, group, typ, seed=hd * 5 + hq)
-    for window in (0, 130):
+    for window in (0, 1, 130):
         a.out.fill_(7.0)
         a(window=window)
         assert pkg.ops.device_status(a.status.data_ptr(), stream()) == 0
@@ -441,6 +441,38 @@ def test_attention_shows_what_is_not_a_number(pkg):
     assert torch.isfinite(got[:2]).all() and torch.isfinite(got[:, 2:]).all() and torch.isnan(got[2:, :2]).any()
     a(window=1)                                            # the last token's window no longer holds position 298
     assert torch.isfinite(a.out[7, :512]).all()
+
+
+@pytest.mark.parametrize("typ", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,hd,group", [(8, 4, 256, 64), (8, 2, 128, 128)])
+def test_chunks_show_what_is_not_a_number_and_bad_pages(pkg, typ, hq, hkv, hd, group):
+    """As below, at sizes that take the tensor-core kernel: sequence 1 has a NaN in one key, sequence 2 in one value, sequence 3 a
+    page outside the pool."""
+    lens, counts = [900, 700, 900, 800], [600, 500, 800, 300]
+    a = Attention(pkg, lens, counts, hq, hkv, hd, group, typ, seed=12)
+    one = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")               # noqa: E731
+    k, v = torch.randn(1, hkv, hd, device="cuda"), torch.randn(1, hkv, hd, device="cuda")
+    k[0, 0, 3] = float("nan")
+    put(pkg, a.cache, one(1), one(650), k, v)
+    k[0, 0, 3], v[0, 1, hd - 1] = 0.0, float("inf")
+    put(pkg, a.cache, one(2), one(500), k, v)
+    a.cache.table[3, 2] = -7
+    a()
+    with pytest.raises(pkg.StatusError) as e:
+        pkg.ops.device_status(a.status.data_ptr(), stream())
+    assert e.value.code == pkg.INVALID_ARGUMENT
+    a.check(skip=(1, 2, 3))
+    g = hq // hkv
+    rows = lambda b: a.out[int(a.start[b]):int(a.start[b]) + counts[b], :hq * hd].view(counts[b], hq, hd)      # noqa: E731
+    for b, pos, head in ((1, 650, 0), (2, 500, 1)):
+        sees = torch.arange(lens[b] - counts[b], lens[b], device="cuda") >= pos
+        bad = torch.isnan(rows(b)[:, head * g:(head + 1) * g]).any(-1)
+        assert bad[sees].all() and not bad[~sees].any()
+        others = [h for h in range(hq) if h // g != head]
+        assert torch.isfinite(rows(b)[:, others]).all()
+    # tiles of rows that do not reach the bad page may be served; those that do are left alone
+    last = rows(3)[-60:]
+    assert (last == 7.0).all()
 
 
 def test_attention_reports_bad_lengths_and_pages(pkg):
@@ -499,6 +531,10 @@ def test_calls_on_another_stream_and_in_a_graph(pkg):
 def test_workspace_is_asked_for_and_checked(pkg):
     a = Attention(pkg, [30000], [1], 4, 1, 256, 64, torch.float32, seed=1)
     assert a.need == pkg.ops.attention_kv4_workspace(1, 1, 256, 4, 1, 30000)
+    for smaller in [(1, 1, 256, 4, 1, 5000), (1, 1, 256, 4, 1, 0)]:
+        assert pkg.ops.attention_kv4_workspace(*smaller) <= a.need
+    sizes = [pkg.ops.attention_kv4_workspace(b, 4, 128, 8, q, 9000) for b in (1, 7, 64, 300, 3000) for q in (1, 40)]
+    assert sizes[0::2] == sorted(sizes[0::2]) and sizes[1::2] == sorted(sizes[1::2])      # a larger one serves smaller calls
     if a.need:
         for ptr, size in ((0, a.need), (a.room.data_ptr(), a.need - 1)):
             with pytest.raises(pkg.StatusError) as e:

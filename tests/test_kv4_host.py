@@ -109,7 +109,7 @@ def test_cache_and_attention_refusals(pkg):
     for bad in [(P, 0, 1, 0, P, P), (P, P, -1, 0, P, P), (P, P, 1, 9, P, P), (P, P, 1, 0, 0, 0), (P, P, 1, 0, P + 2, P), (0, P, 3, 0, P, P), (P, P + 1, 1, 0, P, P)]:
         refused(pkg, 3, pkg.ops.kv4_read, cache, *bad)
     refused(pkg, 3, pkg.ops.device_status, 0)
-    for bad in [(0, 1, 128, 4, 1, 100), (1, 3, 128, 4, 1, 100), (1, 1, 128, 4, 0, 100), (1, 1, 128, 4, 1, -1)]:
+    for bad in [(0, 1, 128, 4, 1, 100), (1, 3, 128, 4, 1, 100), (1, 1, 128, 4, 0, 100), (1, 1, 128, 4, 1, -1), (1, 1, 128, 4, 1 << 29, 100)]:
         refused(pkg, 3, pkg.ops.attention_kv4_workspace, *bad)
     refused(pkg, 12, pkg.ops.attention_kv4_workspace, 1, 1, 80, 4, 1, 100)
 
