@@ -7,8 +7,9 @@
 // of them, and the precision lies in the other operand: x is cut, for each column and block of 128 k, into digits of seven bits,
 // x = 2^e (t0 + t1 / 2^7 + t2 / 2^14 [+ t3 / 2^21]) with |t| <= 64, exact to 2^-20 (three) or 2^-27 (four) of the block's
 // largest value.  A product of eight columns takes four digits of two columns of x; five to eight columns of a 16-bit type take
-// three products, one a digit (their numbers are exact in three unless they are below 2^-9 of the largest).  The integer sums are exact.  They enter fp32 once a group: an accumulator that starts at the bits of
-// 1.5 * 2^23 is read as a float and 1.5 * 2^23 taken off (|sum| <= 128 * 64 * 128 < 2^22, so nothing is rounded).
+// three products, one a digit (their numbers are exact in three unless they are below 2^-9 of the largest).  The integer
+// sums are exact.  They enter fp32 once a group: an accumulator that starts at the bits of 1.5 * 2^23 is read as a float and
+// 1.5 * 2^23 taken off (|sum| <= 128 * 64 * 128 < 2^22, so nothing is rounded).
 //
 // The GPU's CTAs (two an SM) are clusters of `cs` that share the blocks of k and take an equal run of strips (16 rows) each.  A
 // CTA cuts its part of x into digits once (done for every strip it cost 17 us of 43008 x 5376 with eight columns), then its warps
@@ -19,7 +20,6 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
-#include "decode_ops.cuh"
 
 namespace b200lm {
 

@@ -3,9 +3,9 @@
 #include <stdint.h>
 
 #ifdef __CUDACC__
-#define B2_KV4_FN __host__ __device__ __forceinline__
+#define B2_KV4_FN __host__ __device__ __forceinline__ constexpr
 #else
-#define B2_KV4_FN inline
+#define B2_KV4_FN inline constexpr
 #endif
 
 namespace b200lm {

@@ -230,15 +230,30 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[kVec], uint32_t (&
 // Places of the element e0 = 8 i in a K or V row whose planes lie one behind the other: K has the bytes of its neighbours in two
 // words a quarter of a plane's row apart, V has them in the same byte of eight units (`place` of the first four, of the others).
 template <int HD>
-__device__ __forceinline__ uint32_t k_place(uint32_t e0) {
+__host__ __device__ __forceinline__ constexpr uint32_t k_place(uint32_t e0) {
   constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2;
   return e0 / PL * ROW + e0 % 16 / 4 * (ROW / 4) + e0 % PL / 32 * 4;
 }
 template <int HD>
-__device__ __forceinline__ uint32_t v_place(uint32_t slot, uint32_t e0, uint32_t q) {
+__host__ __device__ __forceinline__ constexpr uint32_t v_place(uint32_t slot, uint32_t e0, uint32_t q) {
   constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2;
   return e0 / PL * ROW + (4 * q ^ (PL == 128 ? 4 * (slot >> 1 & 1) : 0)) * (ROW / 8) + e0 % PL / 16;
 }
+
+// These are the layout's own places (kv4.h), for every element.
+template <int HD>
+constexpr bool places_agree() {
+  constexpr int PL = HD < 128 ? HD : 128, ROW = PL / 2;
+  const Kv4Dims d{HD, 64};
+  for (int slot = 0; slot < 4; ++slot)
+    for (int e = 0; e < HD; ++e) {
+      const int behind = ((e / PL) * kKv4Page + slot) * ROW - e / PL * ROW, e0 = e & ~7, j = e & 7;      // planes one behind the other
+      if (d.k_byte(slot, e) - behind != (int)k_place<HD>(e0 & ~16) + j / 4 * (ROW / 4) + j % 4 || d.k_high(e) != ((e0 & 16) != 0)) return false;
+      if (d.v_byte(slot, e) - behind != (int)v_place<HD>(slot, e0, j / 4) + j % 4 * (ROW / 8) || d.v_high(e) != ((e0 & 8) != 0)) return false;
+    }
+  return true;
+}
+static_assert(places_agree<64>() && places_agree<128>() && places_agree<256>(), "the layout of the cache");
 
 // Writes the codes of the warp's rows, those of lane / (HD / 8) = `sub`; `stage` is the warp's own.  Of K a lane has the bytes of whole
 // words (elements 16 apart share a byte, four neighbours a word).  Of V, neighbours lie in different units: the rows are put
@@ -328,13 +343,13 @@ __global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const 
     table_row<VEC>(a.cos, i, ca);
     table_row<VEC>(a.sin, i, sb);
   }
-  auto next = [&]() {                                                // the bodies of an appending kernel's loops stand once: unrolled, they miss the instruction cache
+  auto next = [&]() {                                                // an appending kernel's loops stand once: unrolled, they miss the instruction cache
 #pragma unroll
     for (int i = 0; i + 1 < NP; ++i) raw[i] = raw[i + 1];
   };
-  constexpr int kUnroll = APPEND ? 1 : NP;
   auto normed = [&](auto one, auto&& done) {                          // one: a number of the type that norm and rotation are computed in
     using T = decltype(one);
+    constexpr int kUnroll = APPEND ? 1 : NP;
     T c[kVec], s[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
