@@ -2,7 +2,8 @@
 //
 // A CTA owns 128 query rows of a kv head and a range of keys, walked in tiles of 64.  Codes become fp16 numbers
 // s (c - 8) + (m + 8 s) on the way (the quantiser keeps them inside fp16's range), two roundings of at most 2^-11 of the group's
-// largest (storing a bf16 row costs 2^-8); queries are bf16 numbers times a power of two of their row, exact in fp16.
+// largest (storing a bf16 row costs 2^-8); queries are bf16 numbers times a power of two of
+// their row, exact in fp16 down to 2^-24 of the row's largest.
 //
 //   the others    expand: codes from global memory a tile ahead, K and V rows into swizzled shared memory (two stages each)
 //   warp 8        issues the products: S = Q K^T with Q in tensor memory (read from shared memory it would take half of the
@@ -13,8 +14,10 @@
 // Order of issue: S(j + 1), then O(j), so that the softmax of a tile runs beside the products of its neighbours.
 // Scores of tile j + 1 may overwrite the probabilities of j - 1 when O(j - 1) is complete.
 //
-// What bounds it: shared memory.  Per tile (head size 256) 64 KB of expanded rows are written and read once by the products (1024
-// cycles at 128 B), the products themselves take 1024.
+// What bounds it: issue slots, 60 % busy, most of them the expansion's (every CTA of 128 rows expands its own keys: 64 of them
+// at head size 256 are 32768 codes), beside it shared memory (64 KB a tile written and read once, 1024 cycles, as long as the products
+// take).  Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 113 us = 430 TFLOP/s (26 % of the cuBLAS
+// rate); the scores' factor inside the exponent instead of beside it took 28 us off, K and V by warps of their own 6.
 //
 // A NaN in a group of K or V makes the key's scores NaN, so it spoils the rows that see the key and no others; V's own row is
 // zero then, as is what no row sees.  All waits are bounded; after one that gave up the CTA's threads run to its end without
