@@ -86,6 +86,13 @@ __device__ __forceinline__ void gg_store1(void* p, long long i, int type, float 
   else reinterpret_cast<__half*>(p)[i] = __float2half(v);
 }
 
+// 16 bytes that are read once.  Not .nc: a kernel before may have written them while this one was set up behind its edge.
+__device__ __forceinline__ uint4 gg_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // This lane's part of one block: 16 bytes of each tile, and the scales (and offsets) of its two rows, a word a group.
 template <int GROUP, bool OFF>
 struct GgBlock {
@@ -94,18 +101,18 @@ struct GgBlock {
   uint32_t s[G], o[OFF ? G : 1];
   __device__ __forceinline__ static void words(const uint8_t* p, uint32_t (&d)[G]) {
     if constexpr (G == 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
       d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
     } else if constexpr (G == 2) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
       d[0] = v.x; d[1] = v.y;
     } else {
-      d[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+      d[0] = *reinterpret_cast<const uint32_t*>(p);
     }
   }
   __device__ __forceinline__ void load(const uint8_t* p, int lane) {
-    a = ldg_nc_v4(reinterpret_cast<const uint4*>(p) + lane);
-    b = ldg_nc_v4(reinterpret_cast<const uint4*>(p + 512) + lane);
+    a = gg_stream(reinterpret_cast<const uint4*>(p) + lane);
+    b = gg_stream(reinterpret_cast<const uint4*>(p + 512) + lane);
     words(p + 1024 + (lane >> 2) * 4 * G, s);
     if constexpr (OFF) words(p + 1024 + 32 * G + (lane >> 2) * 4 * G, o);
   }

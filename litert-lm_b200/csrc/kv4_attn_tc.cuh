@@ -116,24 +116,24 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     const long long page_bytes = (long long)a.kv.hkv * d.head_bytes(), head = (long long)kvh * d.head_bytes();
     uint4 raw[2];
     uint32_t ks[2], vs[2];
-    int page_ahead = __ldg(table + t0 * KT / kKv4Page);               // of the next tile to load: its number is a tile ahead of its rows
+    int page_ahead = table[t0 * KT / kKv4Page];               // of the next tile to load: its number is a tile ahead of its rows
     auto load = [&](int j) {
       const int at = (t0 + j) * KT, page = page_ahead, slot = at % kKv4Page + key;
-      if (j + 1 < n) page_ahead = __ldg(table + (at + KT) / kKv4Page);
+      if (j + 1 < n) page_ahead = table[(at + KT) / kKv4Page];
       if (page < 0 || page >= a.kv.num_pages) {
         bad = true;
         return;
       }
       const uint8_t* h = a.kv.pages + page * page_bytes + head;
       const uint8_t* src = h + (has_k ? d.k_codes() : d.v_codes()) + (plane * kKv4Page + slot) * 64 + q * 32;
-      raw[0] = ldg_nc_v4(reinterpret_cast<const uint4*>(src));
-      raw[1] = ldg_nc_v4(reinterpret_cast<const uint4*>(src) + 1);
+      raw[0] = __ldcg(reinterpret_cast<const uint4*>(src));         // not .nc: the kernel before may have written them while this one was set up
+      raw[1] = __ldcg(reinterpret_cast<const uint4*>(src) + 1);
       const uint32_t* kp = reinterpret_cast<const uint32_t*>(h + d.k_scales()) + slot * d.groups() + plane * 128 / GROUP;
       const uint32_t* vp = reinterpret_cast<const uint32_t*>(h + d.v_scales()) + slot * d.groups() + plane * 128 / GROUP;
-      ks[0] = __ldg(kp);
-      vs[0] = __ldg(vp);
-      ks[1] = GROUP == 64 ? __ldg(kp + 1) : ks[0];
-      vs[1] = GROUP == 64 ? __ldg(vp + 1) : vs[0];
+      ks[0] = __ldcg(kp);
+      vs[0] = __ldcg(vp);
+      ks[1] = GROUP == 64 ? __ldcg(kp + 1) : ks[0];
+      vs[1] = GROUP == 64 ? __ldcg(vp + 1) : vs[0];
     };
     raw[0] = raw[1] = make_uint4(0u, 0u, 0u, 0u);
     ks[0] = ks[1] = vs[0] = vs[1] = 0u;

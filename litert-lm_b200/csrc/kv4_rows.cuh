@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const 
 
 // 256 / HD kv heads of a token a warp, K and V of each.
 template <int HD, int TYPE, int GROUP, bool VEC>
-__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const int* __restrict__ seq, const int* __restrict__ pos, int tokens, void* k_out, void* v_out, int* status) {
+__global__ void __launch_bounds__(128) kv4_read_kernel(const Kv4Args kv, const int* seq, const int* pos, int tokens, void* k_out, void* v_out, int* status) {
   constexpr uint32_t PL = HD < 128 ? HD : 128, ROW = PL / 2;
   constexpr int LH = HD / kVec, HP = 32 / LH;
   constexpr Kv4Dims d{HD, GROUP};
