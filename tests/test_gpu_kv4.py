@@ -590,3 +590,54 @@ def test_the_attention_half_of_a_layer(pkg, hidden, hq, hkv, hd):
             assert ((out[b].double() - want).norm() <= 2e-5 * want.norm()).item()
             want = want @ d_out.T
             assert ((y[b].double() - want).norm() <= 4e-5 * want.norm()).item()
+
+
+def test_the_chain_in_a_graph_repeats_bit_for_bit(pkg):
+    """Product -> append -> attention -> product captured once: replays give the bits of the plain calls, step after step, with the
+    tokens' positions, page table and inputs changed in place.  Sums have a fixed order, the joins of shares too."""
+    g, cols, hidden, hq, hkv, hd, group, high = gen(77), 5, 1152, 8, 4, 128, 64, 5000
+    width = (hq + 2 * hkv) * hd
+    images = []
+    for n, k in ((width, hidden), (hidden, hq * hd)):
+        nib = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8).cpu().numpy()
+        scale = (0.01 * torch.rand(n, -(-k // group), device="cuda", generator=g) + 1e-3).half()
+        images.append(torch.from_numpy(pkg.ops.repack_w4_grouped(nib, scale.view(torch.int16).cpu().numpy(), None, group)).cuda())
+    cache = Cache(pkg, cols, 20, hkv, hd, group, fill=0x11)
+    r = Rows(cols, hq, hkv, hd, hd, torch.bfloat16, seed=3, far=high)
+    x = torch.empty(cols, hidden, device="cuda", dtype=torch.bfloat16)
+    out, y = torch.empty(cols, hq * hd, device="cuda", dtype=torch.bfloat16), torch.empty(cols, hidden, device="cuda")
+    kv_len = torch.empty(cols, device="cuda", dtype=torch.int32)
+    need = pkg.ops.attention_kv4_workspace(cols, hkv, hd, hq, 1, high)
+    room = torch.zeros(need, device="cuda", dtype=torch.uint8)
+
+    def chain():
+        pkg.ops.gemv_w4_grouped(images[0].data_ptr(), x.data_ptr(), r.buf.data_ptr(), width, hidden, group, ncols=cols, x_type=1, y_type=1, stream=stream())
+        pkg.ops.qk_norm_rope_append_kv4(cache=cache.c, **{**r.args(), "stream": stream()})
+        pkg.ops.attention_kv4(cache.c, r.q.data_ptr(), 1, hq * hd, kv_len.data_ptr(), 0, cols, 1, high, hq, out.data_ptr(), hq * hd, room.data_ptr(), need, status_dev=r.status.data_ptr(), stream=stream())
+        pkg.ops.gemv_w4_grouped(images[1].data_ptr(), out.data_ptr(), y.data_ptr(), hidden, hq * hd, group, ncols=cols, x_type=1, stream=stream())
+
+    def step(i):
+        torch.manual_seed(i)
+        x.copy_(torch.randn(cols, hidden))
+        r.pos.copy_(torch.tensor([7 + i, 300 + i, 1279 + i, 2600 + i, 4900 + i]))
+        kv_len.copy_(r.pos + 1)
+        torch.cuda.synchronize()
+
+    step(0)
+    chain()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        chain()
+    for i in range(4):
+        step(i)
+        got = []
+        for run in (chain, graph.replay, chain, graph.replay):
+            y.fill_(7.0)
+            run()
+            torch.cuda.synchronize()
+            got.append((y.clone(), out.clone(), cache.pages.clone()))
+        assert torch.isfinite(got[0][0]).all() and (got[0][0] != 7.0).any()
+        for other in got[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    assert pkg.ops.device_status(r.status.data_ptr(), stream()) == 0
