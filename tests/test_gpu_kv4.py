@@ -8,7 +8,8 @@ Tolerances.  u = 2^-24.  A stored value is off by half a step: eps / 2 of it, an
   norm       sum of hd / 32 + 5 adds, a root, a quotient: at most 16 u on the factor, four roundings behind it: 24 u (|a| + |b|)
   cache      codes are decided in 64 bits from values rounded once to 32: equal
   attention  a score is off by dS = 8 u sum |q k| scale + 2^-20 (the exponent's own error, 2^-22, and its argument's rounding among it),
-             a weight by 2 dS and what it is held in, one fp16 term (half a step: 2^-11) for bf16 rows, two (2^-22) else; with the
+             a weight by 2 dS and what it is held in, two fp16 terms (2^-22), or for bf16 rows one,
+             where P, P s and m + 8 s are rounded to fp16 (three times half a step, 2^-11); with the
              sums' own error of 64 u that times the largest |v| bounds the result's.
              Chunks of bf16 rows (head sizes 128 and 256, 16 rows of a kv head and more) may meet K and V as fp16 numbers
              s (c - 8) + (m + 8 s), two roundings of at most 2^-11 of the largest |k| or |v| each.  The roundings of a key's elements
@@ -352,7 +353,7 @@ class Attention:
             p = torch.where(seen, torch.softmax(x.masked_fill(~seen, -math.inf), -1), 0.0) if n else x
             want = torch.einsum("hgts,shd->thgd", p, v)
             d = 8 * U * (size.amax() if n else 0) + 2.0 ** -20
-            held_in = 2.0 ** -11 if self.typ == torch.bfloat16 else 2.0 ** -22
+            held_in = 3 * 2.0 ** -11 if self.typ == torch.bfloat16 else 2.0 ** -22
             if self.typ == torch.bfloat16 and hd >= 128 and self.max_q * (hq // hkv) >= 16 and n:
                 d = d + 6 * 2.0 ** -10 * k.abs().amax() * q.norm(dim=-1).amax() * used
                 held_in += 2.0 ** -10
