@@ -257,9 +257,9 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
 #pragma unroll
     for (int i = 0; i < S::NOFF; ++i) off[c][i] = 0.f;
   }
-  // keys that every row sees, so that tiles within them need no mask
+  // keys that every row sees, so that tiles within them need no mask (rows that the tile does not have are zeros, and never leave)
   const int seen0 = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  const int open1 = rows == RB ? first + 1 : 0, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
+  const int open1 = first + 1, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
 
   auto add = [](float (&acc)[4], const uint32_t (&x)[4], const uint32_t (&y)[2]) {
     if constexpr (!EXACT) {

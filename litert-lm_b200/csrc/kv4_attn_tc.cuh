@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    // keys that every row of the tile sees
-    const int open1 = rows == kKcRows ? first + 1 : 0, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
+    // keys that every row of the tile sees (rows that it does not have are zeros, and never leave)
+    const int open1 = first + 1, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
     float mz = 0.f;
     bool late = false;
 #pragma unroll 1
