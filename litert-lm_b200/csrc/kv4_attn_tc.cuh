@@ -16,7 +16,7 @@
 //
 // What bounds it: issue slots, 60 % busy, most of them the expansion's (every CTA of 128 rows expands its own keys: 64 of them
 // at head size 256 are 32768 codes), beside it shared memory (64 KB a tile written and read once, 1024 cycles, as long as the products
-// take).  Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 113 us = 430 TFLOP/s (26 % of the cuBLAS
+// take).  Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 110 us = 445 TFLOP/s (27 % of the cuBLAS
 // rate); the scores' factor inside the exponent instead of beside it took 28 us off, K and V by warps of their own 6.
 //
 // A NaN in a group of K or V makes the key's scores NaN, so it spoils the rows that see the key and no others; V's own row is

@@ -119,3 +119,17 @@ def test_error_strings_may_be_declined(pkg):
     assert lib.B200LmOps_DeviceStatus(0, None, None, None, None) == 3
     n = C.c_int64(7)
     assert lib.B200LmOps_Kv4PageBytes(1, 96, 64, C.byref(n), None) == 12 and n.value == 7
+
+
+def test_arguments_of_the_extension_module(pkg):
+    """What is not a whole number, or does not fit its type, is refused before the library sees it."""
+    ok = dict(w_dev=P, x_dev=P, y_dev=P, n=64, k=256, group=64)
+    with pytest.raises(TypeError):
+        pkg.ops.gemv_w4_grouped(**{**ok, "w_dev": 1.5})
+    with pytest.raises(TypeError):
+        pkg.ops.gemv_w4_grouped(**{**ok, "x_dev": None})
+    with pytest.raises(OverflowError):
+        pkg.ops.gemv_w4_grouped(**{**ok, "group": 1 << 40})
+    with pytest.raises(OverflowError):
+        pkg.ops.gemv_w4_grouped(**{**ok, "n": 1 << 70})
+    assert "null" in refused(pkg, 3, pkg.ops.gemv_w4_grouped, **{**ok, "w_dev": np.int64(0)})
