@@ -141,6 +141,11 @@ __global__ void __launch_bounds__(kGgThreads, 2) gemv_grouped_kernel(const GgArg
   const int rank = blockIdx.x % a.cs, first = blockIdx.x / a.cs * a.run, strips = min(a.run, a.strips - first);
   const int rs = kGgWarps / a.kw, ks = warp / rs;                                              // strips at a time, this warp's share
   const int b0 = (int)((long long)a.blocks * rank / a.cs), b1 = (int)((long long)a.blocks * (rank + 1) / a.cs);
+  // the first weights into L2 while the kernel before ends (L2 is where it would write them, so nothing stale can come of it)
+  if (warp % rs < strips && lane * 128 < min(b1 - b0, AH) * S::kBlock) {
+    const uint8_t* p = a.w + ((long long)(first + warp % rs) * a.blocks + b0) * S::kBlock + lane * 128;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+  }
   pdl_wait();
   pdl_launch_dependents();
 
