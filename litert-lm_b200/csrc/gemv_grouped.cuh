@@ -17,8 +17,8 @@
 // distributed shared memory: no workspace, a fixed order.  Where a run has fewer strips than warps, kw warps share the blocks
 // of a strip.
 //
-// Measured: 262144 x 1152, groups of 128, two fp32 columns 29.4 us = 5.4 TB/s (83 % of the copy rate), bound by HBM; 20480 x 2560,
-// groups of 64 with offsets, three columns 12.4 us = 2.4 TB/s, bound by one chain of latencies (digits, first blocks, the cluster's
+// Measured: 262144 x 1152, groups of 128, two fp32 columns 29.0 us = 5.4 TB/s (84 % of the copy rate), bound by HBM; 20480 x 2560,
+// groups of 64 with offsets, three columns 12.3 us = 2.4 TB/s, bound by one chain of latencies (digits, first blocks, the cluster's
 // meeting) and the last round of strips; 1536 x 1152, one column 3.3 us, a launch.
 #pragma once
 #include <cuda_fp16.h>
