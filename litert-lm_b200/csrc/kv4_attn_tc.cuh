@@ -24,6 +24,7 @@
 // the products, and the status says so.
 #pragma once
 #include "kv4_attn.cuh"
+#include "kv4_chunk_order.h"
 #include "prefill_gemm_ts.cuh"
 #include "prefill_ops.cuh"
 #include "attn_tc.cuh"
@@ -61,9 +62,10 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
   extern __shared__ __align__(1024) unsigned char kc_sm[];
   float* row_x = reinterpret_cast<float*>(kc_sm + S::kMax);          // [half][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(kc_sm + S::kBars);
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6, *s_full = bars + 8, *p_full = bars + 10, *o_full = bars + 12, *q_ready = bars + 13;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
-  int* gave_up = reinterpret_cast<int*>(bars + 15);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kKcBars);
+  int* gave_up = reinterpret_cast<int*>(bars + kKcBars + 1);
+  auto wait = [&](KcWait w) { return mbar_wait(bars + w.bar, w.parity(), gave_up); };
+  auto wait2 = [&](KcWait w, KcWait x) { return mbar_wait2(bars + w.bar, w.parity(), bars + x.bar, x.parity(), gave_up); };
   __shared__ int last_s;
   const int warp = warp_index(), lane = threadIdx.x & 31;
   pdl_wait();
@@ -86,15 +88,16 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], P * 128);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], P * 128);
-      mbar_init(&v_empty[s], 1);
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 8);
+      mbar_init(&bars[kKcKFull + s], P * 128);
+      mbar_init(&bars[kKcKEmpty + s], 1);
+      mbar_init(&bars[kKcVFull + s], P * 128);
+      mbar_init(&bars[kKcVEmpty + s], 1);
+      mbar_init(&bars[kKcSFull + s], 1);
+      mbar_init(&bars[kKcPFull + s], 8);
     }
-    mbar_init(o_full, 1);
-    mbar_init(q_ready, 8);
+    mbar_init(&bars[kKcOFull], 1);
+    mbar_init(&bars[kKcQReady], 8);
+    mbar_init(&bars[kKcODone], 1);
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     auto nan = [](uint32_t u) { return (u & 0x7C00u) == 0x7C00u; };
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
-      const int st = j & 1, use = j >> 1;
+      const int st = j & 1;
       const uint32_t word[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
       uint32_t k2[2] = {ks[0], ks[1]}, v2[2] = {vs[0], vs[1]};
       if (j + 1 < n) load(j + 1);
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
         if (nan(v2[0])) v2[0] = 0u;
         if (nan(v2[1])) v2[1] = 0u;
       }
-      if (use > 0) ok = ok && mbar_wait(has_k ? &k_empty[st] : &v_empty[st], (use - 1) & 1, gave_up);
+      if (j >= 2) ok = ok && wait(kc_empty(has_k ? kKcKEmpty : kKcVEmpty, j));
       if (has_k && ok) {
         unsigned char* line = kc_sm + st * S::kTile + key * 128;
         __half2 s, mid;
@@ -199,7 +202,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
         }
       }
       fence_async_smem();
-      mbar_arrive(has_k ? &k_full[st] : &v_full[st]);
+      mbar_arrive(&bars[(has_k ? kKcKFull : kKcVFull) + st]);
       ok = __all_sync(0xffffffffu, ok);
     }
   } else if (n > 0 && warp == 8) {
@@ -212,10 +215,10 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i)
         umma_bf16_ts(tmem + S::kS + (j & 1) * KT, tmem + S::kQ + i * 8, umma_desc_sw128(k + i / 4 * KT * 128) + (uint64_t)(i % 4 * 2), idesc_s, i > 0);
-      umma_commit(&s_full[j & 1]);
-      umma_commit(&k_empty[j & 1]);
+      umma_commit(&bars[kc_stage(kKcSFull, j)]);
+      umma_commit(&bars[kc_stage(kKcKEmpty, j)]);
     };
-    ok = __all_sync(0xffffffffu, mbar_wait2(q_ready, 0, &k_full[0], 0, gave_up));
+    ok = __all_sync(0xffffffffu, wait2({kKcQReady, 0}, kc_full(kKcKFull, 0)));
     if (ok) {
       tc_fence_after();
       if (leader) scores(0);
@@ -224,13 +227,13 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
 #pragma unroll 1
     for (int j = 0; j < n && ok; ++j) {
       if (j + 1 < n) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, gave_up) && (j == 0 || mbar_wait(o_full, (j - 1) & 1, gave_up)));
+        ok = __all_sync(0xffffffffu, wait(kc_full(kKcKFull, j + 1)) && (j == 0 || wait(kc_o(j - 1))));
         if (!ok) break;
         tc_fence_after();
         if (leader) scores(j + 1);
         __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, mbar_wait2(&v_full[j & 1], (j >> 1) & 1, &p_full[j & 1], (j >> 1) & 1, gave_up));
+      ok = __all_sync(0xffffffffu, wait2(kc_full(kKcVFull, j), kc_full(kKcPFull, j)));
       if (!ok) break;
       tc_fence_after();
       if (leader) {
@@ -238,8 +241,9 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
           umma_bf16_ts(tmem + S::kO, tmem + S::kS + (j & 1) * KT + k * 8, atc_desc_mn(v + k * 2048, KT * 128), idesc_o, j > 0 || k > 0);
-        umma_commit(o_full);
-        umma_commit(&v_empty[j & 1]);
+        umma_commit(&bars[kKcOFull]);
+        umma_commit(&bars[kc_stage(kKcVEmpty, j)]);
+        if (j + 1 == n) umma_commit(&bars[kKcODone]);
       }
       __syncwarp();
     }
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
+      if (lane == 0) mbar_arrive(&bars[kKcQReady]);
     }
     // keys that every row of the tile sees (rows that it does not have are zeros, and never leave)
     const int open1 = first + 1, open0 = a.window > 0 ? max(0, lastp - a.window + 1) : 0;
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int base = (t0 + j) * KT, mykeys = base + half * HK;
-      const bool got = __all_sync(0xffffffffu, mbar_wait(&s_full[j & 1], (j >> 1) & 1, gave_up)) && !late;
+      const bool got = __all_sync(0xffffffffu, wait(kc_full(kKcSFull, j))) && !late;
       float s[HK], mx = -INFINITY;
       if (got) {
         tc_fence_after();
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
         mz = mn == -INFINITY ? 0.f : mn;
         l *= f;
         if (j > 0) {
-          late = !__all_sync(0xffffffffu, mbar_wait(o_full, (j - 1) & 1, gave_up));
+          late = !__all_sync(0xffffffffu, wait(kc_o(j - 1)));
           if (!late && __any_sync(0xffffffffu, f != 1.f)) {
             tc_fence_after();
 #pragma unroll
@@ -355,9 +359,9 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[j & 1]);
+      if (lane == 0) mbar_arrive(&bars[kc_stage(kKcPFull, j)]);
     }
-    ok = ok && !late && __all_sync(0xffffffffu, mbar_wait(o_full, (n - 1) & 1, gave_up));
+    ok = ok && !late && __all_sync(0xffffffffu, wait(kc_end()));
     tc_fence_after();
   }
   // ---- row sums meet; O out of tensor memory
