@@ -7,10 +7,10 @@
 //   S  int8 products (m16n8k32, unsigned codes): a row of q is cut into four digits of seven bits below its largest power of
 //      two (of three bits and three times seven where the codes enter as 16 c: upper nibbles are masked, not shifted), the eight
 //      columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
-//   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in fp16 terms: two for fp16 and fp32 rows (2^-22
-//      of each weight), one for bf16 rows, where P, P s and m + 8 s are fp16 numbers (3 * 2^-11 in all, storing the row costs 2^-8)
-//      and the second sum is a product too.  P s is held in a power of two below
-//      fp16's range: its reference is the largest scale that the warp has met, so small weights are off by 2^-31 of that.
+//   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in two fp16 terms (2^-22 of each weight).  One
+//      term, with P and m + 8 s as fp16 numbers too, took 5.6 us off the 93 of 64 bf16 sequences and put 3 * 2^-11 on each weight:
+//      one bf16 result in ten came out a step off.  P s is held in a power of two
+//      below fp16's range: its reference is the largest scale that the warp has met, so small weights are off by 2^-31 of that.
 //      Two nibbles of a half word come out of a mask each (1024 + c and 1024 + 16 c) and a fused product makes them c - 8; as
 //      bf16 numbers they would need a shift each, and the logic pipe, half as wide as the others, is what bounds this kernel.
 //      Codes centred at zero keep the sums small; the tensor core cuts its sums off, so fp32 rows take them out after every
@@ -25,8 +25,8 @@
 // keys a share has is decided on the host from the largest length, how many shares a sequence has on the device from its own.
 //
 // What bounds it: issue slots (63 to 67 % busy with 16 warps an SM) and the logic pipe (52 %), not the bytes.  64 sequences of 300 ..
-// 8192 positions, 8 query heads on 4 of 256, bf16: 87.4 us = 3.6 TB/s; three of 40001 .. 65536, 32 on 16 of 128, fp32: 91.4 us =
-// 3.8 TB/s; 16 x 5 rows in a window of 1024: 28.5 us; one sequence of 777 positions: 9.5 us, a chain of latencies with the join.
+// 8192 positions, 8 query heads on 4 of 256, bf16: 93.0 us = 3.4 TB/s; three of 40001 .. 65536, 32 on 16 of 128, fp32: 90.9 us =
+// 3.8 TB/s; 16 x 5 rows in a window of 1024: 28.2 us; one sequence of 777 positions: 9.5 us, a chain of latencies with the join.
 // Tiles of 16 keys at head size 256 because two CTAs an SM leave 14 KB of ring a warp: three stages.
 #pragma once
 #include "kv4_rows.cuh"
@@ -54,15 +54,13 @@ constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps;
 constexpr int kKaTickets = 4096;          // words at the start of a workspace
 constexpr int kKaStages = 3;
 
-// TV terms of P s.
-template <int HD, int GROUP, int RB, int TV>
+template <int HD, int GROUP, int RB>
 struct KaShape {
   static constexpr int PL = HD < 128 ? HD : 128, P = HD / PL;        // plane, planes
   static constexpr int ROW = PL / 2, NG = HD / GROUP;
   static constexpr int NB = RB / 2;                                  // column blocks of S: two rows of four digits
-  static constexpr int CV = RB * TV, NBV = (CV + 7) / 8;             // columns of O, blocks of them
+  static constexpr int CV = RB * 2, NBV = (CV + 7) / 8;              // columns of O (two terms of P s a row), blocks of them
   static constexpr int kCtas = HD / 16 * NBV * 4 > 64 ? 1 : 2;       // of an SM: O takes up to half of a thread's registers, or more
-  static constexpr int NOFF = TV == 2 ? NG : 4;                      // a lane's sums of P (m + 8 s): by group, or a product's accumulator
   static constexpr int KT = HD == 256 ? 16 : 32, SUB = KT / 16, MT = HD / 16;
   static constexpr int kCodes = KT * HD / 2, kScales = KT * NG * 4, kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kKaWarps * kKaStages * kStage;
@@ -71,7 +69,7 @@ struct KaShape {
   static constexpr int kMergeO = kKaWarps * RB * HD * 4, kMergeOff = kKaWarps * RB * NG * 4;
   static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 + RB * 8 <= kRing, "the exchange fits over the ring");
   static_assert(RB * KT * 4 <= kCodes, "P of a tile fits over its K codes");
-  static constexpr float kLazy = TV == 1 ? 4.f : 8.f;                // powers of two by which a score may pass its row's reference
+  static constexpr float kLazy = 8.f;                                // powers of two by which a score may pass its row's reference
   static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
 };
 
@@ -119,9 +117,9 @@ __device__ __forceinline__ void ka_words(const unsigned char* p, uint32_t (&d)[N
   }
 }
 
-template <int HD, int GROUP, int RB, int TV, bool EXACT>
-__global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a) {
-  using S = KaShape<HD, GROUP, RB, TV>;
+template <int HD, int GROUP, int RB, bool EXACT>
+__global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a) {
+  using S = KaShape<HD, GROUP, RB>;
   constexpr int NG = S::NG, NB = S::NB, NBV = S::NBV, KT = S::KT, SUB = S::SUB, W4 = S::PL / 32;
   extern __shared__ __align__(128) unsigned char ka_sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -249,13 +247,13 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
   }
   float wk = 1.f;                                                    // P s is held times this power of two
   uint32_t limit = 1;                                                // and this scale (fp16 bits) is past it
-  float o[S::MT][NBV][4], off[NBV][S::NOFF];
+  float o[S::MT][NBV][4], off[NBV][NG];                              // off: this lane's sums of P (m + 8 s)
 #pragma unroll
   for (int c = 0; c < NBV; ++c) {
 #pragma unroll
     for (int i = 0; i < S::MT; ++i) o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.f;
 #pragma unroll
-    for (int i = 0; i < S::NOFF; ++i) off[c][i] = 0.f;
+    for (int i = 0; i < NG; ++i) off[c][i] = 0.f;
   }
   // keys that every row sees, so that tiles within them need no mask (rows that the tile does not have are zeros, and never leave)
   const int seen0 = a.window > 0 ? max(0, first - a.window + 1) : 0;
@@ -275,36 +273,16 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
   auto products = [&](const unsigned char* st) {
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-      float w[NBV][4];                                               // P in fp32, or
-      uint32_t p2[NBV][2];                                           // in fp16, pairs of keys
+      float w[NBV][4];
 #pragma unroll
       for (int c = 0; c < NBV; ++c) {
-        const int r = (c * 8 + g) / TV, at = (r < RB ? r : 0) * KT + u * 16 + 4 * t;
-        if constexpr (TV == 2) {
-          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(st) + at);
-          w[c][0] = v.x; w[c][1] = v.y; w[c][2] = v.z; w[c][3] = v.w;
-        } else {
-          ka_words<2>(st + at * 2, p2[c]);
-        }
+        const int r = c * 4 + g / 2;
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(st) + (r < RB ? r : 0) * KT + u * 16 + 4 * t);
+        w[c][0] = v.x; w[c][1] = v.y; w[c][2] = v.z; w[c][3] = v.w;
       }
       uint32_t vs[4][NG];
 #pragma unroll
       for (int i = 0; i < 4; ++i) ka_words<NG>(st + 2 * S::kCodes + S::kScales + (u * 16 + t + 4 * i) * NG * 4, vs[i]);
-      if constexpr (TV == 1) {
-        // sum of P (m + 8 s) over the keys, a product with the groups as its rows
-        const __half2 eight = __float2half2_rn(8.f);
-        uint32_t x[4] = {0u, 0u, 0u, 0u}, word[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word[i] = *reinterpret_cast<const uint32_t*>(st + 2 * S::kCodes + S::kScales + ((u * 16 + t + 4 * i) * NG + g % NG) * 4);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t s2 = __byte_perm(word[2 * i], word[2 * i + 1], 0x5410), m2 = __byte_perm(word[2 * i], word[2 * i + 1], 0x7632);
-          const __half2 mid = __hfma2(*reinterpret_cast<const __half2*>(&s2), eight, *reinterpret_cast<const __half2*>(&m2));
-          if (g < NG) x[2 * i] = *reinterpret_cast<const uint32_t*>(&mid);
-        }
-#pragma unroll
-        for (int c = 0; c < NBV; ++c) ka_mma_o(off[c], x, p2[c][0], p2[c][1]);
-      }
       uint32_t bt[NBV][2];
 #pragma unroll
       for (int pl = 0; pl < S::P; ++pl) {
@@ -319,40 +297,28 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
         for (int j = 0; j < WU; ++j) {                               // 64 dims
           const int dim = pl * S::PL + j * 64, grp = dim / GROUP;
           if (dim % GROUP == 0) {
-            if constexpr (TV == 1) {
+            float sc[4], mn[4];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t s2 = __byte_perm(vs[2 * i][grp], vs[2 * i + 1][grp], 0x5410);
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vs[i][grp]));
+              sc[i] = f.x;
+              mn[i] = fmaf(8.f, f.x, f.y);
+            }
 #pragma unroll
-                for (int c = 0; c < NBV; ++c) {
-                  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&p2[c][i]), *reinterpret_cast<const __half2*>(&s2));
-                  bt[c][i] = *reinterpret_cast<const uint32_t*>(&x);
-                }
-              }
-            } else {
-              float sc[4], mn[4];
+            for (int c = 0; c < NBV; ++c) {
+              float x[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vs[i][grp]));
-                sc[i] = f.x;
-                mn[i] = fmaf(8.f, f.x, f.y);
+                x[i] = w[c][i] * sc[i];
+                off[c][grp] = fmaf(w[c][i], mn[i], off[c][grp]);
               }
-#pragma unroll
-              for (int c = 0; c < NBV; ++c) {
-                float x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  x[i] = w[c][i] * sc[i];
-                  off[c][grp] = fmaf(w[c][i], mn[i], off[c][grp]);
-                }
-                uint32_t b0 = ka_pack(x[0], x[1]), b1 = ka_pack(x[2], x[3]);
-                // what the first term left, in the odd columns
-                const float2 y0 = ka_unpack(b0), y1 = ka_unpack(b1);
-                const uint32_t n0 = ka_pack(x[0] - y0.x, x[1] - y0.y), n1 = ka_pack(x[2] - y1.x, x[3] - y1.y);
-                if (g & 1) { b0 = n0; b1 = n1; }
-                bt[c][0] = b0;
-                bt[c][1] = b1;
-              }
+              uint32_t b0 = ka_pack(x[0], x[1]), b1 = ka_pack(x[2], x[3]);
+              // what the first term left, in the odd columns
+              const float2 y0 = ka_unpack(b0), y1 = ka_unpack(b1);
+              const uint32_t n0 = ka_pack(x[0] - y0.x, x[1] - y0.y), n1 = ka_pack(x[2] - y1.x, x[3] - y1.y);
+              if (g & 1) { b0 = n0; b1 = n1; }
+              bt[c][0] = b0;
+              bt[c][1] = b1;
             }
           }
 #pragma unroll
@@ -483,8 +449,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       largest = __reduce_max_sync(0xffffffffu, largest);
       if (largest >= limit) {                                        // largest 2^k in [2^6, 2^7): with P <= 2^8 within fp16's range
         const float top = __half2float(__ushort_as_half((unsigned short)largest));
-        // one term: P itself is an fp16 number, P <= 2^4 and k <= 11
-        const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = TV == 1 ? fminf(64.f / power, 2048.f) : 64.f / power;
+        const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = 64.f / power;
         fk = k / wk;
         wk = k;
         limit = power >= 32768.f ? 0x7C00u : (uint32_t)__half_as_ushort(__float2half_rn(2.f * power));
@@ -514,11 +479,11 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
       };
 #pragma unroll
       for (int c = 0; c < NBV; ++c) {
-        const float f0 = of_row((c * 8 + 2 * t) / TV), f1 = of_row((c * 8 + 2 * t + 1) / TV), fo = of_row((c * 8 + g) / TV);
+        const float fr = of_row(c * 4 + t), fo = of_row(c * 4 + g / 2);      // of this lane's columns 2 t and 2 t + 1, and of column g
 #pragma unroll
-        for (int i = 0; i < S::MT; ++i) { o[i][c][0] *= f0; o[i][c][1] *= f1; o[i][c][2] *= f0; o[i][c][3] *= f1; }
+        for (int i = 0; i < S::MT; ++i) { o[i][c][0] *= fr; o[i][c][1] *= fr; o[i][c][2] *= fr; o[i][c][3] *= fr; }
 #pragma unroll
-        for (int i = 0; i < S::NOFF; ++i) off[c][i] *= TV == 2 ? fo : i == 0 ? f0 : f1;
+        for (int i = 0; i < NG; ++i) off[c][i] *= fo;
       }
     }
     // ---- P in the order of the keys in O's products: key t + 4 i of a block of 16 at 4 t + i.  It lies over the K codes.
@@ -530,9 +495,7 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
         const float x = ka_ex2(p[u][nb] - mz[nb]);
         l[nb] += x;
         const int key = g + 8 * (t & 1);
-        const int at = (2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4;
-        if constexpr (TV == 2) reinterpret_cast<float*>(st)[at] = x * wk;
-        else reinterpret_cast<__half*>(st)[at] = __float2half_rn(x * wk);
+        reinterpret_cast<float*>(st)[(2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4] = x * wk;
       }
     __syncwarp();
 
@@ -558,31 +521,19 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB, TV>::kCtas)
   }
 #pragma unroll
   for (int c = 0; c < NBV; ++c) {
-    if constexpr (TV == 2) {
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        float x = off[c][i];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        if (t == 0 && (c * 8 + g) % TV == 0 && c * 8 + g < S::CV) moff[(warp * RB + (c * 8 + g) / TV) * NG + i] = x * back;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)                                    // group g, rows 2 t and 2 t + 1
-        if (g < NG && 2 * t + i < RB) moff[(warp * RB + 2 * t + i) * NG + g] = off[c][i] * back;
+    for (int i = 0; i < NG; ++i) {
+      float x = off[c][i];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      if (t == 0 && !(g & 1) && c * 8 + g < S::CV) moff[(warp * RB + c * 4 + g / 2) * NG + i] = x * back;
     }
 #pragma unroll
     for (int i = 0; i < S::MT; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int dim = i * 16 + h * 8 + g;
-        if constexpr (TV == 2) {                                     // the two terms of row 4 c + t
-          if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + dim] = (o[i][c][2 * h] + o[i][c][2 * h + 1]) * back;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (2 * t + k < RB) mo[(warp * RB + 2 * t + k) * HD + dim] = o[i][c][2 * h + k] * back;
-        }
+        // the two terms of row 4 c + t
+        if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + i * 16 + h * 8 + g] = (o[i][c][2 * h] + o[i][c][2 * h + 1]) * back;
       }
   }
   __syncthreads();

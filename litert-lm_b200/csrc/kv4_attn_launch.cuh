@@ -4,18 +4,17 @@
 
 namespace b200lm {
 
-template <int HD, int GROUP, int RB, int TV, bool EXACT>
+template <int HD, int GROUP, int RB, bool EXACT>
 void launch_kv4_attn_as(cudaStream_t st, const Kv4AttnArgs& a) {
-  using S = KaShape<HD, GROUP, RB, TV>;
-  raise_dyn_smem(kv4_attn_kernel<HD, GROUP, RB, TV, EXACT>, S::kSmem);
-  launch_pdl(kv4_attn_kernel<HD, GROUP, RB, TV, EXACT>, dim3((unsigned)(a.row_tiles * a.splits * a.kv.hkv), (unsigned)a.kv.batch), dim3(kKaThreads), S::kSmem, st, a);
+  using S = KaShape<HD, GROUP, RB>;
+  raise_dyn_smem(kv4_attn_kernel<HD, GROUP, RB, EXACT>, S::kSmem);
+  launch_pdl(kv4_attn_kernel<HD, GROUP, RB, EXACT>, dim3((unsigned)(a.row_tiles * a.splits * a.kv.hkv), (unsigned)a.kv.batch), dim3(kKaThreads), S::kSmem, st, a);
 }
 
 template <int HD, int GROUP, int RB>
 void launch_kv4_attn_terms(cudaStream_t st, const Kv4AttnArgs& a) {
-  if (a.q_type == kF32) launch_kv4_attn_as<HD, GROUP, RB, 2, true>(st, a);
-  else if (a.q_type == kF16) launch_kv4_attn_as<HD, GROUP, RB, 2, false>(st, a);
-  else launch_kv4_attn_as<HD, GROUP, RB, 1, false>(st, a);
+  if (a.q_type == kF32) launch_kv4_attn_as<HD, GROUP, RB, true>(st, a);
+  else launch_kv4_attn_as<HD, GROUP, RB, false>(st, a);
 }
 
 template <int HD, int GROUP>
