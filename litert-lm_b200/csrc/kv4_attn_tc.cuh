@@ -1,23 +1,28 @@
 // Attention over the cache in 4 bits for many bf16 query rows of a kv head (a prompt's chunk), on the 5th-generation tensor cores.
 //
-// A CTA owns 128 query rows of a kv head and a range of keys, walked in tiles of 64.  Codes become fp16 numbers
-// s (c - 8) + (m + 8 s) on the way (the quantiser keeps them inside fp16's range), two roundings of at most 2^-11 of the group's
-// largest (storing a bf16 row costs 2^-8); queries are bf16 numbers times a power of two of
-// their row, exact in fp16 down to 2^-24 of the row's largest.
+// A CTA owns 128 query rows of a kv head and a range of keys, walked in tiles of 64.
+//   S / 2  s (c - 8) / 2 as two fp16 numbers, each exact: s is cut into its upper seven bits and the four below, and c - 8 has four.
+//          What the offsets bring, sum over the groups of (m / 2 + 4 s) (sum of q), is one more product of 16: m / 2 and 4 s beside the
+//          sums of q over 64 elements, in two terms (2^-22).  (The halves keep 8 s inside fp16's range.)  Queries are bf16 numbers
+//          times a power of two of their row, exact in fp16 down to 2^-24 of the row's largest.  So a score is as good as
+//          fp32; with K as one fp16 number a score of 50 was off by percents of its key's weight.
+//   O      P and V = s c + m as fp16 numbers, one rounding of 2^-11 each, where storing the bf16 row costs 2^-8 (V in two terms and P in
+//          two would be three products instead of one, and the rows of V would not fit beside those of K).
 //
 //   the others    expand: codes from global memory a tile ahead, K and V rows into swizzled shared memory (two stages each)
-//   warp 8        issues the products: S = Q K^T with Q in tensor memory (read from shared memory it would take half of the
-//                 bandwidth that the expanded rows need), O += P V with P in tensor memory, over the scores it was made from
+//   warp 8        issues the products: S = Q K^T with Q in tensor memory (read from shared memory it would take a third of the
+//                 bandwidth that the expanded rows need; the sums of q do come from there), O += P V with P in tensor memory, over the scores it was made from
 //   warps 0 - 7   softmax, two threads a row (half of the keys, half of O each).  A row's reference moves when a score passes it
 //                 by 8 powers of two; only then is O read, scaled and written back, behind the products of the tile before.
 //
 // Order of issue: S(j + 1), then O(j), so that the softmax of a tile runs beside the products of its neighbours.
 // Scores of tile j + 1 may overwrite the probabilities of j - 1 when O(j - 1) is complete.
 //
-// What bounds it: issue slots, 60 % busy, most of them the expansion's (every CTA of 128 rows expands its own keys: 64 of them
-// at head size 256 are 32768 codes), beside it shared memory (64 KB a tile written and read once, 1024 cycles, as long as the products
-// take).  Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 110 us = 445 TFLOP/s (27 % of the cuBLAS
-// rate); the scores' factor inside the exponent instead of beside it took 28 us off, K and V by warps of their own 6.
+// What bounds it: issue slots, most of them the expansion's (every CTA of 128 rows expands its own keys: 64 of them at head size 256
+// are 32768 codes), beside it shared memory (96 KB a tile written and read once, 1536 cycles, as long as the products take).
+// Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 147 us = 333 TFLOP/s (20 % of the cuBLAS
+// rate; 108 us with K in one term), the same of head size 128: 75 us (68); the scores' factor inside the exponent instead of
+// beside it took 28 us off, K and V by warps of their own 6.
 //
 // A NaN in a group of K or V makes the key's scores NaN, so it spoils the rows that see the key and no others; V's own row is
 // zero then, as is what no row sees.  All waits are bounded; after one that gave up the CTA's threads run to its end without
@@ -37,8 +42,11 @@ template <int HD>
 struct KcShape {
   static constexpr int KT = 64;                                      // keys of a tile
   static constexpr int kThreads = kKcSoft + 32 + HD * 2;             // 4 warps for K, 4 for V of every 128 elements
-  static constexpr int kTile = KT * HD * 2;                          // K or V of a tile
-  static constexpr int kMax = 4 * kTile;                             // [2][128] floats
+  static constexpr int kTile = KT * HD * 2;                          // V of a tile, or one term of K
+  static constexpr int kV = 4 * kTile;                               // two stages of K, then of V
+  static constexpr int kLine = 128;                                  // bytes of an operand's row of 64
+  static constexpr int kKx = kV + 2 * kTile, kQx = kKx + 2 * KT * kLine;       // offsets of K (two stages) and sums of q: rows of 16 numbers
+  static constexpr int kMax = kQx + kKcRows * kLine;                 // [2][128] floats
   static constexpr int kBars = kMax + 2 * 128 * 4;
   static constexpr int kSmem = kBars + 256;
   static constexpr uint32_t kO = 0, kQ = HD, kS = HD + HD / 2;       // tensor memory columns; P of a tile over its scores
@@ -46,11 +54,23 @@ struct KcShape {
 };
 __host__ __device__ constexpr uint32_t kc_idesc(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }      // fp16 x fp16 -> fp32
 
-// Two neighbouring codes (nibbles of two bytes, `low` or high) as values.
+// Two neighbouring codes (nibbles of two bytes, `low` or high) as fp16 numbers (c - 8) / 2, or as V's values.
 template <int p>
-__device__ __forceinline__ uint32_t kc_values(uint32_t x, __half2 s, __half2 mid) {
-  const uint32_t c = ka_codes<p>(x);
-  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c), s, mid);
+__device__ __forceinline__ __half2 kc_centred(uint32_t x) {
+  const uint32_t y = (x & (p ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;       // 1024 + c, or 1024 + 16 c
+  const __half2 h = *reinterpret_cast<const __half2*>(&y);
+  return p ? __hfma2(h, __float2half2_rn(1.f / 32), __float2half2_rn(-36.f)) : __hfma2(h, __float2half2_rn(0.5f), __float2half2_rn(-516.f));
+}
+template <int p>
+__device__ __forceinline__ uint32_t kc_values(uint32_t x, __half2 s, __half2 m) {
+  const uint32_t y = (x & (p ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+  const __half2 h = *reinterpret_cast<const __half2*>(&y);
+  const __half2 c = p ? __hfma2(h, __float2half2_rn(1.f / 16), __float2half2_rn(-64.f)) : __hadd2(h, __float2half2_rn(-1024.f));
+  const __half2 v = __hfma2(c, s, m);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t kc_product(__half2 a, __half2 b) {
+  const __half2 v = __hmul2(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
@@ -60,6 +80,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
   constexpr int KT = S::KT, P = HD / 128, HK = KT / 2;
   constexpr Kv4Dims d{HD, GROUP};
   extern __shared__ __align__(1024) unsigned char kc_sm[];
+  unsigned char *kx = kc_sm + S::kKx, *qx = kc_sm + S::kQx;
   float* row_x = reinterpret_cast<float*>(kc_sm + S::kMax);          // [half][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(kc_sm + S::kBars);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kKcBars);
@@ -101,6 +122,8 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  for (int i = threadIdx.x; i < (S::kMax - S::kKx) / 16; i += S::kThreads) reinterpret_cast<uint4*>(kx)[i] = make_uint4(0u, 0u, 0u, 0u);      // places of 64 that a head does not have
+  fence_async_smem();
   if (warp == 8) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -141,11 +164,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     raw[0] = raw[1] = make_uint4(0u, 0u, 0u, 0u);
     ks[0] = ks[1] = vs[0] = vs[1] = 0u;
     load(0);
-    auto pair = [](uint32_t u, __half2& s, __half2& mid) {
-      const __half2 x = *reinterpret_cast<const __half2*>(&u);
-      s = __half2half2(__low2half(x));
-      mid = __half2half2(__hfma(__low2half(x), __float2half(8.f), __high2half(x)));
-    };
+    auto both = [](uint32_t half) { return __half2half2(__ushort_as_half((unsigned short)half)); };
     auto nan = [](uint32_t u) { return (u & 0x7C00u) == 0x7C00u; };
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
@@ -162,17 +181,35 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       }
       if (j >= 2) ok = ok && wait(kc_empty(has_k ? kKcKEmpty : kKcVEmpty, j));
       if (has_k && ok) {
-        unsigned char* line = kc_sm + st * S::kTile + key * 128;
-        __half2 s, mid;
+        unsigned char* line = kc_sm + st * 2 * S::kTile + key * S::kLine;
+        __half2 hi, lo;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                                // 32 elements: 8 q .. and 16 more, of the words 2 q and 2 q + 1
-          if (i == 0 || (GROUP == 64 && i == 2)) pair(k2[i / 2], s, mid);
-          const uint32_t x0 = __byte_perm(word[i], 0, 0x4140), x1 = __byte_perm(word[i], 0, 0x4342), x2 = __byte_perm(word[4 + i], 0, 0x4140), x3 = __byte_perm(word[4 + i], 0, 0x4342);
-          unsigned char* at = line + (plane * 2 + i / 2) * KT * 128;
+          if (i == 0 || (GROUP == 64 && i == 2)) {
+            hi = both(k2[i / 2] & 0xFFF0u);
+            lo = __hsub2(both(k2[i / 2]), hi);                       // NaN stays NaN
+          }
+          const uint32_t x[4] = {__byte_perm(word[i], 0, 0x4140), __byte_perm(word[i], 0, 0x4342), __byte_perm(word[4 + i], 0, 0x4140), __byte_perm(word[4 + i], 0, 0x4342)};
+          unsigned char* at = line + (plane * 2 + i / 2) * KT * S::kLine;
           const int c = 4 * (i & 1) + q;
-          *reinterpret_cast<uint4*>(at + ((c ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
-          *reinterpret_cast<uint4*>(at + (((c + 2) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
+          __half2 v[4];
+          auto put = [&](int where) {
+            unsigned char* to = at + ((where ^ (key & 7)) << 4);
+            *reinterpret_cast<uint4*>(to) = make_uint4(kc_product(v[0], hi), kc_product(v[1], hi), kc_product(v[2], hi), kc_product(v[3], hi));
+            *reinterpret_cast<uint4*>(to + S::kTile) = make_uint4(kc_product(v[0], lo), kc_product(v[1], lo), kc_product(v[2], lo), kc_product(v[3], lo));
+          };
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = kc_centred<0>(x[k]);
+          put(c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = kc_centred<1>(x[k]);
+          put(c + 2);
         }
+        // m / 2 of the blocks of 64 elements, then 4 s: beside the first term of the sums (q = 0) and beside the second
+        unsigned char* offsets = kx + st * KT * S::kLine + key * S::kLine + ((q ^ (key & 7)) << 4) + plane * 4;
+        const uint32_t s2 = __byte_perm(k2[0], k2[1], 0x5410), m2 = __byte_perm(k2[0], k2[1], 0x7632);
+        *reinterpret_cast<uint32_t*>(offsets) = kc_product(*reinterpret_cast<const __half2*>(&m2), __float2half2_rn(0.5f));
+        *reinterpret_cast<uint32_t*>(offsets + 8) = kc_product(*reinterpret_cast<const __half2*>(&s2), __float2half2_rn(4.f));
       }
       // V: this thread has two words of four units; it wants word q of all eight, the partner (lane ^ 16) the other words
       if (!has_k) {
@@ -182,22 +219,21 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
           mine[i] = q ? word[2 * i + 1] : word[2 * i];
           got[i] = __shfl_xor_sync(0xffffffffu, q ? word[2 * i] : word[2 * i + 1], 16);
         }
-        const bool low = q == (slot >> 1 & 1);                         // the units that it has are the first four
+        const bool front = q == (slot >> 1 & 1);                         // the units that it has are the first four
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          unit[i] = low ? mine[i] : got[i];
-          unit[4 + i] = low ? got[i] : mine[i];
+          unit[i] = front ? mine[i] : got[i];
+          unit[4 + i] = front ? got[i] : mine[i];
         }
         if (ok) {
-          unsigned char* line = kc_sm + (2 + st) * S::kTile + (plane * 2 + q) * KT * 128 + key * 128;
-          __half2 s, mid;
-          pair(v2[GROUP == 64 ? q : 0], s, mid);
+          unsigned char* line = kc_sm + S::kV + st * S::kTile + (plane * 2 + q) * KT * S::kLine + key * S::kLine;
+          const __half2 s = both(v2[GROUP == 64 ? q : 0] & 0xFFFFu), low = both(v2[GROUP == 64 ? q : 0] >> 16);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {                                // byte i of the words: 16 neighbours
             const uint32_t sel = i | (4 + i) << 8;
             const uint32_t x0 = __byte_perm(unit[0], unit[1], sel), x1 = __byte_perm(unit[2], unit[3], sel), x2 = __byte_perm(unit[4], unit[5], sel), x3 = __byte_perm(unit[6], unit[7], sel);
-            *reinterpret_cast<uint4*>(line + (((2 * i) ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, mid), kc_values<0>(x1, s, mid), kc_values<0>(x2, s, mid), kc_values<0>(x3, s, mid));
-            *reinterpret_cast<uint4*>(line + (((2 * i + 1) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, mid), kc_values<1>(x1, s, mid), kc_values<1>(x2, s, mid), kc_values<1>(x3, s, mid));
+            *reinterpret_cast<uint4*>(line + (((2 * i) ^ (key & 7)) << 4)) = make_uint4(kc_values<0>(x0, s, low), kc_values<0>(x1, s, low), kc_values<0>(x2, s, low), kc_values<0>(x3, s, low));
+            *reinterpret_cast<uint4*>(line + (((2 * i + 1) ^ (key & 7)) << 4)) = make_uint4(kc_values<1>(x0, s, low), kc_values<1>(x1, s, low), kc_values<1>(x2, s, low), kc_values<1>(x3, s, low));
           }
         }
       }
@@ -211,10 +247,13 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     const bool leader = elect_one();
     const uint32_t ring = smem_u32(kc_sm);
     auto scores = [&](int j) {
-      const uint32_t k = ring + (j & 1) * S::kTile;
+      const uint32_t k = ring + (j & 1) * 2 * S::kTile, to = tmem + S::kS + (j & 1) * KT;
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
-        umma_bf16_ts(tmem + S::kS + (j & 1) * KT, tmem + S::kQ + i * 8, umma_desc_sw128(k + i / 4 * KT * 128) + (uint64_t)(i % 4 * 2), idesc_s, i > 0);
+      for (int term = 0; term < 2; ++term)
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i)
+          umma_bf16_ts(to, tmem + S::kQ + i * 8, umma_desc_sw128(k + term * S::kTile + i / 4 * KT * S::kLine) + (uint64_t)(i % 4 * 2), idesc_s, term > 0 || i > 0);
+      umma_bf16(to, umma_desc_sw128(smem_u32(qx)), umma_desc_sw128(smem_u32(kx) + (j & 1) * KT * S::kLine), idesc_s, 1);
       umma_commit(&bars[kc_stage(kKcSFull, j)]);
       umma_commit(&bars[kc_stage(kKcKEmpty, j)]);
     };
@@ -237,10 +276,10 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       if (!ok) break;
       tc_fence_after();
       if (leader) {
-        const uint32_t v = ring + (2 + (j & 1)) * S::kTile;
+        const uint32_t v = ring + S::kV + (j & 1) * S::kTile;
 #pragma unroll
         for (int k = 0; k < KT / 16; ++k)
-          umma_bf16_ts(tmem + S::kO, tmem + S::kS + (j & 1) * KT + k * 8, atc_desc_mn(v + k * 2048, KT * 128), idesc_o, j > 0 || k > 0);
+          umma_bf16_ts(tmem + S::kO, tmem + S::kS + (j & 1) * KT + k * 8, atc_desc_mn(v + k * 2048, KT * S::kLine), idesc_o, j > 0 || k > 0);
         umma_commit(&bars[kKcOFull]);
         umma_commit(&bars[kc_stage(kKcVEmpty, j)]);
         if (j + 1 == n) umma_commit(&bars[kKcODone]);
@@ -275,7 +314,8 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       const int e = max((int)(bits >> 23), 30);
       const bool spoilt = bits >= 0x7F800000u;
       const float f = spoilt ? 0.f : __uint_as_float((uint32_t)(254 + 7 - e) << 23);             // largest |q| f in [2^7, 2^8)
-      unit = spoilt ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 7) << 23) * a.qscale;
+      unit = spoilt ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 6) << 23) * a.qscale;       // of S / 2
+      float sum = 0.f;
 #pragma unroll 1
       for (int i = 0; i < V; i += 32) {                              // the second time from the cache
         uint32_t y[16];
@@ -284,10 +324,21 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
           float x[8];
           get(i + k, x);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) y[k / 2 + c] = spoilt ? 0u : ka_pack(x[2 * c] * f, x[2 * c + 1] * f);
+          for (int c = 0; c < 4; ++c) {
+            y[k / 2 + c] = spoilt ? 0u : ka_pack(x[2 * c] * f, x[2 * c + 1] * f);
+            sum += spoilt ? 0.f : x[2 * c] * f + x[2 * c + 1] * f;
+          }
         }
         tmem_st16(lane_addr + S::kQ + half * (HD / 4) + i / 2, y);
+        if (i % 64 == 32) {                                          // below 2^14: a block's sum in two terms, each beside m / 2 and beside 4 s
+          const __half t0 = __float2half_rn(sum), t1 = __float2half_rn(sum - __half2float(t0));
+          unsigned char* line = qx + row * S::kLine + (half * V + i) / 64 * 2;
+          *reinterpret_cast<__half*>(line + ((row & 7) << 4)) = *reinterpret_cast<__half*>(line + ((row & 7) << 4) + 8) = t0;
+          *reinterpret_cast<__half*>(line + ((1 ^ (row & 7)) << 4)) = *reinterpret_cast<__half*>(line + ((1 ^ (row & 7)) << 4) + 8) = t1;
+          sum = 0.f;
+        }
       }
+      fence_async_smem();
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();

@@ -176,14 +176,14 @@ static Kv4Plan plan_attention(int batch, int hkv, int hd, int hq, int max_q, int
   return p;
 }
 
-// Which of the two a call takes, by what they would cost in us.  Fitted to 2 .. 1024 rows over 2048 and 4096 keys of 1, 16 and 64
-// sequences: mma.sync grows with rows x keys (64 sequences x 4 kv heads x 16 rows x 4096 keys of 256: 243 us, 32 rows 434),
-// the tensor-core kernel with tiles of 128 rows (261 and 263, and 25 us at the least, where four rows over 4096 keys take 11).
+// Which of the two a call takes, by what they would cost in us.  Fitted to 16 .. 64 rows over 2048 and 4096 keys of 1, 16 and 64
+// sequences: mma.sync grows with rows x keys (64 sequences x 4 kv heads x 16 rows x 4096 keys of 256: 289 us, 32 rows 565),
+// the tensor-core kernel with tiles of 128 rows (265 and 268, and 26 us at the least, where 16 rows over 2048 keys take 13).
 static bool chunk_pays(const Kv4Plan& few, const Kv4Plan& many, int hd, int max_kv, int window, int max_q, int sms) {
   const double keys = window > 0 ? std::min<double>(max_kv, (double)window + max_q) : max_kv;
   const double simple = 8 + 0.25e-6 * (double)few.units * keys * hd;
   const double tiles = (double)((many.units * many.splits + sms - 1) / sms) * many.share / 64;
-  return 20 + tiles * (hd == 256 ? 1.45 : 0.8) < simple;
+  return 20 + tiles * (hd == 256 ? 1.85 : 0.9) < simple;
 }
 
 }  // namespace b200lm

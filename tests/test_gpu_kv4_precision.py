@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv4 import Attention
+from test_gpu_kv4 import U, Attention, gen, put
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,40 @@ def test_16_bit_rows_are_rounded_once(pkg, hq, hkv, hd, group, typ, share):
             other += (a.out[at, :want.shape[1]] != want.to(typ)).sum().item()
             total += want.numel()
         assert other <= share * total, (other, total)
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", [(8, 4, 256, 64), (8, 4, 256, 128), (8, 4, 128, 64), (16, 2, 128, 128)])
+@pytest.mark.parametrize("how", ["one dim", "offsets"])
+def test_large_scores_of_chunks(pkg, hq, hkv, hd, group, how):
+    """Chunks of bf16 rows where one dim carries a score of 50, or where all keys lie far from zero: a score that is off by a share of
+    itself is off by percents of its key's weight.  Per row, as in test_gpu_kv4_chunks.py: storing costs 2^-8 |o|; ahead of that P is
+    rounded once (2^-11 / sqrt(3) of itself), V once, and a score is off by 2^-20 sum |q k| scale (its sums and its exponent's)."""
+    lens, counts = [900, 600, 2500], [600, 599, 200]
+    a = Attention(pkg, lens, counts, hq, hkv, hd, group, torch.bfloat16, seed=hd + group)
+    q = a.q[:, :hq * hd].view(-1, hq, hd)
+    if how == "one dim":
+        q[..., 0] = 6 * hd ** 0.5
+    seq = torch.cat([torch.full((n,), b, dtype=torch.int32) for b, n in enumerate(lens)]).cuda()
+    pos = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]).cuda()
+    k, v = (torch.randn(len(seq), hkv, hd, device="cuda", generator=gen(s)) for s in (1, 2))
+    if how == "one dim":
+        k[..., 0] = 8 + 0.5 * k[..., 0]
+    else:
+        k += 40
+    a.k, a.v = (x.split(lens) for x in put(pkg, a.cache, seq, pos, k, v))
+    a()
+    assert pkg.ops.device_status(a.status.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    for b, (n, count) in enumerate(zip(lens, counts)):
+        at = slice(int(a.start[b]), int(a.start[b]) + count)
+        got = a.out[at, :hq * hd].double().view(count, hq, hd)
+        seen = torch.arange(n, device="cuda")[None] <= torch.arange(n - count, n, device="cuda")[:, None]
+        for h in range(hq):
+            qh, kh, vh = q[at, h].double(), a.k[b][:, h // (hq // hkv)].double(), a.v[b][:, h // (hq // hkv)].double()
+            p = torch.softmax((qh @ kh.T * hd ** -0.5).masked_fill(~seen, -math.inf), -1)
+            o, p2 = p @ vh, p * p
+            tau = 2.0 ** -11 * vh.abs().amax() / 3 ** 0.5
+            sigma = torch.sqrt((2.0 ** -20 * (qh.abs() @ kh.abs().T).amax(-1) * hd ** -0.5) ** 2 + (2.0 ** -11) ** 2 / 3)
+            gap = p2 @ vh.square().sum(-1) - 2 * ((p2 @ vh) * o).sum(-1) + p2.sum(-1) * o.square().sum(-1)
+            inner = 6 * torch.sqrt(sigma ** 2 * gap.clamp(min=0) + hd * tau ** 2 * p2.sum(-1)) + 64 * U * vh.abs().amax() * hd ** 0.5
+            err = (got[:, h] - o).norm(dim=-1)
+            assert (err <= 2.0 ** -8 * (o.norm(dim=-1) + inner) + inner).all(), (b, h, (err / o.norm(dim=-1)).max().item())
