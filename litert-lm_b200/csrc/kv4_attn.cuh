@@ -60,7 +60,6 @@ struct KaShape {
   static constexpr int ROW = PL / 2, NG = HD / GROUP;
   static constexpr int NB = RB / 2;                                  // column blocks of S: two rows of four digits
   static constexpr int CV = RB * 2, NBV = (CV + 7) / 8;              // columns of O (two terms of P s a row), blocks of them
-  static constexpr int kCtas = HD / 16 * NBV * 4 > 64 ? 1 : 2;       // of an SM: O takes up to half of a thread's registers, or more
   static constexpr int KT = HD == 256 ? 16 : 32, SUB = KT / 16, MT = HD / 16;
   static constexpr int kCodes = KT * HD / 2, kScales = KT * NG * 4, kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kKaWarps * kKaStages * kStage;
@@ -118,7 +117,7 @@ __device__ __forceinline__ void ka_words(const unsigned char* p, uint32_t (&d)[N
 }
 
 template <int HD, int GROUP, int RB, bool EXACT>
-__global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB>::kCtas) kv4_attn_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnArgs a) {
   using S = KaShape<HD, GROUP, RB>;
   constexpr int NG = S::NG, NB = S::NB, NBV = S::NBV, KT = S::KT, SUB = S::SUB, W4 = S::PL / 32;
   extern __shared__ __align__(128) unsigned char ka_sm[];
@@ -635,9 +634,9 @@ __global__ void __launch_bounds__(kKaThreads, KaShape<HD, GROUP, RB>::kCtas) kv4
   }
 }
 
-// Rows of a CTA for `rows` query rows of a kv head: the fewest that hold them, and four at head size 256, where O of eight in two
-// terms would not fit the registers and eight in one term cost more than twice four (64 x 8 rows over 4096 keys: 149 us against
-// 141, with 216 bytes of spills).
-constexpr int ka_rows(int hd, long long rows) { return rows <= 2 ? 2 : rows <= 4 || hd == 256 ? 4 : 8; }
+// Rows of a CTA for `rows` query rows of a kv head: the fewest that hold them, eight at head size 64 only.  O of eight in two terms
+// does not fit the registers at 256, and at 128 takes 300 to 480 bytes of spills: 32 x 8 rows over 2000 .. 4096 keys of four kv
+// heads 51.1 us against 47.4 with twice four (fp32 52.6 and 48.4, groups of 128 48.1 and 44.1; five rows 51.0 and 47.2).
+constexpr int ka_rows(int hd, long long rows) { return rows <= 2 ? 2 : rows <= 4 || hd >= 128 ? 4 : 8; }
 
 }  // namespace b200lm

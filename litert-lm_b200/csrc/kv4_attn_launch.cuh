@@ -21,7 +21,7 @@ template <int HD, int GROUP>
 void launch_kv4_attn_rows(cudaStream_t st, const Kv4AttnArgs& a, int rb) {
   if (rb == 2) launch_kv4_attn_terms<HD, GROUP, 2>(st, a);
   else if (rb == 4) launch_kv4_attn_terms<HD, GROUP, 4>(st, a);
-  else if constexpr (HD < 256) launch_kv4_attn_terms<HD, GROUP, 8>(st, a);
+  else if constexpr (HD < 128) launch_kv4_attn_terms<HD, GROUP, 8>(st, a);
 }
 
 template <int HD>

@@ -183,7 +183,7 @@ static bool chunk_pays(const Kv4Plan& few, const Kv4Plan& many, int hd, int max_
   const double keys = window > 0 ? std::min<double>(max_kv, (double)window + max_q) : max_kv;
   const double simple = 8 + 0.25e-6 * (double)few.units * keys * hd;
   const double tiles = (double)((many.units * many.splits + sms - 1) / sms) * many.share / 64;
-  return 20 + tiles * (hd == 256 ? 1.85 : 0.9) < simple;
+  return (hd == 256 ? 20 + 1.85 * tiles : 14 + 0.9 * tiles) < simple;
 }
 
 }  // namespace b200lm
