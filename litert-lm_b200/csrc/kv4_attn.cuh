@@ -68,6 +68,7 @@ struct KaShape {
   static constexpr int kMergeO = kKaWarps * RB * HD * 4, kMergeOff = kKaWarps * RB * NG * 4;
   static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 + RB * 8 <= kRing, "the exchange fits over the ring");
   static_assert(RB * KT * 4 <= kCodes, "P of a tile fits over its K codes");
+  static_assert(RB * NG <= 32, "a bit for each row and group");
   static constexpr float kLazy = 8.f;                                // powers of two by which a score may pass its row's reference
   static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
 };
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
   using S = KaShape<HD, GROUP, RB>;
   constexpr int NG = S::NG, NB = S::NB, NBV = S::NBV, KT = S::KT, SUB = S::SUB, W4 = S::PL / 32;
   extern __shared__ __align__(128) unsigned char ka_sm[];
+  __shared__ unsigned poison_s;                                      // bit r NG + g: row r sees a NaN in group g of V
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
   pdl_launch_dependents();
@@ -140,6 +142,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
   if (split >= nsplit) return;
   const int t0 = (key0 + split * a.share) / KT, t1 = (min(key1, key0 + (split + 1) * a.share) + KT - 1) / KT;
 
+  if (threadIdx.x == 0) poison_s = 0u;
   // ---- this warp's ring
   unsigned char* ring = ka_sm + warp * (kKaStages * S::kStage);
   const Kv4Dims d{HD, GROUP};
@@ -347,24 +350,27 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
     if (++slot == kKaStages) slot = 0;
     const bool edge = tl * KT < open0 || tl * KT + KT > open1;
 
-    // ---- V's scales: the largest; in tiles that not every row sees whole, what no row sees may hold anything (zeros do no harm), and a
-    // NaN that some see moves into the key's scores, where the rows that do not see it are masked
+    // ---- V's scales: the largest; a NaN spoils its group's sums by itself where every row sees it.  In tiles that not every row sees
+    // whole it is taken out and noted for the rows that do; what no row sees may hold anything (zeros do no harm)
     uint32_t largest = 0;
     {
       constexpr int WL = KT * NG / 32;                               // every scale of V once in the warp
-      uint32_t* scales = reinterpret_cast<uint32_t*>(st + 2 * S::kCodes);        // of K, then of V
+      uint32_t* scales = reinterpret_cast<uint32_t*>(st + 2 * S::kCodes + S::kScales);
       uint32_t w[WL];
-      ka_words<WL>(st + 2 * S::kCodes + S::kScales + lane * WL * 4, w);
+      ka_words<WL>(reinterpret_cast<const unsigned char*>(scales) + lane * WL * 4, w);
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
         uint32_t x = w[i] & 0xFFFFu;
         if (edge) {
-          const int j = (lane * WL + i) / NG, key = tl * KT + j;
+          const int key = tl * KT + (lane * WL + i) / NG;
           const bool seen = key >= seen0 && key < key1;
-          if (!seen || x >= 0x7C00u) {
-            if (seen) scales[j * NG] = 0x7E007E00u;
-            scales[KT * NG + lane * WL + i] = x = 0u;
+          if (seen && x >= 0x7C00u) {
+            for (int r = 0; r < rows; ++r) {
+              const int at = len - nq + (r0 + r) / G;
+              if (key <= at && (a.window <= 0 || key > at - a.window)) atomicOr(&poison_s, 1u << (r * NG + (lane * WL + i) % NG));
+            }
           }
+          if (!seen || x >= 0x7C00u) scales[lane * WL + i] = x = 0u;
         }
         if (x < 0x7C00u) largest = max(largest, x);
       }
@@ -578,6 +584,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
       const float4 x = *reinterpret_cast<const float4*>(mo + (w * RB + r) * HD + dim);
       v[0] = fmaf(f, x.x + add_all, v[0]); v[1] = fmaf(f, x.y + add_all, v[1]); v[2] = fmaf(f, x.z + add_all, v[2]); v[3] = fmaf(f, x.w + add_all, v[3]);
     }
+    if (poison_s >> (r * NG + dim / GROUP) & 1u) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
     if (nsplit > 1) *reinterpret_cast<float4*>(rec + r * HD + dim) = make_float4(v[0], v[1], v[2], v[3]);
     else if (r < rows && !spoilt) store(r, dim, v, total[2 * r + 1]);
   }

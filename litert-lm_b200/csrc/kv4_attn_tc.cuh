@@ -20,12 +20,12 @@
 //
 // What bounds it: issue slots, most of them the expansion's (every CTA of 128 rows expands its own keys: 64 of them at head size 256
 // are 32768 codes), beside it shared memory (96 KB a tile written and read once, 1536 cycles, as long as the products take).
-// Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 147 us = 333 TFLOP/s (20 % of the cuBLAS
-// rate; 108 us with K in one term), the same of head size 128: 75 us (68); the scores' factor inside the exponent instead of
+// Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 131 us = 374 TFLOP/s (23 % of the cuBLAS
+// rate; 108 us with K in one term), the same of head size 128: 73 us (68); the scores' factor inside the exponent instead of
 // beside it took 28 us off, K and V by warps of their own 6.
 //
-// A NaN in a group of K or V makes the key's scores NaN, so it spoils the rows that see the key and no others; V's own row is
-// zero then, as is what no row sees.  All waits are bounded; after one that gave up the CTA's threads run to its end without
+// A NaN in a group of K makes the key's scores NaN, so it spoils the rows that see the key and no others.  One of V is noted for
+// those rows, whose dims of the group become NaN at the end; V itself is zero there, as is what no row sees.  All waits are bounded; after one that gave up the CTA's threads run to its end without
 // the products, and the status says so.
 #pragma once
 #include "kv4_attn.cuh"
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
   auto wait = [&](KcWait w) { return mbar_wait(bars + w.bar, w.parity(), gave_up); };
   auto wait2 = [&](KcWait w, KcWait x) { return mbar_wait2(bars + w.bar, w.parity(), bars + x.bar, x.parity(), gave_up); };
   __shared__ int last_s;
+  __shared__ unsigned poison[kKcRows];                               // bit i: the row sees a NaN among the elements 64 i .. of V
   const int warp = warp_index(), lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int i = threadIdx.x; i < (S::kMax - S::kKx) / 16; i += S::kThreads) reinterpret_cast<uint4*>(kx)[i] = make_uint4(0u, 0u, 0u, 0u);      // places of 64 that a head does not have
+  if (threadIdx.x < kKcRows) poison[threadIdx.x] = 0u;
   fence_async_smem();
   if (warp == 8) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
@@ -141,7 +143,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     const int* table = a.kv.table + b * a.kv.table_stride;
     const long long page_bytes = (long long)a.kv.hkv * d.head_bytes(), head = (long long)kvh * d.head_bytes();
     uint4 raw[2];
-    uint32_t ks[2], vs[2];
+    uint32_t sm[2];                                           // (s, m) of K or V, for each 64 of the plane's elements
     int page_ahead = table[t0 * KT / kKv4Page];               // of the next tile to load: its number is a tile ahead of its rows
     auto load = [&](int j) {
       const int at = (t0 + j) * KT, page = page_ahead, slot = at % kKv4Page + key;
@@ -154,31 +156,22 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       const uint8_t* src = h + (has_k ? d.k_codes() : d.v_codes()) + (plane * kKv4Page + slot) * 64 + q * 32;
       raw[0] = __ldcg(reinterpret_cast<const uint4*>(src));         // not .nc: the kernel before may have written them while this one was set up
       raw[1] = __ldcg(reinterpret_cast<const uint4*>(src) + 1);
-      const uint32_t* kp = reinterpret_cast<const uint32_t*>(h + d.k_scales()) + slot * d.groups() + plane * 128 / GROUP;
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>(h + d.v_scales()) + slot * d.groups() + plane * 128 / GROUP;
-      ks[0] = __ldcg(kp);
-      vs[0] = __ldcg(vp);
-      ks[1] = GROUP == 64 ? __ldcg(kp + 1) : ks[0];
-      vs[1] = GROUP == 64 ? __ldcg(vp + 1) : vs[0];
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(h + (has_k ? d.k_scales() : d.v_scales())) + slot * d.groups() + plane * 128 / GROUP;
+      sm[0] = __ldcg(p);
+      sm[1] = GROUP == 64 ? __ldcg(p + 1) : sm[0];
     };
     raw[0] = raw[1] = make_uint4(0u, 0u, 0u, 0u);
-    ks[0] = ks[1] = vs[0] = vs[1] = 0u;
+    sm[0] = sm[1] = 0u;
     load(0);
     auto both = [](uint32_t half) { return __half2half2(__ushort_as_half((unsigned short)half)); };
-    auto nan = [](uint32_t u) { return (u & 0x7C00u) == 0x7C00u; };
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int st = j & 1;
       const uint32_t word[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-      uint32_t k2[2] = {ks[0], ks[1]}, v2[2] = {vs[0], vs[1]};
+      uint32_t now[2] = {sm[0], sm[1]};
       if (j + 1 < n) load(j + 1);
       const int slot = (t0 + j) * KT % kKv4Page + key, where = (t0 + j) * KT + key;
-      if (where < seen0 || where >= key1) v2[0] = v2[1] = 0u, k2[0] = k2[1] = 0u;    // what no row sees: zeros
-      else if (nan(v2[0]) || nan(v2[1])) {
-        k2[0] = 0x7E007E00u;
-        if (nan(v2[0])) v2[0] = 0u;
-        if (nan(v2[1])) v2[1] = 0u;
-      }
+      if (where < seen0 || where >= key1) now[0] = now[1] = 0u;      // what no row sees: zeros
       if (j >= 2) ok = ok && wait(kc_empty(has_k ? kKcKEmpty : kKcVEmpty, j));
       if (has_k && ok) {
         unsigned char* line = kc_sm + st * 2 * S::kTile + key * S::kLine;
@@ -186,8 +179,8 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                                // 32 elements: 8 q .. and 16 more, of the words 2 q and 2 q + 1
           if (i == 0 || (GROUP == 64 && i == 2)) {
-            hi = both(k2[i / 2] & 0xFFF0u);
-            lo = __hsub2(both(k2[i / 2]), hi);                       // NaN stays NaN
+            hi = both(now[i / 2] & 0xFFF0u);
+            lo = __hsub2(both(now[i / 2]), hi);                       // NaN stays NaN
           }
           const uint32_t x[4] = {__byte_perm(word[i], 0, 0x4140), __byte_perm(word[i], 0, 0x4342), __byte_perm(word[4 + i], 0, 0x4140), __byte_perm(word[4 + i], 0, 0x4342)};
           unsigned char* at = line + (plane * 2 + i / 2) * KT * S::kLine;
@@ -207,7 +200,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
         }
         // m / 2 of the blocks of 64 elements, then 4 s: beside the first term of the sums (q = 0) and beside the second
         unsigned char* offsets = kx + st * KT * S::kLine + key * S::kLine + ((q ^ (key & 7)) << 4) + plane * 4;
-        const uint32_t s2 = __byte_perm(k2[0], k2[1], 0x5410), m2 = __byte_perm(k2[0], k2[1], 0x7632);
+        const uint32_t s2 = __byte_perm(now[0], now[1], 0x5410), m2 = __byte_perm(now[0], now[1], 0x7632);
         *reinterpret_cast<uint32_t*>(offsets) = kc_product(*reinterpret_cast<const __half2*>(&m2), __float2half2_rn(0.5f));
         *reinterpret_cast<uint32_t*>(offsets + 8) = kc_product(*reinterpret_cast<const __half2*>(&s2), __float2half2_rn(4.f));
       }
@@ -227,7 +220,15 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
         }
         if (ok) {
           unsigned char* line = kc_sm + S::kV + st * S::kTile + (plane * 2 + q) * KT * S::kLine + key * S::kLine;
-          const __half2 s = both(v2[GROUP == 64 ? q : 0] & 0xFFFFu), low = both(v2[GROUP == 64 ? q : 0] >> 16);
+          uint32_t pair = q ? now[1] : now[0];
+          if ((pair & 0x7C00u) == 0x7C00u) {
+            for (int r = 0; r < rows; ++r) {
+              const int at = len - nq + (r0 + r) / G;
+              if (where <= at && (a.window <= 0 || where > at - a.window)) atomicOr(&poison[r], 1u << (plane * 2 + q));
+            }
+            pair = 0u;
+          }
+          const __half2 s = both(pair & 0xFFFFu), low = both(pair >> 16);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {                                // byte i of the words: 16 neighbours
             const uint32_t sel = i | (4 + i) << 8;
@@ -433,6 +434,10 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = 0u;
+      }
+      if (poison[row] >> ((half * (HD / 2) + c) / 64) & 1u) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = 0x7FC00000u;
       }
       if (row < rows && nsplit > 1) {
 #pragma unroll
