@@ -9,8 +9,8 @@
 //      columns are four digits of two rows, the sums are exact integers and enter fp32 once a group.
 //   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in two fp16 terms (2^-22 of each weight).  One
 //      term, with P and m + 8 s as fp16 numbers too, took 5.6 us off the 93 of 64 bf16 sequences and put 3 * 2^-11 on each weight:
-//      one bf16 result in ten came out a step off.  P s is held in a power of two
-//      below fp16's range: its reference is the largest scale that the warp has met, so small weights are off by 2^-31 of that.
+//      one bf16 result in ten came out a step off.  P s is held in a power of two below fp16's range, one for each group of
+//      dims: its reference is the largest scale of the group that the warp has met, so small weights are off by 2^-31 of that.
 //      Two nibbles of a half word come out of a mask each (1024 + c and 1024 + 16 c) and a fused product makes them c - 8; as
 //      bf16 numbers they would need a shift each, and the logic pipe, half as wide as the others, is what bounds this kernel.
 //      Codes centred at zero keep the sums small; the tensor core cuts its sums off, so fp32 rows take them out after every
@@ -25,8 +25,8 @@
 // keys a share has is decided on the host from the largest length, how many shares a sequence has on the device from its own.
 //
 // What bounds it: issue slots (63 to 67 % busy with 16 warps an SM) and the logic pipe (52 %), not the bytes.  64 sequences of 300 ..
-// 8192 positions, 8 query heads on 4 of 256, bf16: 93.0 us = 3.4 TB/s; three of 40001 .. 65536, 32 on 16 of 128, fp32: 90.9 us =
-// 3.8 TB/s; 16 x 5 rows in a window of 1024: 28.2 us; one sequence of 777 positions: 9.5 us, a chain of latencies with the join.
+// 8192 positions, 8 query heads on 4 of 256, bf16: 97.5 us = 3.2 TB/s; three of 40001 .. 65536, 32 on 16 of 128, fp32: 92.9 us =
+// 3.7 TB/s; 16 x 5 rows in a window of 1024: 28.7 us; one sequence of 777 positions: 10.0 us, a chain of latencies with the join.
 // Tiles of 16 keys at head size 256 because two CTAs an SM leave 14 KB of ring a warp: three stages.
 #pragma once
 #include "kv4_rows.cuh"
@@ -247,8 +247,13 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
     m[nb] = -INFINITY;
     mz[nb] = l[nb] = 0.f;
   }
-  float wk = 1.f;                                                    // P s is held times this power of two
-  uint32_t limit = 1;                                                // and this scale (fp16 bits) is past it
+  constexpr int WL = KT * NG / 32;                                   // scales of V of a tile that a lane looks at, of groups (lane WL + i) % NG
+  float wk[NG];                                                      // P s is held times this power of two: at first any scale is past it
+  uint32_t limit[WL];                                                // and scales (fp16 bits) from this one on are
+#pragma unroll
+  for (int i = 0; i < NG; ++i) wk[i] = 1099511627776.f;
+#pragma unroll
+  for (int i = 0; i < WL; ++i) limit[i] = 1u;
   float o[S::MT][NBV][4], off[NBV][NG];                              // off: this lane's sums of P (m + 8 s)
 #pragma unroll
   for (int c = 0; c < NBV; ++c) {
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vs[i][grp]));
-              sc[i] = f.x;
+              sc[i] = f.x * wk[grp];
               mn[i] = fmaf(8.f, f.x, f.y);
             }
 #pragma unroll
@@ -352,15 +357,15 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
 
     // ---- V's scales: the largest; a NaN spoils its group's sums by itself where every row sees it.  In tiles that not every row sees
     // whole it is taken out and noted for the rows that do; what no row sees may hold anything (zeros do no harm)
-    uint32_t largest = 0;
+    bool over = false;
+    uint32_t w[WL];                                                  // every scale of V once in the warp
     {
-      constexpr int WL = KT * NG / 32;                               // every scale of V once in the warp
       uint32_t* scales = reinterpret_cast<uint32_t*>(st + 2 * S::kCodes + S::kScales);
-      uint32_t w[WL];
       ka_words<WL>(reinterpret_cast<const unsigned char*>(scales) + lane * WL * 4, w);
 #pragma unroll
       for (int i = 0; i < WL; ++i) {
-        uint32_t x = w[i] & 0xFFFFu;
+        uint32_t& x = w[i];
+        x &= 0xFFFFu;
         if (edge) {
           const int key = tl * KT + (lane * WL + i) / NG;
           const bool seen = key >= seen0 && key < key1;
@@ -372,11 +377,11 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
           }
           if (!seen || x >= 0x7C00u) scales[lane * WL + i] = x = 0u;
         }
-        if (x < 0x7C00u) largest = max(largest, x);
+        if (x >= 0x7C00u) x = 0u;
+        over = over || x >= limit[i];
       }
       if (edge) __syncwarp();
     }
-    bool over = largest >= limit;
 
     // ---- S: lane (g, t) gathers the digit pair t & 1 of row 2 nb + (t >> 1) for the keys g and g + 8
     float s[SUB][NB][2], smin[SUB][NB];
@@ -450,14 +455,23 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
         over = over || x > m[nb] + S::kLazy;
       }
     if (__any_sync(0xffffffffu, over)) {
-      float f[NB], fk = 1.f;
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      if (largest >= limit) {                                        // largest 2^k in [2^6, 2^7): with P <= 2^8 within fp16's range
-        const float top = __half2float(__ushort_as_half((unsigned short)largest));
-        const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = 64.f / power;
-        fk = k / wk;
-        wk = k;
-        limit = power >= 32768.f ? 0x7C00u : (uint32_t)__half_as_ushort(__float2half_rn(2.f * power));
+      float f[NB], fk[NG];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        uint32_t largest = 0;
+#pragma unroll
+        for (int j = 0; j < WL; ++j)
+          if ((lane * WL + j) % NG == i) largest = max(largest, w[j]);
+        const float top = __half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, largest)));
+        fk[i] = 1.f;
+        if (top * wk[i] >= 128.f) {                                  // largest 2^k in [2^6, 2^7): with P <= 2^8 within fp16's range
+          const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = 64.f / power;
+          fk[i] = k / wk[i];
+          wk[i] = k;
+#pragma unroll
+          for (int j = 0; j < WL; ++j)
+            if ((lane * WL + j) % NG == i) limit[j] = power >= 32768.f ? 0x7C00u : (uint32_t)__half_as_ushort(__float2half_rn(2.f * power));
+        }
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -471,7 +485,6 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
         m[nb] = top;
         mz[nb] = top == -INFINITY ? 0.f : top;
         l[nb] *= f[nb];
-        f[nb] *= fk;
       }
       auto of_row = [&](int r) {                                     // factor of row r, from a lane that holds it
         float v = 1.f;
@@ -486,7 +499,10 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
       for (int c = 0; c < NBV; ++c) {
         const float fr = of_row(c * 4 + t), fo = of_row(c * 4 + g / 2);      // of this lane's columns 2 t and 2 t + 1, and of column g
 #pragma unroll
-        for (int i = 0; i < S::MT; ++i) { o[i][c][0] *= fr; o[i][c][1] *= fr; o[i][c][2] *= fr; o[i][c][3] *= fr; }
+        for (int i = 0; i < S::MT; ++i) {
+          const float x = fr * fk[i * 16 / GROUP];
+          o[i][c][0] *= x; o[i][c][1] *= x; o[i][c][2] *= x; o[i][c][3] *= x;
+        }
 #pragma unroll
         for (int i = 0; i < NG; ++i) off[c][i] *= fo;
       }
@@ -500,7 +516,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
         const float x = ka_ex2(p[u][nb] - mz[nb]);
         l[nb] += x;
         const int key = g + 8 * (t & 1);
-        reinterpret_cast<float*>(st)[(2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4] = x * wk;
+        reinterpret_cast<float*>(st)[(2 * nb + (t >> 1)) * KT + u * 16 + key % 4 * 4 + key / 4] = x;
       }
     __syncwarp();
 
@@ -508,7 +524,6 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
   }
 
   // ---- the warps' sums
-  const float back = 1.f / wk;                                       // a power of two
   float* mo = reinterpret_cast<float*>(ka_sm);                       // [warp][RB][HD]
   float* moff = mo + S::kMergeO / 4;                                 // [warp][RB][NG]
   float* ml = moff + S::kMergeOff / 4;                               // [warp][RB][2]
@@ -531,14 +546,14 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
       float x = off[c][i];
       x += __shfl_xor_sync(0xffffffffu, x, 1);
       x += __shfl_xor_sync(0xffffffffu, x, 2);
-      if (t == 0 && !(g & 1) && c * 8 + g < S::CV) moff[(warp * RB + c * 4 + g / 2) * NG + i] = x * back;
+      if (t == 0 && !(g & 1) && c * 8 + g < S::CV) moff[(warp * RB + c * 4 + g / 2) * NG + i] = x;
     }
 #pragma unroll
     for (int i = 0; i < S::MT; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        // the two terms of row 4 c + t
-        if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + i * 16 + h * 8 + g] = (o[i][c][2 * h] + o[i][c][2 * h + 1]) * back;
+        // the two terms of row 4 c + t, out of the group's power of two
+        if (c * 4 + t < RB) mo[(warp * RB + c * 4 + t) * HD + i * 16 + h * 8 + g] = (o[i][c][2 * h] + o[i][c][2 * h + 1]) * (1.f / wk[i * 16 / GROUP]);
       }
   }
   __syncthreads();

@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv4 import U, Attention, gen, put
+from test_gpu_kv4 import U, Attention, gen, put, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,28 @@ def test_large_scores_of_chunks(pkg, hq, hkv, hd, group, how):
             inner = 6 * torch.sqrt(sigma ** 2 * gap.clamp(min=0) + hd * tau ** 2 * p2.sum(-1)) + 64 * U * vh.abs().amax() * hd ** 0.5
             err = (got[:, h] - o).norm(dim=-1)
             assert (err <= 2.0 ** -8 * (o.norm(dim=-1) + inner) + inner).all(), (b, h, (err / o.norm(dim=-1)).max().item())
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", [(4, 1, 256, 64), (8, 4, 256, 128), (4, 2, 128, 64)])
+@pytest.mark.parametrize("typ", [torch.float32, torch.float16])
+@pytest.mark.parametrize("count", [1, 4])
+def test_small_groups_beside_large_ones(pkg, hq, hkv, hd, group, typ, count):
+    """Groups of V three million times smaller than their neighbours, some of which grow on the way: each is as exact as it would be alone.
+    2^-22 for the terms of a weight, 2 * 2^-20 for the weights (scores of up to 16), 64 u for the sums, of the group's largest value."""
+    lens = [700, 1500, 90]
+    a = Attention(pkg, lens, [count] * 3, hq, hkv, hd, group, typ, seed=hd, tail=0)
+    size = torch.full((max(lens), hd // group), 1e-3, device="cuda")
+    size[:, 0] = 3000.0
+    size[:, -1] = torch.where(torch.arange(max(lens), device="cuda") > 300, 10.0, 1e-4)
+    seq = torch.cat([torch.full((n,), b, dtype=torch.int32) for b, n in enumerate(lens)]).cuda()
+    pos = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]).cuda()
+    k, v = (torch.randn(len(seq), hkv, hd, device="cuda", generator=gen(s)) for s in (1, 2))
+    a.k, a.v = (x.split(lens) for x in put(pkg, a.cache, seq, pos, k, v * size[pos.long()].repeat_interleave(group, 1)[:, None]))
+    a()
+    for b in range(3):
+        at, want = exact(a, b)
+        err = (a.out[at, :hq * hd].double() - want).abs().view(count, hkv, -1, hd // group, group)
+        want = want.view_as(err)
+        top = a.v[b].double().view(lens[b], hkv, 1, hd // group, group).abs().amax((0, 4), keepdim=True)
+        bound = (2.0 ** -22 + 2.0 ** -19 + 64 * U) * top
+        assert (err <= rounded(bound, want, typ)).all(), ((err - rounded(bound * 0, want, typ)) / top).amax((0, 1, 2, 4)).tolist()
