@@ -328,6 +328,7 @@ extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cach
   require_device(device);
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
+  if (window < 0 || window >= max_kv) window = 0;           // it hides nothing; and a position less a window stays within 32 bits
   a.q = q_dev; a.q_type = q_type; a.q_stride = q_stride; a.kv_len = kv_len_dev; a.q_start = q_start_dev;
   a.tokens = tokens; a.max_q = max_q; a.max_kv = max_kv; a.hq = hq; a.window = window;
   a.qscale = 1.4426950408889634f * (scale > 0.f ? scale : 1.f / sqrtf((float)cache->hd));
