@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
       auto get = [&](int i, float (&x)[8]) {
         RawRow<kBf16, 8> raw;
-        if (row < rows) raw.load(src, i, vec);
+        if (hi >= 0) raw.load(src, i, vec);                          // rows that see nothing are zeros, whatever they hold
         else raw.u[0] = raw.u[1] = raw.u[2] = raw.u[3] = 0u;
         raw.get(x);
       };

@@ -20,3 +20,21 @@ def test_windows_as_large_as_their_type(pkg, hq, hkv, hd, group, typ, lens, coun
         a(window=window)
         assert pkg.ops.device_status(a.status.data_ptr(), stream()) == 0
         a.check(window)
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", HEADS)
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("lens,counts", [([3, 70, 0], [7, 72, 3]), ([700, 300, 900], [720, 310, 5])])
+def test_rows_that_see_nothing_are_zero_whatever_they_hold(pkg, hq, hkv, hd, group, typ, lens, counts):
+    a = Attention(pkg, lens, counts, hq, hkv, hd, group, typ, seed=hd + hq)
+    for b, (n, count) in enumerate(zip(lens, counts)):
+        rows = a.q[int(a.start[b]):int(a.start[b]) + max(0, count - n)]
+        rows[0::2, 5], rows[1::2, hd - 1] = float("nan"), float("inf")
+    for window in (0, 40):
+        a.out.fill_(7.0)
+        a(window=window)
+        assert pkg.ops.device_status(a.status.data_ptr(), stream()) == 0
+        for b, (n, count) in enumerate(zip(lens, counts)):
+            rows = a.out[int(a.start[b]):int(a.start[b]) + count, :hq * hd]
+            assert (rows[:max(0, count - n)] == 0).all(), (b, window)
+            assert torch.isfinite(rows).all() and (rows[max(0, count - n):] != 0).any(-1).all()
