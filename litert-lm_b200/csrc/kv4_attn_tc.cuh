@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
       const int e = max((int)(bits >> 23), 30);
       const bool spoilt = bits >= 0x7F800000u;
       const float f = spoilt ? 0.f : __uint_as_float((uint32_t)(254 + 7 - e) << 23);             // largest |q| f in [2^7, 2^8)
-      unit = spoilt ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)(e - 6) << 23) * a.qscale;       // of S / 2
+      // of S / 2; never zero, as masked scores are -inf times this
+      unit = spoilt ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float((uint32_t)(e - 6) << 23) * a.qscale, __uint_as_float(1u << 23));
       float sum = 0.f;
 #pragma unroll 1
       for (int i = 0; i < V; i += 32) {                              // the second time from the cache

@@ -38,3 +38,17 @@ def test_rows_that_see_nothing_are_zero_whatever_they_hold(pkg, hq, hkv, hd, gro
             rows = a.out[int(a.start[b]):int(a.start[b]) + count, :hq * hd]
             assert (rows[:max(0, count - n)] == 0).all(), (b, window)
             assert torch.isfinite(rows).all() and (rows[max(0, count - n):] != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", HEADS)
+@pytest.mark.parametrize("typ", TYPES)
+def test_scales_as_small_as_their_type(pkg, hq, hkv, hd, group, typ):
+    """All weights of a row are the same, those of masked keys zero; rows of zeros among the queries."""
+    a = Attention(pkg, [700, 300, 900], [700, 300, 5], hq, hkv, hd, group, typ, seed=hd + hq)
+    a.q[10:400:3] = 0
+    for scale in (1e-12, 1e-25, 1e-40):
+        for window in (0, 40):
+            a.out.fill_(7.0)
+            a(window=window, scale=scale)
+            assert pkg.ops.device_status(a.status.data_ptr(), stream()) == 0
+            a.check(window, scale)
