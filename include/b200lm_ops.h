@@ -198,6 +198,7 @@ int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_typ
  * q_out_dev [tokens] rows of q_stride, keys to k_out_dev rows of k_stride, in
  * qkv's type; they may be the rows' own places.  hd is 64, 128 or 256, rot a
  * multiple of 16 up to hd (0: no rotation; cos_dev and sin_dev are not read).
+ * Norms hold over the whole range of the types (sums of squares beyond fp32's are taken in fp64); a row of zeros with eps 0 gives NaN.
  * A token with a negative position is padding: its rows are left alone. */
 int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens, int32_t hq,
                          int32_t hkv, int32_t hd, int32_t rot, const float* q_gain_dev, const float* k_gain_dev, float eps,

@@ -5,14 +5,14 @@
 //   m = fp16(low), s = fp16((high - low) / 15), code = rint((x - m) / s) held to 0 .. 15
 //
 // Every byte is read and written once.  What bounds it are issue slots and latencies of the rows' chains, behind them HBM: 8191
-// rows of 8 and 4 heads of 256 in bf16 take 24.4 us = 4.5 TB/s (70 % of the copy rate); 2001 rows of 32 and 16 heads of 128 with
+// rows of 8 and 4 heads of 256 in bf16 take 24.7 us = 4.4 TB/s (68 % of the copy rate); 2001 rows of 32 and 16 heads of 128 with
 // their codes 28.6 us, where the bytes take 9 (300 instructions a pass of 256 elements; ALU 45 %, conversions 25 % busy; with
 // registers for 24 warps an SM 28.6 us, unbounded 35); reading them back 9.4 us = 4.5 TB/s; a single token 1.7 us.
 //
 // A lane holds eight neighbouring elements, so a pass of a warp takes 1, 2 or 4 heads (of 256, 128, 64); the other halves of the
 // pairs lie at the same place of a lane rot / 16 further and come from there as they lay in memory.  A warp takes up to four
 // passes over heads of one kind and token, asks for their rows at once and keeps gain and rotation multiplied in registers.
-// Queries are computed in fp32.  Keys that go into the cache are computed in fp64 and rounded to fp32 before their
+// Queries, and keys that are written out, are computed in fp32, heads whose squares leave that in fp64.  Keys that go into the cache are computed in fp64 and rounded to fp32 before their
 // codes are decided: a code next to a border would otherwise depend on the order of the sum, and one step of a code is a
 // fifteenth of the group's range.
 #pragma once
@@ -145,20 +145,41 @@ __device__ __forceinline__ void row_load(const void* p, long long i, int type, f
 
 constexpr int kVec = 8;             // elements of a lane
 
+// 1 / sqrt(m) to 2^-43 for every m: m = 4^k f with f in 1 .. 4, where fp32's root starts.
+static __device__ __noinline__ double far_root(double m) {
+  if (!(m > 0.0 && m < INFINITY)) return m == 0.0 ? INFINITY : m > 0.0 ? 0.0 : NAN;
+  const int hi = __double2hiint(m), k = ((hi >> 20) - 1023) >> 1;
+  const double f = __hiloint2double(hi - k * (1 << 21), __double2loint(m)), r = rsqrtf((float)f);
+  return r * (1.5 - 0.5 * f * r * r) * __hiloint2double((1023 - k) << 20, 0);
+}
+__device__ __forceinline__ double inverse_root(double m) {
+  // inside fp32's range, 2^-120 .. 2^120, without the detour
+  if ((uint32_t)(__double2hiint(m) - ((1023 - 120) << 20)) >= 240u << 20) return far_root(m);
+  const double r = rsqrtf((float)m);
+  return r * (1.5 - 0.5 * m * r * r);
+}
+// What fp32 can root: outside, the squares of a row leave it (or all of them are zero).
+__device__ __forceinline__ bool far_from_one(float mean) { return !(mean >= 0x1p-100f && mean <= 0x1p100f); }
+
 // Norm and rotation of the elements x that this lane holds of a head, `other` being those of the lane with the other halves of the
-// pairs: y = inv (x ca + other sb), ca = gain * cos, sb = +- the other's gain * sin.
+// pairs: y = inv (x ca + other sb), ca = gain * cos, sb = +- the other's gain * sin.  True where that has to be done in fp64.
 template <typename T, int HD>
-__device__ __forceinline__ void norm_rotate(const float (&x)[kVec], const float (&other)[kVec], bool norm, float eps, const T (&ca)[kVec], const T (&sb)[kVec], bool rotates, T (&y)[kVec]) {
+__device__ __forceinline__ bool norm_rotate(const float (&x)[kVec], const float (&other)[kVec], bool norm, float eps, const T (&ca)[kVec], const T (&sb)[kVec], bool rotates, T (&y)[kVec]) {
   T inv = 1;
+  bool far = false;
   if (norm) {
     T sum = 0;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) sum += (T)x[j] * (T)x[j];
 #pragma unroll
     for (int o = HD / kVec / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const T mean = sum * (T)(1.0 / HD) + (T)eps;
-    inv = rsqrtf((float)mean);
-    if constexpr (sizeof(T) == 8) inv = inv * (1.5 - 0.5 * mean * inv * inv);      // 2^-22 -> 2^-43
+    const T mean = sum * (T)(1.0 / HD);
+    if constexpr (sizeof(T) == 8) {
+      inv = inverse_root(mean + (T)eps);
+    } else {
+      inv = rsqrtf(mean + eps);
+      far = far_from_one(mean);
+    }
   }
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
@@ -166,6 +187,7 @@ __device__ __forceinline__ void norm_rotate(const float (&x)[kVec], const float 
     if (rotates) y[j] += (T)other[j] * sb[j];
     y[j] *= inv;
   }
+  return far;
 }
 
 // What fp64 says where fp32 leaves it open; kept out of the loops, which it would push out of the instruction cache.
@@ -301,30 +323,87 @@ __device__ __forceinline__ void table_row(const float* p, long long i, float (&x
   r.get(x);
 }
 
-// NP passes of 256 / HD heads of one kind and token a warp; GROUP 0: keys are written out, else keys and values go into the cache.
+// What a warp has to do: NP passes of 256 / HD heads of one kind and token.
+template <int HD, int NP, bool APPEND>
+struct RowJob {
+  static constexpr int LH = HD / kVec, HP = 32 / LH, NH = NP * HP;     // lanes of a head, heads of a pass, of a warp
+  int tok, heads, passes, mine;                                        // mine: this lane's first head; those behind the last compute the last one's and write nothing
+  bool is_q, is_v;
+  long long row;                                                       // of qkv, at this lane's elements of head 0
+  __device__ __forceinline__ explicit RowJob(const RowArgs& a) {
+    const int lane = threadIdx.x & 31;
+    // a token's jobs: query heads, key heads, value heads
+    const int jq = (a.hq + NH - 1) / NH, jk = (a.hkv + NH - 1) / NH;
+    const uint32_t per = jq + (APPEND ? 2 : 1) * jk, job = blockIdx.x * 4 + (threadIdx.x >> 5);
+    tok = (int)(job / per);
+    const int part = (int)(job - tok * per);
+    is_q = part < jq;
+    is_v = APPEND && part >= jq + jk;
+    heads = is_q ? a.hq : a.hkv;
+    const int h0 = (is_q ? part : is_v ? part - jq - jk : part - jq) * NH;
+    passes = min(NP, (heads - h0 + HP - 1) / HP);
+    mine = h0 + lane / LH;
+    row = tok * a.stride + (is_q ? 0 : is_v ? a.hq + a.hkv : a.hq) * HD + lane % LH * kVec;
+  }
+};
+
+// The heads of a warp whose squares leave fp32 (a bit for each pass, by lane), once more in fp64 from memory, where they are as they were.
+// It finds out by itself what the warp's job is, so that nothing of that stays in registers for it (the loops of the others lost a fifth
+// to that: 24.7 us -> 29.0 for 8191 rows).
+template <int HD, int TYPE, int NP, bool APPEND, bool VEC>
+static __device__ __noinline__ void far_heads(const RowArgs* args, uint32_t far) {
+  using Job = RowJob<HD, NP, APPEND>;
+  const RowArgs& a = *args;
+  const Job w(a);
+  const int lane = threadIdx.x & 31, e0 = lane % Job::LH * kVec, half = a.rot / 2;
+  const bool rotates = e0 < a.rot, first = e0 < half;
+  const int other_lane = lane + (rotates ? (first ? half / kVec : -(half / kVec)) : 0);
+  const float* gain = (w.is_q ? a.q_gain : a.k_gain) + e0;
+  const long long turn = (long long)a.pos[w.tok] * half + e0 - (first ? 0 : half);
+  void* out = w.is_q ? a.q_out : a.k_out;
+  const long long at = w.tok * (w.is_q ? a.q_stride : a.k_stride) + e0;
+#pragma unroll 1
+  for (int i = 0; i < w.passes; ++i) {
+    if (!__any_sync(0xffffffffu, far >> i & 1)) continue;
+    const int head = w.mine + i * Job::HP;
+    RawRow<TYPE, kVec> raw;
+    raw.load(a.qkv, w.row + min(head, w.heads - 1) * HD, VEC);
+    float x[kVec];
+    raw.get(x);
+    double sum = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) sum += (double)x[j] * x[j];
+#pragma unroll
+    for (int o = Job::LH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double inv = inverse_root(sum * (1.0 / HD) + (double)a.eps);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const double v = (double)x[j] * gain[j], other = __shfl_sync(0xffffffffu, v, other_lane);
+      x[j] = (float)((rotates ? v * a.cos[turn + j] + (first ? -other : other) * a.sin[turn + j] : v) * inv);
+    }
+    raw.put(x);
+    if ((far >> i & 1) && head < w.heads) raw.store(out, at + head * HD, VEC);
+  }
+}
+
+// GROUP 0: keys are written out, else keys and values go into the cache.
 // VEC: all rows and tables start on 16-byte boundaries.
 template <int HD, int TYPE, int GROUP, int NP, bool VEC>
-__global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const RowArgs a) {
-  constexpr int LH = HD / kVec, HP = 32 / LH, NH = NP * HP;             // lanes of a head, heads of a pass, of a warp
+__global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const __grid_constant__ RowArgs a) {
+  constexpr int LH = HD / kVec, HP = 32 / LH;                           // lanes of a head, heads of a pass
   constexpr bool APPEND = GROUP > 0;
   __shared__ __align__(16) uint8_t stage[4][APPEND ? 128 : 16];
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  // a token's jobs: query heads, key heads, value heads
-  const int jq = (a.hq + NH - 1) / NH, jk = (a.hkv + NH - 1) / NH;
-  const uint32_t per = jq + (APPEND ? 2 : 1) * jk, job = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int tok = (int)(job / per), part = (int)(job - tok * per);
+  const int lane = threadIdx.x & 31, e0 = lane % LH * kVec;
+  const RowJob<HD, NP, APPEND> job(a);
+  const int tok = job.tok, heads = job.heads, passes = job.passes, mine = job.mine;
+  const bool is_q = job.is_q, is_v = job.is_v;
   if (tok >= a.tokens) return;
-  const bool is_q = part < jq, is_v = APPEND && part >= jq + jk;
-  // this lane's first head; those behind the last compute the last one's and write nothing
-  const int heads = is_q ? a.hq : a.hkv, h0 = (is_q ? part : is_v ? part - jq - jk : part - jq) * NH, passes = min(NP, (heads - h0 + HP - 1) / HP), mine = h0 + lane / LH;
-  const int e0 = lane % LH * kVec;
-  const long long row = tok * a.stride + (is_q ? 0 : is_v ? a.hq + a.hkv : a.hq) * HD + e0;
   RawRow<TYPE, kVec> raw[NP];
 #pragma unroll
   for (int i = 0; i < NP; ++i)
-    if (i < passes) raw[i].load(a.qkv, row + min(mine + i * HP, heads - 1) * HD, VEC);
+    if (i < passes) raw[i].load(a.qkv, job.row + min(mine + i * HP, heads - 1) * HD, VEC);
   const int pos = a.pos[tok];
   if (pos < 0) return;
   if (a.rot > 0 && pos >= a.rope_rows) { set_status(a.status, kDevBadPosition); return; }
@@ -370,26 +449,29 @@ __global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const 
       raw[0].get(x);
       fellow.get(f);
       T y[kVec];
-      norm_rotate<T, HD>(x, f, norm, a.eps, c, s, rotates, y);
+      const bool far = norm_rotate<T, HD>(x, f, norm, a.eps, c, s, rotates, y);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) x[j] = (float)y[j];
-      done(i, x);
+      done(i, x, far);
       next();
     }
   };
   if (is_q || !APPEND) {
     void* out = is_q ? a.q_out : a.k_out;
     const long long at = tok * (is_q ? a.q_stride : a.k_stride) + e0;
-    normed(1.f, [&](int i, const float (&x)[kVec]) {
+    uint32_t left = 0;
+    normed(1.f, [&](int i, const float (&x)[kVec], bool far) {
       RawRow<TYPE, kVec> y;
       y.put(x);
-      if (mine + i * HP < heads) y.store(out, at + (mine + i * HP) * HD, VEC);
+      if (mine + i * HP < heads && !far) y.store(out, at + (mine + i * HP) * HD, VEC);
+      left |= (uint32_t)far << i;
     });
+    if (__any_sync(0xffffffffu, left != 0)) far_heads<HD, TYPE, NP, APPEND, VEC>(&a, left);
   }
   if constexpr (APPEND) {
     constexpr Kv4Dims d{HD, GROUP};
     constexpr int GL = GROUP / kVec;
-    auto put = [&](int i, const float (&x)[kVec]) {
+    auto put = [&](int i, const float (&x)[kVec], bool) {
       const int h = mine + i * HP;
       uint8_t* head = page + (long long)h * d.head_bytes();
       uint32_t word[2];
@@ -402,7 +484,7 @@ __global__ void __launch_bounds__(128, GROUP ? 6 : 1) qk_norm_rope_kernel(const 
       for (int i = 0; i < passes; ++i) {
         float x[kVec];
         raw[0].get(x);
-        put(i, x);
+        put(i, x, false);
         next();
       }
     } else if (!is_q) {
