@@ -185,7 +185,7 @@ int B200LmOps_RepackW4Grouped(const uint8_t* packed, const uint16_t* scale, cons
  * 32, 64 or 128 (the last group may be shorter), scale_type B200LM_BF16 or _F16.
  * w_dev is the image above, on a 16-byte boundary.  Sums are in fp32, and x
  * enters exact to 2^-27 of the largest value of a block of 128 (2^-20 with more
- * than four columns of a 16-bit type); an infinity or NaN in a column makes all of its outputs NaN. */
+ * than four columns of a 16-bit type), of 2^-117 where all of them are smaller; an infinity or NaN in a column makes all of its outputs NaN. */
 int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_type, int32_t has_offset, int64_t n, int64_t k,
                             int32_t group, const void* x_dev, int32_t x_type, int64_t ldx, int32_t ncols, void* y_dev,
                             int32_t y_type, int64_t ldy, void* stream, char** err);

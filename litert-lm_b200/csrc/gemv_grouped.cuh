@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(kGgThreads, 2) gemv_grouped_kernel(const GgArg
       const float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
       const bool odd = !isfinite(x.x) || !isfinite(x.y) || !isfinite(x.z) || !isfinite(x.w);
       const uint32_t bits = __reduce_max_sync(0xffffffffu, odd ? 0x7F800000u : __float_as_uint(top));
-      // 2^5 <= largest |x| f < 2^6; the power stays inside fp32 for the smallest and largest x
-      const int e = max((int)(bits >> 23), 30);
+      // 2^5 <= largest |x| f < 2^6, for the smallest x (below 2^-117) less; f and the digits' unit below are normal numbers
+      const int e = max((int)(bits >> 23), 10);
       const float f = __uint_as_float((uint32_t)(254 + 5 - e) << 23);
       float r[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
       if (bits >= 0x7F800000u) r[0] = r[1] = r[2] = r[3] = 0.f;
