@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.util
 import os
+import sysconfig
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -25,7 +26,7 @@ from . import sharding  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200lm.so")
-CALLS_PATH = os.path.join(_HERE, "_calls.so")
+CALLS_PATH = os.path.join(_HERE, "_calls" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 # absl::StatusCode
 OK, CANCELLED, INVALID_ARGUMENT, DEADLINE_EXCEEDED, NOT_FOUND = 0, 1, 3, 4, 5
@@ -183,7 +184,7 @@ def _calls():
     if _calls_module is None:
         load_library()
         if not os.path.exists(CALLS_PATH):
-            raise RuntimeError(f"{CALLS_PATH} is missing: build it with `python litert-lm_b200/build.py`")
+            raise RuntimeError(f"{CALLS_PATH} is missing: build it with `python litert-lm_b200/build.py` (which needs Python.h for it)")
         spec = importlib.util.spec_from_file_location("_calls", CALLS_PATH)
         _calls_module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(_calls_module)
