@@ -157,8 +157,9 @@ int B200LmOps_AttentionDecodeStaticStatus(int32_t device, void* stream, int32_t*
  *   - status_dev (may be NULL) is a word of the caller's, zero at first, to which
  *     the kernels add what only they can see: a position or a length outside the
  *     cache, the page table or the rotation table, a page number outside the
- *     pool.  What such a token or sequence would have written stays as it was;
- *     the others are served.  B200LmOps_DeviceStatus reads the word. */
+ *     pool (of the pages that a token, or any row of a sequence, needs).  What
+ *     such a token or sequence would have written stays as it was; the others
+ *     are served.  B200LmOps_DeviceStatus reads the word. */
 #define B200LM_F32 0
 #define B200LM_BF16 1
 #define B200LM_F16 2

@@ -104,6 +104,17 @@ __device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
 }
 __device__ __forceinline__ float2 ka_unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
+// A thread's look at the pages that the rows of a sequence need, from the first that the first row sees to the last: `one` of `all` threads.
+// A page outside the pool leaves all rows of the sequence alone, also those of CTAs that would not read it.
+__device__ __forceinline__ bool ka_bad_page(const Kv4AttnArgs& a, const int* table, int len, int nq, int one, int all) {
+  bool bad = false;
+  for (int i = (a.window > 0 ? max(0, len - nq - a.window + 1) : 0) / kKv4Page + one; i < (len + kKv4Page - 1) / kKv4Page; i += all) {
+    const int page = table[i];
+    bad = bad || page < 0 || page >= a.kv.num_pages;
+  }
+  return bad;
+}
+
 template <int N>
 __device__ __forceinline__ void ka_words(const unsigned char* p, uint32_t (&d)[N]) {
   if constexpr (N == 4) {
@@ -148,7 +159,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
   const Kv4Dims d{HD, GROUP};
   const long long head = (long long)kvh * d.head_bytes(), page_bytes = (long long)a.kv.hkv * d.head_bytes();
   const int* table = a.kv.table + b * a.kv.table_stride;
-  bool bad = false;
+  bool bad = ka_bad_page(a, table, len, nq, threadIdx.x, kKaThreads);
   int next = t0 + warp, slot_in = 0;
   int page = next < t1 ? table[next * KT / kKv4Page] : 0;
   auto issue = [&]() {

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
   int* gave_up = reinterpret_cast<int*>(bars + kKcBars + 1);
   auto wait = [&](KcWait w) { return mbar_wait(bars + w.bar, w.parity(), gave_up); };
   auto wait2 = [&](KcWait w, KcWait x) { return mbar_wait2(bars + w.bar, w.parity(), bars + x.bar, x.parity(), gave_up); };
-  __shared__ int last_s;
+  __shared__ int last_s, closed_s;                                   // closed: a page that the sequence needs lies outside the pool
   __shared__ unsigned poison[kKcRows];                               // bit i: the row sees a NaN among the elements 64 i .. of V
   const int warp = warp_index(), lane = threadIdx.x & 31;
   pdl_wait();
@@ -126,12 +126,17 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
   for (int i = threadIdx.x; i < (S::kMax - S::kKx) / 16; i += S::kThreads) reinterpret_cast<uint4*>(kx)[i] = make_uint4(0u, 0u, 0u, 0u);      // places of 64 that a head does not have
   if (threadIdx.x < kKcRows) poison[threadIdx.x] = 0u;
   fence_async_smem();
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    const bool closed = __any_sync(0xffffffffu, ka_bad_page(a, a.kv.table + b * a.kv.table_stride, len, nq, lane, 32));
+    if (lane == 0) closed_s = closed;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
+  const int* table = a.kv.table + b * a.kv.table_stride;
   bool ok = true, bad = false;                                       // none of this thread's waits has given up; a page outside the pool
   const int quarter = warp & 3, half = (warp >> 2) & 1, row = quarter * 32 + lane;     // softmax
   const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -140,7 +145,6 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     // ---- expansion: the first half of the warps has K rows, the other V rows; thread (key, plane, q): 32 bytes, 64 elements
     const int w = (warp - 9) % (4 * P), key = w / P * 16 + (lane & 15), plane = w % P, q = lane >> 4;
     const bool has_k = warp - 9 < 4 * P;
-    const int* table = a.kv.table + b * a.kv.table_stride;
     const long long page_bytes = (long long)a.kv.hkv * d.head_bytes(), head = (long long)kvh * d.head_bytes();
     uint4 raw[2];
     uint32_t sm[2];                                           // (s, m) of K or V, for each 64 of the plane's elements
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(KcShape<HD>::kThreads, 1) kv4_chunk_kernel(con
     tc_fence_after();
   }
   // ---- row sums meet; O out of tensor memory
-  const bool spoilt = __syncthreads_or(bad) != 0, failed = __syncthreads_or(!ok) != 0;
+  const bool spoilt = __syncthreads_or(bad || closed_s) != 0, failed = __syncthreads_or(!ok) != 0;
   const long long u = ((long long)b * a.kv.hkv + kvh) * a.row_tiles + tile;
   constexpr int REC = kKcRows * (HD + 2);
   float* rec = a.parts + (u * a.splits + split) * REC;

@@ -52,3 +52,27 @@ def test_scales_as_small_as_their_type(pkg, hq, hkv, hd, group, typ):
             a(window=window, scale=scale)
             assert pkg.ops.device_status(a.status.data_ptr(), stream()) == 0
             a.check(window, scale)
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", HEADS)
+@pytest.mark.parametrize("typ", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens,counts", [([1500, 600, 900], [1, 1, 1]), ([1500, 600, 900], [600, 200, 700])])
+def test_a_bad_page_leaves_its_whole_sequence(pkg, hq, hkv, hd, group, typ, lens, counts):
+    """Rows that do not reach the page themselves too, however rows share CTAs; pages ahead of every row's window are nobody's."""
+    a = Attention(pkg, lens, counts, hq, hkv, hd, group, typ, seed=hd)
+    table = a.cache.table.clone()
+    for page in (0, 3, 5):
+        a.cache.table[0, page] = -1 if page else a.cache.n
+        a.out.fill_(7.0)
+        a()
+        with pytest.raises(pkg.StatusError) as e:
+            pkg.ops.device_status(a.status.data_ptr(), stream())
+        assert e.value.code == pkg.INVALID_ARGUMENT
+        assert (a.out[:counts[0]] == 7.0).all()
+        a.check(skip=(0,))
+        a.cache.table.copy_(table)
+    a.cache.table[0, 0], a.cache.table[0, 1] = -1, 2 ** 31 - 1      # positions below 512; the first row's window begins behind 600
+    a.out.fill_(7.0)
+    a(window=200)
+    assert pkg.ops.device_status(a.status.data_ptr(), stream()) == 0
+    a.check(200)
