@@ -6,6 +6,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <exception>
 #include <string>
 
 #include "common.cuh"
@@ -45,6 +46,14 @@ inline void require_device(int device) {
   }
   B2_CHECK(device >= 0 && device < ndev, kInvalidArgument, "device ordinal out of range");
 }
+
+// Around the body of an entry point: failures become status codes and messages.
+#define OP_TRY if (err) *err = nullptr; try {
+#define OP_END                                                                                                    \
+  return ::b200lm::kOk; }                                                                                         \
+  catch (const ::b200lm::Error& e_) { return ::b200lm::static_fail(err, e_.code, e_.msg); }                       \
+  catch (const std::exception& e_) { return ::b200lm::static_fail(err, ::b200lm::kInternal, e_.what()); }         \
+  catch (...) { return ::b200lm::static_fail(err, ::b200lm::kInternal, "unknown failure"); }
 
 // Multiprocessors of `device`, asked for once.
 inline int device_sms(int device) {

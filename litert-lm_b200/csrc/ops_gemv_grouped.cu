@@ -4,7 +4,6 @@
 #include "op_host.h"
 
 #include <algorithm>
-#include <exception>
 
 namespace b200lm {
 
@@ -75,24 +74,17 @@ static void launch_gg_cols(cudaStream_t st, const GgArgs& a, int sms) {
 
 using namespace b200lm;
 
-#define GG_TRY if (err) *err = nullptr; try {
-#define GG_END                                                                          \
-  return kOk; }                                                                         \
-  catch (const Error& e_) { return static_fail(err, e_.code, e_.msg); }                 \
-  catch (const std::exception& e_) { return static_fail(err, kInternal, e_.what()); }   \
-  catch (...) { return static_fail(err, kInternal, "unknown failure"); }
-
 extern "C" int B200LmOps_GemvW4GroupedBytes(int64_t n, int64_t k, int32_t group, int32_t has_offset, int64_t* bytes, char** err) {
-  GG_TRY
+  OP_TRY
   B2_CHECK(bytes, kInvalidArgument, "null pointer");
   check_grouped(n, k, group);
   *bytes = grouped_bytes(n, k, group, has_offset != 0);
-  GG_END
+  OP_END
 }
 
 extern "C" int B200LmOps_RepackW4Grouped(const uint8_t* packed, const uint16_t* scale, const uint16_t* offset, int64_t n, int64_t k,
                                          int32_t group, uint8_t* out, char** err) {
-  GG_TRY
+  OP_TRY
   B2_CHECK(packed && scale && out, kInvalidArgument, "null pointer");
   check_grouped(n, k, group);
   const int64_t blocks = (k + 127) / 128, bytes = grouped_block(group, offset != nullptr), groups = (k + group - 1) / group;
@@ -112,13 +104,13 @@ extern "C" int B200LmOps_RepackW4Grouped(const uint8_t* packed, const uint16_t* 
       if (offset) memcpy(at + 32 * per, offset + r * groups + j, 2);
     }
   }
-  GG_END
+  OP_END
 }
 
 extern "C" int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_type, int32_t has_offset, int64_t n, int64_t k,
                                        int32_t group, const void* x_dev, int32_t x_type, int64_t ldx, int32_t ncols, void* y_dev,
                                        int32_t y_type, int64_t ldy, void* stream, char** err) {
-  GG_TRY
+  OP_TRY
   B2_CHECK(w_dev && x_dev && y_dev, kInvalidArgument, "null pointer");
   check_grouped(n, k, group);
   B2_CHECK(scale_type == kBf16 || scale_type == kF16, kInvalidArgument, "scale_type must be B200LM_BF16 or B200LM_F16");
@@ -149,5 +141,5 @@ extern "C" int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_
   if (group == 32) has_offset ? launch_gg_cols<32, true>(st, a, sms) : launch_gg_cols<32, false>(st, a, sms);
   else if (group == 64) has_offset ? launch_gg_cols<64, true>(st, a, sms) : launch_gg_cols<64, false>(st, a, sms);
   else has_offset ? launch_gg_cols<128, true>(st, a, sms) : launch_gg_cols<128, false>(st, a, sms);
-  GG_END
+  OP_END
 }

@@ -5,7 +5,6 @@
 #include "op_host.h"
 
 #include <algorithm>
-#include <exception>
 
 namespace b200lm {
 
@@ -190,15 +189,8 @@ static bool chunk_pays(const Kv4Plan& few, const Kv4Plan& many, int hd, int max_
 
 using namespace b200lm;
 
-#define KV4_TRY if (err) *err = nullptr; try {
-#define KV4_END                                                                         \
-  return kOk; }                                                                         \
-  catch (const Error& e_) { return static_fail(err, e_.code, e_.msg); }                 \
-  catch (const std::exception& e_) { return static_fail(err, kInternal, e_.what()); }   \
-  catch (...) { return static_fail(err, kInternal, "unknown failure"); }
-
 extern "C" int B200LmOps_DeviceStatus(int32_t device, void* stream, int32_t* status_dev, int32_t* device_error, char** err) {
-  KV4_TRY
+  OP_TRY
   check_pointer(status_dev, 4, "status_dev");
   require_device(device);
   DeviceScope scope(device);
@@ -211,16 +203,16 @@ extern "C" int B200LmOps_DeviceStatus(int32_t device, void* stream, int32_t* sta
   if (word == kDevBadPosition) throw Error{kInvalidArgument, "a position, length or page lay outside its table"};
   if (word == kDevBarrierTimeout) throw Error{kDeadlineExceeded, "a bounded device-side wait gave up"};
   if (word != kDevOk) throw Error{kInternal, "device error word " + std::to_string(word)};
-  KV4_END
+  OP_END
 }
 
 extern "C" int B200LmOps_Kv4PageBytes(int32_t hkv, int32_t hd, int32_t group, int64_t* bytes, char** err) {
-  KV4_TRY
+  OP_TRY
   B2_CHECK(bytes, kInvalidArgument, "null pointer");
   check_heads(hkv, hd);
   check_group(hd, group);
   *bytes = (int64_t)hkv * Kv4Dims{hd, group}.head_bytes();
-  KV4_END
+  OP_END
 }
 
 extern "C" int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens, int32_t hq,
@@ -228,7 +220,7 @@ extern "C" int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t
                                     const float* cos_dev, const float* sin_dev, int32_t rope_rows, const int32_t* pos_dev,
                                     void* q_out_dev, int64_t q_stride, void* k_out_dev, int64_t k_stride, int32_t* status_dev,
                                     void* stream, char** err) {
-  KV4_TRY
+  OP_TRY
   RowArgs a = row_args(qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev, q_out_dev, q_stride, status_dev);
   check_pointer(k_out_dev, elem_size(type), "k_out_dev");
   B2_CHECK(k_stride >= (int64_t)hkv * hd, kInvalidArgument, "a row stride is shorter than its row");
@@ -238,7 +230,7 @@ extern "C" int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
   launch_rows(reinterpret_cast<cudaStream_t>(stream), a, hd, 0, device_sms(device));
-  KV4_END
+  OP_END
 }
 
 extern "C" int B200LmOps_QkNormRopeAppendKv4(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens,
@@ -247,7 +239,7 @@ extern "C" int B200LmOps_QkNormRopeAppendKv4(int32_t device, const void* qkv_dev
                                              int32_t rope_rows, const int32_t* pos_dev, void* q_out_dev, int64_t q_stride,
                                              const B200LmKv4Cache* cache, const int32_t* seq_dev, int32_t* status_dev, void* stream,
                                              char** err) {
-  KV4_TRY
+  OP_TRY
   RowArgs a = row_args(qkv_dev, type, qkv_stride, tokens, hq, hkv, hd, rot, q_gain_dev, k_gain_dev, eps, cos_dev, sin_dev, rope_rows, pos_dev, q_out_dev, q_stride, status_dev);
   a.kv = cache_args(cache);
   B2_CHECK(cache->hkv == hkv && cache->hd == hd, kInvalidArgument, "the cache's heads are not the rows'");
@@ -258,13 +250,13 @@ extern "C" int B200LmOps_QkNormRopeAppendKv4(int32_t device, const void* qkv_dev
   if (tokens == 0) return kOk;
   DeviceScope scope(device);
   launch_rows(reinterpret_cast<cudaStream_t>(stream), a, hd, cache->group, device_sms(device));
-  KV4_END
+  OP_END
 }
 
 extern "C" int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, const int32_t* seq_dev, const int32_t* pos_dev,
                                  int32_t tokens, int32_t out_type, void* k_out_dev, void* v_out_dev, int32_t* status_dev, void* stream,
                                  char** err) {
-  KV4_TRY
+  OP_TRY
   const Kv4Args kv = cache_args(cache);
   check_type(out_type);
   B2_CHECK(tokens >= 0, kInvalidArgument, "tokens is negative");
@@ -281,7 +273,7 @@ extern "C" int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, co
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const auto read = kv.d.hd == 64 ? launch_read<64, 64> : kv.d.hd == 128 ? (kv.d.group == 64 ? launch_read<128, 64> : launch_read<128, 128>) : kv.d.group == 64 ? launch_read<256, 64> : launch_read<256, 128>;
   read(st, out_type, kv, seq_dev, pos_dev, tokens, k_out_dev, v_out_dev, status_dev);
-  KV4_END
+  OP_END
 }
 
 static void check_attention(int batch, int hkv, int hd, int hq, int max_q, int max_kv) {
@@ -295,7 +287,7 @@ static void check_attention(int batch, int hkv, int hd, int hq, int max_q, int m
 
 extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, int32_t hkv, int32_t hd, int32_t hq, int32_t max_q,
                                                int32_t max_kv, int64_t* bytes, char** err) {
-  KV4_TRY
+  OP_TRY
   B2_CHECK(bytes, kInvalidArgument, "null pointer");
   check_attention(batch, hkv, hd, hq, max_q, max_kv);
   require_device(device);
@@ -303,14 +295,14 @@ extern "C" int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, in
   const int sms = device_sms(device);
   *bytes = plan_attention(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes;
   if (hd >= 128 && (long long)max_q * (hq / hkv) >= kChunkRows) *bytes = std::max(*bytes, plan_chunk(batch, hkv, hd, hq, max_q, max_kv, 0, sms).bytes);
-  KV4_END
+  OP_END
 }
 
 extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cache, const void* q_dev, int32_t q_type, int64_t q_stride,
                                       const int32_t* kv_len_dev, const int32_t* q_start_dev, int32_t tokens, int32_t max_q,
                                       int32_t max_kv, int32_t hq, int32_t window, float scale, void* out_dev, int64_t out_stride,
                                       void* workspace_dev, int64_t workspace_bytes, int32_t* status_dev, void* stream, char** err) {
-  KV4_TRY
+  OP_TRY
   Kv4AttnArgs a{};
   a.kv = cache_args(cache);
   check_attention(cache->batch, cache->hkv, cache->hd, hq, max_q, max_kv);
@@ -351,5 +343,5 @@ extern "C" int B200LmOps_AttentionKv4(int32_t device, const B200LmKv4Cache* cach
   else if (cache->hd == 64) launch_kv4_attn_64(st, a, p.rb);
   else if (cache->hd == 128) launch_kv4_attn_128(st, a, p.rb);
   else launch_kv4_attn_256(st, a, p.rb);
-  KV4_END
+  OP_END
 }
