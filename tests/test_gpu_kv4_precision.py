@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_kv4 import U, Attention, gen, put, rounded
+from test_gpu_kv4 import TYPES, U, Attention, gen, put, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,29 @@ def test_small_groups_beside_large_ones(pkg, hq, hkv, hd, group, typ, count):
         top = a.v[b].double().view(lens[b], hkv, 1, hd // group, group).abs().amax((0, 4), keepdim=True)
         bound = (2.0 ** -22 + 2.0 ** -19 + 64 * U) * top
         assert (err <= rounded(bound, want, typ)).all(), ((err - rounded(bound * 0, want, typ)) / top).amax((0, 1, 2, 4)).tolist()
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", [(8, 4, 256, 64), (16, 2, 128, 128)])
+@pytest.mark.parametrize("gap", [12.0, 18.0, 20.0])
+@pytest.mark.parametrize("typ", TYPES)
+def test_many_small_weights_beside_a_large_one(pkg, hq, hkv, hd, group, gap, typ):
+    """One key `gap` above all others, whose value is zero, and thousands of e^-gap with values of one: what is left is their sum, to 2^-9
+    ahead of storing it (weights to 2^-11, one exponent) and 2^-36 a key: fp16 numbers are 2^-24 apart below 2^-14, so a weight that is held
+    times 2^11 is off by at most 2^-25-11 of the largest."""
+    lens, counts = [9000, 3000], [200, 150]
+    a = Attention(pkg, lens, counts, hq, hkv, hd, group, typ, seed=1, tail=0)
+    a.q[:] = 0
+    a.q[:, :hq * hd].view(-1, hq, hd)[..., 0] = 1.0
+    seq = torch.cat([torch.full((n,), b, dtype=torch.int32) for b, n in enumerate(lens)]).cuda()
+    pos = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]).cuda()
+    k, v = torch.zeros(len(seq), hkv, hd, device="cuda"), torch.ones(len(seq), hkv, hd, device="cuda")
+    first = pos == 3
+    k[first, :, 0], v[first] = gap * hd ** 0.5, 0.0
+    k, v = put(pkg, a.cache, seq, pos, k, v)
+    assert (v[~first] == 1).all() and (v[first] == 0).all() and (k[~first] == 0).all()
+    a()
+    for b, (n, count) in enumerate(zip(lens, counts)):
+        rows = a.out[int(a.start[b]):int(a.start[b]) + count, :hq * hd].double()
+        rest = torch.arange(n - count, n, device="cuda", dtype=torch.float64) * torch.exp(-k[first][b, 0, 0].double() * hd ** -0.5)
+        want = (rest / (1 + rest))[:, None]
+        assert ((rows - want).abs() <= rounded(want * 2.0 ** -9 + n * 2.0 ** -36, want, typ)).all(), (rows / want).aminmax()
