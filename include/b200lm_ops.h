@@ -263,7 +263,7 @@ int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, const int32_t
  * `window` of those.  A row that sees none gives zeros.  kv_len_dev[b] is at most
  * max_kv, max_kv at most 256 * table_stride.  scale <= 0 means 1/sqrt(hd).  out_dev
  * is of q's type; rows behind the last sequence's are left as they were.  Scores are sums of exact products in fp32, a
- * key's weight, times its scales, enters the second product to 2^-22.  bf16 calls with many rows of a kv head (16 and more, head sizes 128
+ * key's weight, times its scales, enters the second product to 2^-22 (2^-36 of the row's largest where that is more).  bf16 calls with many rows of a kv head (16 and more, head sizes 128
  * and 256) may run on a kernel that rounds weights and values to fp16 for the second product, 2^-11 of each
  * (weights 2^-36 of the row's largest where that is more).
  * A group that stands for NaN makes, in V, its own elements of the rows that see the position NaN, in K those rows.

@@ -10,7 +10,7 @@
 //   O  fp16 products (m16n8k16) with the codes as numbers c - 8 (exact) and P s in two fp16 terms (2^-22 of each weight).  One
 //      term, with P and m + 8 s as fp16 numbers too, took 5.6 us off the 93 of 64 bf16 sequences and put 3 * 2^-11 on each weight:
 //      one bf16 result in ten came out a step off.  P s is held in a power of two below fp16's range, one for each group of
-//      dims: its reference is the largest scale of the group that the warp has met, so small weights are off by 2^-31 of that.
+//      dims: its reference is the largest scale of the group that the warp has met, so small weights are off by 2^-36 of that.
 //      Two nibbles of a half word come out of a mask each (1024 + c and 1024 + 16 c) and a fused product makes them c - 8; as
 //      bf16 numbers they would need a shift each, and the logic pipe, half as wide as the others, is what bounds this kernel.
 //      Codes centred at zero keep the sums small; the tensor core cuts its sums off, so fp32 rows take them out after every
@@ -19,7 +19,7 @@
 // A warp walks its own tiles of keys (16 at head size 256, else 32) with a ring of its own that it fills by 16-byte asynchronous
 // copies: K and V rows lie in the cache in the order in which the fragments want them, so a lane's loads are 8 or 16 bytes
 // wide and free of bank conflicts.  Warps meet only at the end.  The softmax keeps a reference per row and warp that moves when a
-// score passes it by 8 powers of two, so that an ordinary tile takes one vote and no exchange of maxima.
+// score passes it by 4 powers of two, so that an ordinary tile takes one vote and no exchange of maxima.
 //
 // A CTA serves RB rows over a share of the keys; shares of a sequence are joined by the last CTA to arrive.  How many
 // keys a share has is decided on the host from the largest length, how many shares a sequence has on the device from its own.
@@ -69,7 +69,7 @@ struct KaShape {
   static_assert(kMergeO + kMergeOff + kKaWarps * RB * 8 + RB * 8 <= kRing, "the exchange fits over the ring");
   static_assert(RB * KT * 4 <= kCodes, "P of a tile fits over its K codes");
   static_assert(RB * NG <= 32, "a bit for each row and group");
-  static constexpr float kLazy = 8.f;                                // powers of two by which a score may pass its row's reference
+  static constexpr float kLazy = 4.f;                                // powers of two by which a score may pass its row's reference
   static constexpr int kSmem = kUnit + RB * 4 + RB * NG * 4;
 };
 
@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
           if ((lane * WL + j) % NG == i) largest = max(largest, w[j]);
         const float top = __half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, largest)));
         fk[i] = 1.f;
-        if (top * wk[i] >= 128.f) {                                  // largest 2^k in [2^6, 2^7): with P <= 2^8 within fp16's range
-          const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = 64.f / power;
+        if (top * wk[i] >= 2048.f) {                                 // largest 2^k in [2^10, 2^11): with P <= 2^4 within fp16's range
+          const float power = __uint_as_float(__float_as_uint(top) & 0x7F800000u), k = 1024.f / power;
           fk[i] = k / wk[i];
           wk[i] = k;
 #pragma unroll

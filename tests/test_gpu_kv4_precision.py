@@ -127,3 +127,26 @@ def test_many_small_weights_beside_a_large_one(pkg, hq, hkv, hd, group, gap, typ
         rest = torch.arange(n - count, n, device="cuda", dtype=torch.float64) * torch.exp(-k[first][b, 0, 0].double() * hd ** -0.5)
         want = (rest / (1 + rest))[:, None]
         assert ((rows - want).abs() <= rounded(want * 2.0 ** -9 + n * 2.0 ** -36, want, typ)).all(), (rows / want).aminmax()
+
+
+@pytest.mark.parametrize("hq,hkv,hd,group", [(4, 2, 256, 64), (8, 4, 128, 128), (5, 1, 64, 64)])
+@pytest.mark.parametrize("count", [1, 3])
+def test_small_weights_in_fp32(pkg, hq, hkv, hd, group, count):
+    """As above with random values under the large key, each of weight e^-10.5 (2.8e-5): fp32 rows to 2e-6 in the 2-norm.  ex2 and the two terms
+    of a weight are off by 2^-22 and 2^-22, those below the terms' range by 2^-36 of the largest (5e-7 of these), of which a
+    third of the square is expected in the sum of independent ones: 4e-7, five times allowed."""
+    lens = [9000, 5000]
+    a = Attention(pkg, lens, [count] * 2, hq, hkv, hd, group, torch.float32, seed=1, tail=0)
+    a.q[:] = 0
+    a.q[:, :hq * hd].view(-1, hq, hd)[..., 0] = 1.0
+    seq = torch.cat([torch.full((n,), b, dtype=torch.int32) for b, n in enumerate(lens)]).cuda()
+    pos = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]).cuda()
+    k, v = torch.zeros(len(seq), hkv, hd, device="cuda"), torch.randn(len(seq), hkv, hd, device="cuda", generator=gen(5))
+    first = pos % 100 == 3                                 # each warp meets one
+    k[first, :, 0], v[first] = 10.5 * hd ** 0.5, 0.0
+    a.k, a.v = (x.split(lens) for x in put(pkg, a.cache, seq, pos, k, v))
+    a()
+    for b in range(2):
+        at, want = exact(a, b)
+        err = (a.out[at, :hq * hd].double() - want).view(count, hq, hd).norm(dim=-1)
+        assert (err <= 2e-6 * want.view(count, hq, hd).norm(dim=-1)).all(), (err / want.view(count, hq, hd).norm(dim=-1)).max().item()
