@@ -166,7 +166,9 @@ int B200LmOps_AttentionDecodeStaticStatus(int32_t device, void* stream, int32_t*
 
 /* Waits for `stream`, then reads and clears *status_dev.  OK when the word was
  * zero, InvalidArgument for a bad position, length or page, DeadlineExceeded when
- * a bounded device-side wait gave up; *device_error (optional) receives the word. */
+ * a bounded device-side wait gave up; *device_error (optional) receives the word.
+ * Not for a stream that is being captured.  Calls on other streams need words of
+ * their own: what they add between the read and the clearing would be lost. */
 int B200LmOps_DeviceStatus(int32_t device, void* stream, int32_t* status_dev, int32_t* device_error, char** err);
 
 /* Weights of a grouped int4 product, laid out once on the host.  packed as above
@@ -186,7 +188,8 @@ int B200LmOps_RepackW4Grouped(const uint8_t* packed, const uint16_t* scale, cons
  * 32, 64 or 128 (the last group may be shorter), scale_type B200LM_BF16 or _F16.
  * w_dev is the image above, on a 16-byte boundary.  Sums are in fp32, and x
  * enters exact to 2^-27 of the largest value of a block of 128 (2^-20 with more
- * than four columns of a 16-bit type), of 2^-117 where all of them are smaller; an infinity or NaN in a column makes all of its outputs NaN. */
+ * than four columns of a 16-bit type), of 2^-117 where all of them are smaller; an
+ * infinity or NaN in a column makes all of its outputs NaN. */
 int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_type, int32_t has_offset, int64_t n, int64_t k,
                             int32_t group, const void* x_dev, int32_t x_type, int64_t ldx, int32_t ncols, void* y_dev,
                             int32_t y_type, int64_t ldy, void* stream, char** err);
@@ -199,7 +202,8 @@ int B200LmOps_GemvW4Grouped(int32_t device, const void* w_dev, int32_t scale_typ
  * q_out_dev [tokens] rows of q_stride, keys to k_out_dev rows of k_stride, in
  * qkv's type; they may be the rows' own places.  hd is 64, 128 or 256, rot a
  * multiple of 16 up to hd (0: no rotation; cos_dev and sin_dev are not read).
- * Norms hold over the whole range of the types (sums of squares beyond fp32's are taken in fp64); a row of zeros with eps 0 gives NaN.
+ * Norms hold over the whole range of the types (sums of squares beyond fp32's are
+ * taken in fp64); a row of zeros with eps 0 gives NaN.
  * A token with a negative position is padding: its rows are left alone. */
 int B200LmOps_QkNormRope(int32_t device, const void* qkv_dev, int32_t type, int64_t qkv_stride, int32_t tokens, int32_t hq,
                          int32_t hkv, int32_t hd, int32_t rot, const float* q_gain_dev, const float* k_gain_dev, float eps,
@@ -262,16 +266,20 @@ int B200LmOps_Kv4Read(int32_t device, const B200LmKv4Cache* cache, const int32_t
  * kv_len - n + i, sees the positions up to its own and, with window > 0, the last
  * `window` of those.  A row that sees none gives zeros.  kv_len_dev[b] is at most
  * max_kv, max_kv at most 256 * table_stride.  scale <= 0 means 1/sqrt(hd).  out_dev
- * is of q's type; rows behind the last sequence's are left as they were.  Scores are sums of exact products in fp32, a
- * key's weight, times its scales, enters the second product to 2^-22 (2^-36 of the row's largest where that is more).  bf16 calls with many rows of a kv head (16 and more, head sizes 128
- * and 256) may run on a kernel that rounds weights and values to fp16 for the second product, 2^-11 of each
- * (weights 2^-36 of the row's largest where that is more).
- * A group that stands for NaN makes, in V, its own elements of the rows that see the position NaN, in K those rows.
+ * is of q's type; rows behind the last sequence's are left as they were.
+ *
+ * Scores are sums of exact products in fp32.  A key's weight, times its scales,
+ * enters the second product to 2^-22, or 2^-36 of the row's largest where that is
+ * more.  bf16 calls with many rows of a kv head (16 and more, head sizes 128 and
+ * 256) may run on a kernel that rounds weights and values to fp16 for the second
+ * product, 2^-11 of each (weights 2^-36 of the row's largest where that is more).
+ * A group that stands for NaN makes, in V, its own elements of the rows that see
+ * the position NaN, in K all of those rows.
  *
  * workspace_dev (16-byte boundary) holds the partial results of sequences whose
  * keys are shared out; AttentionKv4Workspace says how many bytes calls up to the
- * given sizes may need (10 MB for single tokens, up to 20 MB for chunks).  Zero it once before its
- * first use; every call leaves the part that has to be zero at zero.  It serves one
+ * given sizes may need (on 148 multiprocessors up to 5 MB for single tokens, 20 MB
+ * for chunks).  Zero it once before its first use; every call leaves the part that has to be zero at zero.  It serves one
  * call at a time: calls, or replays of captured ones, that may overlap need
  * workspaces of their own. */
 int B200LmOps_AttentionKv4Workspace(int32_t device, int32_t batch, int32_t hkv, int32_t hd, int32_t hq, int32_t max_q,

@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kKaThreads, 2) kv4_attn_kernel(const Kv4AttnAr
               const float low = t & 1 ? s1.y : s0.y;
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) {
-                // both digits' sums carry 1.5 * 2^23; every step is exact
+                // both digits' sums carry 1.5 * 2^23; taking that off is exact, the sum of the two is rounded once
                 constexpr float big = 12582912.f * (1.f + 1.f / 128);
                 const float d0 = fmaf(__int_as_float(c[u][nb][1]), 1.f / 128, __int_as_float(c[u][nb][0]) - big);
                 const float d1 = fmaf(__int_as_float(c[u][nb][3]), 1.f / 128, __int_as_float(c[u][nb][2]) - big);
