@@ -17,9 +17,10 @@
 // distributed shared memory: no workspace, a fixed order.  Where a run has fewer strips than warps, kw warps share the blocks
 // of a strip.
 //
-// Measured: 262144 x 1152, groups of 128, two fp32 columns 29.0 us = 5.4 TB/s (84 % of the copy rate), bound by HBM; 20480 x 2560,
-// groups of 64 with offsets, three columns 12.3 us = 2.4 TB/s, bound by one chain of latencies (digits, first blocks, the cluster's
-// meeting) and the last round of strips; 1536 x 1152, one column 3.3 us, a launch.
+// Measured: 262144 x 1152, groups of 128, two fp32 columns 32.2 us = 4.9 TB/s (76 % of the copy rate), bound by HBM (29.0 us where the
+// same 158 MB come again at once, part of them from L2); 20480 x 2560, groups of 64 with offsets, three columns 12.3 us = 2.4 TB/s,
+// bound by one chain of latencies (digits, first blocks, the cluster's meeting) and the last round of strips; 1536 x 1152, one column
+// 3.4 us, a launch; 43008 x 5376, groups of 64, eight bf16 columns 44.8 us = 2.8 TB/s.
 #pragma once
 #include <cuda_fp16.h>
 

@@ -24,9 +24,9 @@
 // A CTA serves RB rows over a share of the keys; shares of a sequence are joined by the last CTA to arrive.  How many
 // keys a share has is decided on the host from the largest length, how many shares a sequence has on the device from its own.
 //
-// What bounds it: issue slots (63 to 67 % busy with 16 warps an SM) and the logic pipe (52 %), not the bytes.  64 sequences of 300 ..
-// 8192 positions, 8 query heads on 4 of 256, bf16: 97.5 us = 3.2 TB/s; three of 40001 .. 65536, 32 on 16 of 128, fp32: 92.9 us =
-// 3.7 TB/s; 16 x 5 rows in a window of 1024: 28.7 us; one sequence of 777 positions: 10.0 us, a chain of latencies with the join.
+// What bounds it: issue slots (65 % busy with 16 warps an SM) and the logic pipe (52 %), not the bytes.  64 sequences of 300 ..
+// 8192 positions, 8 query heads on 4 of 256, bf16: 97.4 us = 3.2 TB/s; three of 40001 .. 65536, 32 on 16 of 128, fp32: 93.7 us =
+// 3.7 TB/s; 16 x 5 rows in a window of 1024: 29.4 us; one sequence of 777 positions: 10.1 us, a chain of latencies with the join.
 // Tiles of 16 keys at head size 256 because two CTAs an SM leave 14 KB of ring a warp: three stages.
 #pragma once
 #include "kv4_rows.cuh"

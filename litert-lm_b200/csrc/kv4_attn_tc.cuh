@@ -19,7 +19,7 @@
 // Order of issue: S(j + 1), then O(j), so that the softmax of a tile runs beside the products of its neighbours.
 // Scores of tile j + 1 may overwrite the probabilities of j - 1 when O(j - 1) is complete.
 //
-// What bounds it: issue slots, most of them the expansion's (every CTA of 128 rows expands its own keys: 64 of them at head size 256
+// What bounds it: issue slots, 57 % busy, and the tensor pipe, 43 %, most of the instructions the expansion's (every CTA of 128 rows expands its own keys: 64 of them at head size 256
 // are 32768 codes), beside it shared memory (96 KB a tile written and read once, 1536 cycles, as long as the products take).
 // Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 139 us = 353 TFLOP/s (21 % of the cuBLAS
 // rate; 108 us with K in one term), the same of head size 128: 75 us (68); the scores' factor inside the exponent instead of

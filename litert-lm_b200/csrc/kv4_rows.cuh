@@ -6,8 +6,8 @@
 //
 // Every byte is read and written once.  What bounds it are issue slots and latencies of the rows' chains, behind them HBM: 8191
 // rows of 8 and 4 heads of 256 in bf16 take 24.7 us = 4.4 TB/s (68 % of the copy rate); 2001 rows of 32 and 16 heads of 128 with
-// their codes 28.6 us, where the bytes take 9 (300 instructions a pass of 256 elements; ALU 45 %, conversions 25 % busy; with
-// registers for 24 warps an SM 28.6 us, unbounded 35); reading them back 9.4 us = 4.5 TB/s; a single token 1.7 us.
+// their codes 29.1 us, where the bytes take 9 (300 instructions a pass of 256 elements; ALU 45 %, conversions 25 % busy; with
+// registers for 24 warps an SM, unbounded a fifth more); reading them back 9.4 us = 3.9 TB/s; a single token 1.9 us.
 //
 // A lane holds eight neighbouring elements, so a pass of a warp takes 1, 2 or 4 heads (of 256, 128, 64); the other halves of the
 // pairs lie at the same place of a lane rot / 16 further and come from there as they lay in memory.  A warp takes up to four
