@@ -128,3 +128,41 @@ def test_last_tiles_that_carry_the_result(pkg, hq, hkv, hd, group):
         a.out.fill_(7.0)
         a()
         check_rows(a)
+
+
+def test_one_workspace_serves_calls_in_turn(pkg):
+    """Chunks, drafted and single tokens of different sizes, one behind the other over one workspace, called and from one graph: each as alone,
+    and the tickets at zero behind every call, bad pages and lengths among them."""
+    makes = [([6000, 40], [128, 40], 8, 4, 256, 64), ([9000], [1], 4, 1, 256, 64), ([9000, 3000], [200, 150], 16, 2, 128, 128), ([700] * 6, [5] * 6, 8, 4, 128, 64), ([20000, 3], [1, 1], 12, 4, 64, 64)]
+    calls = [Attention(pkg, lens, counts, hq, hkv, hd, group, torch.bfloat16, seed=i) for i, (lens, counts, hq, hkv, hd, group) in enumerate(makes)]
+    room = torch.zeros(max(a.need for a in calls), device="cuda", dtype=torch.uint8)
+    alone = []
+    for a in calls:
+        a()
+        alone.append(a.out.clone())
+        a.room, a.need = room, room.numel()
+    for a, want in zip(calls, alone):
+        a.out.fill_(7.0)
+        a()
+        assert torch.equal(a.out, want) and not room[:16384].any()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        for a in calls:
+            a()
+    for _ in range(5):
+        for a in calls:
+            a.out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.out, want) for a, want in zip(calls, alone)) and not room[:16384].any()
+    calls[0].cache.table[0, 20], calls[2].kv_len[1], calls[4].cache.table[0, 70] = -1, 9001, 2 ** 30
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not room[:16384].any()
+    for i in (0, 2, 4):
+        with pytest.raises(pkg.StatusError):
+            pkg.ops.device_status(calls[i].status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(calls[i].out, alone[i])         # the last replay's results stay where they were not written
+    for i in (1, 3):
+        assert torch.equal(calls[i].out, alone[i])

@@ -60,6 +60,30 @@ def test_rows_of_every_size(pkg, hq, hkv, hd, rot, typ, eps):
     assert torch.equal(kg.double()[ok], held(kw.float(), 64)[ok]) and torch.equal(vg.double(), held(v.float(), 64))
 
 
+@pytest.mark.parametrize("hq,hkv,hd,rot", [(4, 1, 256, 256), (8, 4, 128, 64), (5, 3, 64, 64)])
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("t,pad", [(600, 0), (600, 8), (40, 3)])
+def test_many_rows_of_every_size_in_their_own_places(pkg, hq, hkv, hd, rot, typ, t, pad):
+    """Several passes a warp, ordinary heads beside far ones, results over the rows themselves."""
+    r = Rows(t, hq, hkv, hd, rot, typ, pad, seed=hd + rot)
+    sizes = torch.tensor(SIZES, device="cuda", dtype=torch.float64)
+    pick = (torch.arange(t, device="cuda")[:, None] * 5 + torch.arange(hq + 2 * hkv, device="cuda")) % len(SIZES)
+    if typ == torch.float16:
+        sizes = sizes.clamp(1e-4, 1e4)
+    r.rows.copy_((r.rows.double().unflatten(1, (-1, hd)) * sizes[pick][..., None]).flatten(1).to(typ))
+    q, k, v = (x.clone() for x in r.heads())
+    at, args, stride = r.pos.long(), r.args(), r.buf.numel() // t
+    args.update(q_out_dev=r.buf.data_ptr(), q_stride=stride)
+    pkg.ops.qk_norm_rope(k_out_dev=r.buf.data_ptr() + hq * hd * r.buf.element_size(), k_stride=stride, **args)
+    assert pkg.ops.device_status(r.status.data_ptr(), stream()) == 0
+    got_q, got_k, got_v = r.heads()
+    assert torch.equal(got_v, v)
+    for got, x, gain in ((got_q, q, r.q_gain), (got_k, k, r.k_gain)):
+        want = norm_rope(x, gain, r.cos[at], r.sin[at], rot, 1e-6)
+        size = torch.cat([(want[..., :rot // 2].abs() + want[..., rot // 2:rot].abs()).repeat(1, 1, 2), want[..., rot:].abs()], -1) * 1.5
+        close(got, want, typ, size)
+
+
 @pytest.mark.parametrize("rot", [0, 128])
 def test_an_infinity_in_a_key_spoils_its_groups(pkg, rot):
     """The other elements of the head are x / inf = 0; with rotation the element's partner is spoilt too."""
