@@ -6,28 +6,30 @@
 //          sums of q over 64 elements, in two terms (2^-22).  (The halves keep 8 s inside fp16's range.)  Queries are bf16 numbers
 //          times a power of two of their row, exact in fp16 down to 2^-24 of the row's largest.  So a score is as good as
 //          fp32; with K as one fp16 number a score of 50 was off by percents of its key's weight.
-//   O      P and V = s c + m as fp16 numbers, one rounding of 2^-11 each (P times 2^11, so that it is a normal number down to 2^-25 of
-//          its row's reference, and what lies below is off by 2^-36 of that), where storing the bf16 row costs 2^-8 (V in two terms and P in
-//          two would be three products instead of one, and the rows of V would not fit beside those of K).
+//   O      P and V = s c + m as fp16 numbers, one rounding of 2^-11 each, where storing the bf16 row costs 2^-8 (V in two terms and P
+//          in two would be three products instead of one, and the rows of V would not fit beside those of K).  P is held times 2^11:
+//          a normal number down to 2^-25 of its row's reference, and what lies below is off by 2^-36 of that.
 //
 //   the others    expand: codes from global memory a tile ahead, K and V rows into swizzled shared memory (two stages each)
 //   warp 8        issues the products: S = Q K^T with Q in tensor memory (read from shared memory it would take a third of the
-//                 bandwidth that the expanded rows need; the sums of q do come from there), O += P V with P in tensor memory, over the scores it was made from
+//                 bandwidth that the expanded rows need; the sums of q do come from there), O += P V with P in tensor memory, over
+//                 the scores it was made from
 //   warps 0 - 7   softmax, two threads a row (half of the keys, half of O each).  A row's reference moves when a score passes it
 //                 by 4 powers of two; only then is O read, scaled and written back, behind the products of the tile before.
 //
 // Order of issue: S(j + 1), then O(j), so that the softmax of a tile runs beside the products of its neighbours.
 // Scores of tile j + 1 may overwrite the probabilities of j - 1 when O(j - 1) is complete.
 //
-// What bounds it: issue slots, 57 % busy, and the tensor pipe, 43 %, most of the instructions the expansion's (every CTA of 128 rows expands its own keys: 64 of them at head size 256
-// are 32768 codes), beside it shared memory (96 KB a tile written and read once, 1536 cycles, as long as the products take).
+// What bounds it: issue slots, 57 % busy, and the tensor pipe, 43 %; most instructions are the expansion's (every CTA of 128 rows
+// expands its own keys: 64 of them at head size 256 are 32768 codes), beside it shared memory (96 KB a tile written and read once,
+// 1536 cycles, as long as the products take).
 // Two chunks of 512 tokens over 4000 and 8192 positions, 8 query heads on 4 of 256: 139 us = 353 TFLOP/s (21 % of the cuBLAS
 // rate; 108 us with K in one term), the same of head size 128: 75 us (68); the scores' factor inside the exponent instead of
 // beside it took 28 us off, K and V by warps of their own 6.
 //
 // A NaN in a group of K makes the key's scores NaN, so it spoils the rows that see the key and no others.  One of V is noted for
-// those rows, whose dims of the group become NaN at the end; V itself is zero there, as is what no row sees.  All waits are bounded; after one that gave up the CTA's threads run to its end without
-// the products, and the status says so.
+// those rows, whose dims of the group become NaN at the end; V itself is zero there, as is what no row sees.  All waits are bounded;
+// after one that gave up the CTA's threads run to its end without the products, and the status says so.
 #pragma once
 #include "kv4_attn.cuh"
 #include "kv4_chunk_order.h"
@@ -38,7 +40,8 @@
 namespace b200lm {
 
 constexpr int kKcRows = 128, kKcSoft = 256;
-constexpr float kKcLazy = 4.f, kKcRange = 11.f;                      // P <= 2^15: powers of two by which a score may pass its row's reference, and that P is held above it (6 and 9: 135 us instead of 139)
+// Powers of two by which a score may pass its row's reference, and by which P is held above that: P <= 2^15 (6 and 9: 135 us instead of 139).
+constexpr float kKcLazy = 4.f, kKcRange = 11.f;
 
 template <int HD>
 struct KcShape {
